@@ -539,6 +539,79 @@ int32_t sb_gemm(sb_ctx* ctx, const void* d_a, const void* d_w, const float* d_bi
                 const float* d_col_scale, void* d_out, int64_t M, int64_t N, int64_t K, int32_t fp8, int32_t act,
                 int32_t out_mode, float alpha);
 
+/* ------------------------------------------ products whose weights a row chooses */
+
+/* sb_gemm multiplies every row with the same weights.  The entry points of this section are for packed batches whose rows
+ * (encoder frames of many clips and streams) differ in that: rows that go to one of several experts or to the output layer
+ * of their language (sb_route_topk, sb_grouped_gemm, sb_combine_rows), and rows of customers who brought a low-rank
+ * adapter to a shared projection (sb_adapter_gemm).  No counterpart in the reference.
+ * All of them are asynchronous on the context's stream, allocate nothing and may be captured into a CUDA graph; scratch
+ * memory is the caller's (d_work), and calls that may run at the same time need one each.  Sizes and offsets that live in
+ * device memory are not read by the host.  Pointers are device pointers of the context's GPU.  Zero rows are a call
+ * without effect (sb_route_topk still writes its offsets). */
+
+/* Scratch bytes of sb_route_topk and sb_adapter_gemm; 0 for sizes that those refuse. */
+int64_t sb_route_topk_workspace(int64_t rows, int64_t n_experts, int64_t top_k);
+int64_t sb_adapter_gemm_workspace(int64_t M, int64_t rank);
+
+/* The top_k best experts of every row, their weights, and the order that puts the rows of one expert side by side.
+ *   d_logits   [rows x n_experts] f32, or bf16 if logits_bf16; row pitch ld_logits elements
+ *   d_experts  [rows x top_k] the chosen experts, best first, equal logits by the lower index; -1 where a row has fewer than
+ *              top_k logits above -inf (-inf and NaN are never chosen; +inf counts as the largest finite value)
+ *   d_weights  [rows x top_k] f32: softmax over the row's experts (normalize = 0) or over the chosen ones (normalize = 1);
+ *              0 where d_experts is -1
+ *   d_offsets  [n_experts + 1]: the places of expert e are [d_offsets[e], d_offsets[e + 1]), rows in ascending order
+ *   d_order    [rows x top_k]: the row at each place; -1 behind the last one
+ *   d_slots    [rows x top_k]: the place of every choice; -1 where there is none
+ * n_experts <= 1024, top_k <= min(n_experts, 16), rows * top_k < 2^31.  Deterministic. */
+int32_t sb_route_topk(sb_ctx* ctx, const void* d_logits, int32_t logits_bf16, int64_t ld_logits, int64_t rows,
+                      int64_t n_experts, int64_t top_k, int32_t normalize, int32_t* d_experts, float* d_weights,
+                      int32_t* d_offsets, int32_t* d_order, int32_t* d_slots, void* d_work, int64_t work_bytes);
+
+/* Products grouped by expert: for d_offsets[g] <= i < d_offsets[g + 1]
+ *   out[i] = epilogue(A[d_rows[i]] * W[g]^T)           (act, out_mode, alpha as in sb_gemm)
+ *   d_a        [a_rows x K], row pitch lda elements, bf16 (fp8 = 0) or e4m3 (fp8 = 1)
+ *   d_rows     [M] int32: the row of A behind each output row, e.g. d_order of sb_route_topk; NULL: row i behind output row
+ *              i (then a_rows >= M).  An index outside [0, a_rows) stands for a row of zeros.
+ *   d_w        [n_groups x N x K] dense, nn.Linear layout, same type as d_a;  d_bias  [n_groups x N] f32 or NULL
+ *   d_row_scale [a_rows], d_col_scale [n_groups x N] f32 or NULL (fp8 only): result and scales are multiplied before the bias
+ *   d_offsets  [n_groups + 1] int32 in device memory, ascending, at most M: groups may be empty, of any size, and need not
+ *              cover all M rows
+ *   d_out      [M x N], row pitch ldo elements; rows outside the groups are left as they are
+ * Any M, N and n_groups; K a multiple of 8 (bf16) or 16 (fp8).  d_a and d_w on 16-byte boundaries, lda * element size a
+ * multiple of 16.  bf16 results are rounded once from the 32-bit sum; a row's numbers depend neither on its place nor on the
+ * other rows. */
+int32_t sb_grouped_gemm(sb_ctx* ctx, const void* d_a, int64_t lda, int64_t a_rows, const int32_t* d_rows, const void* d_w,
+                        const float* d_bias, const float* d_row_scale, const float* d_col_scale, const int32_t* d_offsets,
+                        int64_t n_groups, void* d_out, int64_t ldo, int64_t M, int64_t N, int64_t K, int32_t fp8,
+                        int32_t act, int32_t out_mode, float alpha);
+
+/* The experts' rows back to one per row: out[t] = alpha * sum_j d_weights[t][j] * y[d_slots[t][j]], summed in 32 bits in the
+ * order of j.
+ *   d_y        [y_rows x cols], row pitch ldy elements, bf16, or f32 if y_f32
+ *   d_slots    [rows x top_k] int32; a slot outside [0, y_rows) adds nothing
+ *   d_weights  [rows x top_k] f32, or NULL for ones
+ *   d_out      [rows x cols], row pitch ldo elements; out_mode 0: bf16, 1: f32, 2: f32 added to */
+int32_t sb_combine_rows(sb_ctx* ctx, const void* d_y, int32_t y_f32, int64_t ldy, int64_t y_rows, const int32_t* d_slots,
+                        const float* d_weights, void* d_out, int64_t ldo, int64_t rows, int64_t top_k, int64_t cols,
+                        int32_t out_mode, float alpha);
+
+/* A shared projection with a low-rank adapter per row: with a = d_row_adapter[i]
+ *   out[i] = epilogue(A[i] * W^T + d_scale[a] * (A[i] * down[a]^T) * up[a]^T)      (bias, act, out_mode, alpha as in sb_gemm)
+ *   d_a        [M x K] bf16, row pitch lda elements;  d_w [N x K] bf16;  d_bias [N] f32 or NULL
+ *   d_down     [n_adapters x rank x K] bf16;  d_up [n_adapters x N x rank] bf16;  d_scale [n_adapters] f32 or NULL for ones
+ *              (adapters of a lower rank: rows of down and columns of up filled up with zeros)
+ *   d_row_adapter [M] int32; an id outside [0, n_adapters) stands for no adapter.  Rows of one adapter need not be
+ *              neighbours, but a run of 128 rows costs a pass over `up` for each adapter in it.
+ *   d_out      [M x N], row pitch ldo elements
+ *   d_work     sb_adapter_gemm_workspace(M, rank) bytes on a 16-byte boundary
+ * Any M, N and n_adapters (n_adapters * N < 2^31); K and rank multiples of 8, rank <= 128; alignment as for sb_grouped_gemm.
+ * Nothing of one adapter, inf and NaN included, reaches rows of another. */
+int32_t sb_adapter_gemm(sb_ctx* ctx, const void* d_a, int64_t lda, const void* d_w, const float* d_bias, const void* d_down,
+                        const void* d_up, const float* d_scale, const int32_t* d_row_adapter, int64_t n_adapters,
+                        int64_t rank, void* d_out, int64_t ldo, int64_t M, int64_t N, int64_t K, int32_t act,
+                        int32_t out_mode, float alpha, void* d_work, int64_t work_bytes);
+
 #ifdef __cplusplus
 }
 #endif

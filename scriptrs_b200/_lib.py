@@ -152,6 +152,14 @@ SIGNATURES = {
     "sb_vad_process": (_I32, [_VP, _VP, _I64, _VP, _I64, C.POINTER(_I64)]),
     "sb_vad_process_device": (_I32, [_VP, _VP, _I64, _VP]),
     "sb_gemm": (_I32, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64, _I32, _I32, _I32, C.c_float]),
+    "sb_route_topk_workspace": (_I64, [_I64, _I64, _I64]),
+    "sb_adapter_gemm_workspace": (_I64, [_I64, _I64]),
+    "sb_route_topk": (_I32, [_VP, _VP, _I32, _I64, _I64, _I64, _I64, _I32, _VP, _VP, _VP, _VP, _VP, _VP, _I64]),
+    "sb_grouped_gemm": (_I32, [_VP, _VP, _I64, _I64, _VP, _VP, _VP, _VP, _VP, _VP, _I64, _VP, _I64, _I64, _I64, _I64, _I32,
+                               _I32, _I32, C.c_float]),
+    "sb_combine_rows": (_I32, [_VP, _VP, _I32, _I64, _I64, _VP, _VP, _VP, _I64, _I64, _I64, _I64, _I32, C.c_float]),
+    "sb_adapter_gemm": (_I32, [_VP, _VP, _I64, _VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _VP, _I64, _I64, _I64, _I64, _I32,
+                               _I32, C.c_float, _VP, _I64]),
 }
 
 

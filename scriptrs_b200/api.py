@@ -167,6 +167,53 @@ def gemm(ctx: Context, d_a: int, d_w: int, d_out: int, M: int, N: int, K: int, d
                              M, N, K, int(fp8), act, out_mode, float(alpha)))
 
 
+def route_topk_workspace(rows: int, n_experts: int, top_k: int) -> int:
+    """Bytes of d_work for route_topk."""
+    return _lib.lib().sb_route_topk_workspace(rows, n_experts, top_k)
+
+
+def adapter_gemm_workspace(M: int, rank: int) -> int:
+    """Bytes of d_work for adapter_gemm."""
+    return _lib.lib().sb_adapter_gemm_workspace(M, rank)
+
+
+def route_topk(ctx: Context, d_logits: int, d_experts: int, d_weights: int, d_offsets: int, d_order: int, d_slots: int,
+               rows: int, n_experts: int, top_k: int, d_work: int, work_bytes: int, ld: int | None = None,
+               bf16: bool = False, normalize: bool = True):
+    """The top_k best experts of every row, their weights, and the rows in the experts' order; device pointers; asynchronous."""
+    check(_lib.lib().sb_route_topk(ctx.handle, d_logits, bf16, n_experts if ld is None else ld, rows, n_experts, top_k,
+                                   normalize, d_experts, d_weights, d_offsets, d_order, d_slots, d_work, work_bytes))
+
+
+def grouped_gemm(ctx: Context, d_a: int, d_w: int, d_out: int, d_offsets: int, n_groups: int, M: int, N: int, K: int,
+                 d_rows: int = 0, a_rows: int | None = None, lda: int | None = None, ldo: int | None = None, d_bias: int = 0,
+                 act: int = 0, out_mode: int = 0, alpha: float = 1.0, fp8: bool = False, d_row_scale: int = 0,
+                 d_col_scale: int = 0):
+    """out[i] = epilogue(A[d_rows[i]] @ W[g]^T) for the rows i of group g; device pointers; asynchronous."""
+    check(_lib.lib().sb_grouped_gemm(ctx.handle, d_a, K if lda is None else lda, M if a_rows is None else a_rows, d_rows,
+                                     d_w, d_bias, d_row_scale, d_col_scale, d_offsets, n_groups, d_out,
+                                     N if ldo is None else ldo, M, N, K, fp8, act, out_mode, alpha))
+
+
+def combine_rows(ctx: Context, d_y: int, d_slots: int, d_weights: int, d_out: int, rows: int, top_k: int, cols: int,
+                 y_rows: int, ldy: int | None = None, ldo: int | None = None, y_f32: bool = False, out_mode: int = 0,
+                 alpha: float = 1.0):
+    """out[t] = alpha * sum_j weights[t, j] * y[slots[t, j]]; device pointers; asynchronous."""
+    check(_lib.lib().sb_combine_rows(ctx.handle, d_y, y_f32, cols if ldy is None else ldy, y_rows, d_slots, d_weights, d_out,
+                                     cols if ldo is None else ldo, rows, top_k, cols, out_mode, alpha))
+
+
+def adapter_gemm(ctx: Context, d_a: int, d_w: int, d_down: int, d_up: int, d_row_adapter: int, d_out: int, n_adapters: int,
+                 rank: int, M: int, N: int, K: int, d_work: int, work_bytes: int, lda: int | None = None,
+                 ldo: int | None = None, d_scale: int = 0, d_bias: int = 0, act: int = 0, out_mode: int = 0,
+                 alpha: float = 1.0):
+    """out[i] = epilogue(A[i] @ W^T + scale[a] * (A[i] @ down[a]^T) @ up[a]^T), a = row_adapter[i]; device pointers;
+    asynchronous."""
+    check(_lib.lib().sb_adapter_gemm(ctx.handle, d_a, K if lda is None else lda, d_w, d_bias, d_down, d_up, d_scale,
+                                     d_row_adapter, n_adapters, rank, d_out, N if ldo is None else ldo, M, N, K, act,
+                                     out_mode, alpha, d_work, work_bytes))
+
+
 def load_model(ctx: Context, weights: dict, encoder_layers: int, scale_input: bool = False,
                has_encoder: bool = True, has_decoder: bool = False, fp8_weights: bool = False):
     """Uploads a dict of named float32 arrays (see sb_model_load for the names)."""

@@ -1,690 +1,32 @@
-// Products whose weights a row chooses, on tcgen05 tensor cores:
-//   grouped:   out[i] = alpha act(s W_e x[rows[i]] + b_e)            for offsets[e] <= i < offsets[e + 1]
-//   adapters:  out[i] = alpha act(W x[i] + U_a low[i] + b)           with the adapter a of row i, low = scale_a D_a x[i]
-//
-// One CTA per SM, warp-specialised like the shared product of gemm.cu: a TMA producer, an MMA issuer (128 rows x BN columns in
-// tensor memory, two accumulators), eight epilogue warps.  What differs:
-//   - The tiles are found on the device.  A tile belongs to one group: 128 consecutive rows of it (the last ones of a group may
-//     be missing) times BN columns.  Every warp walks the offsets 32 groups at a time with a prefix sum over its lanes, so no
-//     table of groups is kept and the host never learns the sizes.
-//   - Rows picked by an index arrive by TMA gathers of four rows each; a tile with few rows fetches only those.
-//   - Rows leave through a swizzled slab per warp and ordinary stores of 16 bytes a lane, predicated by row and column: the rows
-//     after a group's last one belong to its neighbour.
-//   - The low-rank addition is K = rank more columns of the same product, accumulated in the same tensor memory: `low` as two
-//     bf16 terms (hi + lo, 2^-17 of it dropped) against the rows of U_a.  A tile may hold rows of several adapters: its MMAs run
-//     once for each, with the lanes of the other rows disabled, so that nothing of one adapter (not even a NaN) reaches rows of
-//     another, and the shared weights are read once whatever the adapters.
-//   - The tensor core adds into its accumulator by truncation, 1e-6 of the result at K = 1024 and 4.4e-6 at 4096 (measured).
-//     Where the result is stored in 32 bits, it is collected in registers every kSegment columns of K, rounded to nearest.
-// Every wait on an mbarrier is bounded; when one runs out the kernel sets *error, drains, frees its tensor memory and returns.
+// Dispatch of the products whose weights a row chooses (rows_kernel.cuh; one file per form, so that they compile side by side).
 #include <cuda.h>
-#include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-#include <algorithm>
-
 #include "gemm_tile.h"
-#include "launch.cuh"
 #include "rows.h"
-#include "tc_ptx.cuh"
 
 namespace sb {
 
 namespace {
-
-using namespace ptx;
-
-constexpr int kBM = 128;
-constexpr int kRowBytes = 128;  // of an operand row in a stage: one swizzle row
-constexpr int kEpiWarps = 8;
-constexpr int kSlabBytes = 32 * 128;
-constexpr int kSegment = 4;     // stages (64 bf16 or 128 e4m3 columns of K each) between two collections of a 32-bit result
-constexpr int kRankChunk = 32;  // columns of `low` in a stage: 32 hi + 32 lo
-
-enum RowsMode : int { kGrouped = 0, kGathered = 1, kAdapters = 2 };
-
-template <int BN>
-struct RCfg {
-    static constexpr int kStages = BN <= 64 ? 8 : (BN == 256 ? 4 : 6);
-    static constexpr int kHalves = gemm_halves(BN);
-    static constexpr int kHalfCols = BN / kHalves;
-    static constexpr int kABytes = kBM * kRowBytes;
-    static constexpr int kBBytes = BN * kRowBytes;
-    static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kBarBytes = 384;
-    static constexpr int kSmemBytes = kStages * kStageBytes + kEpiWarps * kSlabBytes + kBarBytes + 1024;
-    static constexpr uint32_t kTmemCols = 2 * BN;
-};
-
-constexpr int rows_threads(int mode) { return mode == kAdapters ? 448 : 320; }
-
-template <int BN, bool FP8>
-__device__ __forceinline__ uint32_t rows_idesc() {
-    const uint32_t fmt = FP8 ? 0u : 1u;  // e4m3 / bf16; fp32 accumulate, both operands K-major
-    return (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
-}
-
-// Four rows of the map (box one row high) to four consecutive 128-byte rows.
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int r0, int r1, int r2, int r3) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
-        ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(r0), "r"(r1), "r"(r2), "r"(r3)
-        : "memory");
-}
-// The product is added in the tensor-memory lanes whose bit in `off` is clear.
-__device__ __forceinline__ void tc_mma_lanes(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, const uint32_t (&off)[4]) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, 1, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7}, p;\n\t}"
-        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3])
-        : "memory");
-}
-
-struct RowsParams {
-    const int32_t* rows;
-    const int32_t* offsets;
-    const float* bias;
-    const float* row_scale;
-    const float* col_scale;
-    void* out;
-    int64_t a_rows, ldo;
-    int M, N, K, n_groups, act, out_mode;
-    float alpha;
-    bool out_vec;    // output rows on 16-byte boundaries
-    bool bias_vec;   // bias and column scales of every group on 16-byte boundaries
-    // adapters
-    const int32_t* row_adapter;
-    const float* low;
-    const int32_t* lists;
-    int rank;
-};
-
-// A tile: rows [row0, row1) of the output, columns from col0, weights of group `group`.
-struct RowsTile {
-    int group, row0, row1, col0;
-};
-
-// Finds tile t.  All lanes of a warp call it together, with ascending t.
-struct TileWalk {
-    const int32_t* offsets;
-    int M, n_groups, n_tiles, lane;
-    int first_group;      // of the 32 groups that the lanes hold
-    long long first_tile; // tiles of the groups before them
-    int lo, hi, upto;     // this lane's group: rows, tiles of the groups up to and including it
-    int total;            // tiles of the 32 groups
-
-    __device__ __forceinline__ TileWalk(const int32_t* off, int m, int groups, int nt, int ln)
-        : offsets(off), M(m), n_groups(groups), n_tiles(nt), lane(ln), first_group(0), first_tile(0) {
-        load();
-    }
-    __device__ __forceinline__ void load() {
-        const int g = first_group + lane;
-        lo = hi = 0;
-        if (g < n_groups) {
-            // whatever the offsets hold, rows stay inside [0, M)
-            lo = offsets ? min(max(__ldg(offsets + g), 0), M) : 0;
-            hi = offsets ? max(min(__ldg(offsets + g + 1), M), lo) : M;
-        }
-        upto = (int)(((long long)(hi - lo) + kBM - 1) / kBM) * n_tiles;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, upto, d);
-            if (lane >= d) upto += v;
-        }
-        total = __shfl_sync(0xffffffffu, upto, 31);
-    }
-    __device__ __forceinline__ bool find(long long t, int bn, RowsTile& out) {
-        while (t >= first_tile + total) {
-            if (first_group + 32 >= n_groups) return false;
-            first_tile += total;
-            first_group += 32;
-            load();
-        }
-        const int r = (int)(t - first_tile);
-        const int src = __ffs(__ballot_sync(0xffffffffu, upto > r)) - 1;
-        const int before = src ? __shfl_sync(0xffffffffu, upto, src ? src - 1 : 0) : 0;
-        const int glo = __shfl_sync(0xffffffffu, lo, src), ghi = __shfl_sync(0xffffffffu, hi, src);
-        const int mt = (r - before) / n_tiles, nt = (r - before) % n_tiles;
-        out.group = first_group + src;
-        out.row0 = glo + mt * kBM;
-        out.row1 = min(ghi, out.row0 + kBM);
-        out.col0 = nt * bn;
-        return true;
-    }
-};
-
-__device__ __forceinline__ float rows_act(float x, int act) {
-    if (act == kActSilu) return __fdividef(x, 1.0f + __expf(-x));
-    return act == kActRelu ? fmaxf(x, 0.0f) : x;
-}
-
-// 32 accumulator columns -> scales, bias, activation.
-template <bool FP8>
-__device__ __forceinline__ void rows_finish(float (&x)[32], const RowsParams& p, int group, int col0, float rs, bool known) {
-    const int64_t at = (int64_t)group * p.N + col0;
-    if (!known) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) x[j] = 0.0f;
-    }
-    if (p.bias_vec) {
-#pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-            if (col0 + j >= p.N) break;
-            if (FP8) {
-                const float4 cs = p.col_scale ? __ldg(reinterpret_cast<const float4*>(p.col_scale + at + j)) : make_float4(1.f, 1.f, 1.f, 1.f);
-                x[j] *= rs * cs.x; x[j + 1] *= rs * cs.y; x[j + 2] *= rs * cs.z; x[j + 3] *= rs * cs.w;
-            }
-            if (p.bias) {
-                const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + at + j));
-                x[j] += b.x; x[j + 1] += b.y; x[j + 2] += b.z; x[j + 3] += b.w;
-            }
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            if (col0 + j >= p.N) break;
-            if (FP8) x[j] *= rs * (p.col_scale ? __ldg(p.col_scale + at + j) : 1.0f);
-            if (p.bias) x[j] += __ldg(p.bias + at + j);
-        }
-    }
-    if (p.act != kActNone) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) x[j] = rows_act(x[j], p.act);
-    }
-}
-
-// The slab's 32 rows x COLS columns to memory, the rows below row1 and the columns below N.
-template <typename T, int COLS>
-__device__ __forceinline__ void rows_store(const unsigned char* slab, const RowsParams& p, int row0, int row1, int col0, int lane) {
-    constexpr int kBytes = COLS * (int)sizeof(T), kChunks = kBytes / 16, kPer = 16 / (int)sizeof(T), kStep = 32 / kChunks;
-    constexpr int kShift = kBytes == 64 ? 1 : 0, kMask = kChunks - 1;
-    T* out = static_cast<T*>(p.out);
-    const bool add = sizeof(T) == 4 && p.out_mode == kOutResidual;
-    if (p.out_vec) {
-        const int ch = lane % kChunks, col = col0 + ch * kPer;
-#pragma unroll
-        for (int i = 0; i < 32; i += kStep) {
-            const int r = i + lane / kChunks;
-            if (row0 + r >= row1 || col >= p.N) continue;
-            const uint4 v = *reinterpret_cast<const uint4*>(slab + r * kBytes + ((ch ^ ((r >> kShift) & kMask)) << 4));
-            T* dst = out + (int64_t)(row0 + r) * p.ldo + col;
-            if (col + kPer <= p.N) {
-                if constexpr (sizeof(T) == 4) {
-                    float4 f = make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
-                    if (add) {
-                        const float4 o = *reinterpret_cast<const float4*>(dst);
-                        f = make_float4(o.x + f.x, o.y + f.y, o.z + f.z, o.w + f.w);
-                    }
-                    *reinterpret_cast<float4*>(dst) = f;
-                } else {
-                    *reinterpret_cast<uint4*>(dst) = v;
-                }
-            } else {
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int j = 0; j < kPer; ++j) {
-                    if (col + j >= p.N) break;
-                    if constexpr (sizeof(T) == 4) dst[j] = __uint_as_float(w[j]) + (add ? dst[j] : 0.0f);
-                    else dst[j] = __ushort_as_bfloat16((unsigned short)(w[j / 2] >> (16 * (j & 1))));
-                }
-            }
-        }
-    } else {
-        for (int r = 0; r < 32 && row0 + r < row1; ++r) {
-#pragma unroll
-            for (int c = 0; c < COLS; c += 32) {
-                const int cc = c + lane;
-                if (col0 + cc >= p.N) continue;
-                const int byte = cc * (int)sizeof(T);
-                const T v = *reinterpret_cast<const T*>(slab + r * kBytes + (((byte >> 4) ^ ((r >> kShift) & kMask)) << 4) + (byte & 15));
-                T* dst = out + (int64_t)(row0 + r) * p.ldo + col0 + cc;
-                if constexpr (sizeof(T) == 4) *dst = add ? *dst + v : v;
-                else *dst = v;
-            }
-        }
-    }
-}
-
-__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-    __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&v);
-}
-
-template <int BN, bool FP8, int MODE, bool F32>
-__global__ void __launch_bounds__(rows_threads(MODE), 1)
-rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_w,
-            const __grid_constant__ CUtensorMap tma_up, const RowsParams p, int* __restrict__ error) {
-    using C = RCfg<BN>;
-    constexpr int S = C::kStages;
-    constexpr int kStepCols = FP8 ? 128 : 64;
-    extern __shared__ unsigned char smem_dyn[];
-    const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
-    unsigned char* base_ptr = smem_dyn + (base - smem_u32(smem_dyn));
-    const uint32_t a_base = base, b_base = base + S * C::kABytes;
-    const uint32_t bar_base = base + S * C::kStageBytes + kEpiWarps * kSlabBytes;
-    auto full_bar = [&](int s) { return bar_base + 8u * s; };
-    auto empty_bar = [&](int s) { return bar_base + 8u * (S + s); };
-    auto go_bar = [&](int s) { return bar_base + 8u * (2 * S + s); };        // slot free for `low`
-    auto low_bar = [&](int s) { return bar_base + 8u * (3 * S + s); };       // `low` is there
-    auto tfull_bar = [&](int a) { return bar_base + 8u * (4 * S + a); };
-    auto tempty_bar = [&](int a) { return bar_base + 8u * (4 * S + 2 + a); };
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + S * C::kStageBytes + kEpiWarps * kSlabBytes + 8 * (4 * S + 4));
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-
-    const int warp = warp_index(), lane = threadIdx.x & 31;
-    const int n_tiles = (p.N + BN - 1) / BN;
-    const int k_tiles = (p.K + kStepCols - 1) / kStepCols;
-    const int rank_chunks = MODE == kAdapters ? (p.rank + kRankChunk - 1) / kRankChunk : 0;
-
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < S; ++s) {
-            mbar_init(full_bar(s), 1);
-            mbar_init(empty_bar(s), 1);
-            mbar_init(go_bar(s), 1);
-            mbar_init(low_bar(s), 4);
-        }
-        for (int a = 0; a < 2; ++a) {
-            mbar_init(tfull_bar(a), 1);
-            mbar_init(tempty_bar(a), 4 * C::kHalves);
-        }
-        *abort_flag = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    if (warp == 1) {
-        tmem_alloc(smem_u32(tmem_slot), C::kTmemCols);
-        tmem_relinquish();
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem_base = *tmem_slot;
-    pdl_trigger();
-    // The adapters' kernel ahead in the stream waits for everything before it and lets this one start after that: only what
-    // it writes itself (low, lists) has to be waited for here, by the warps that read it.
-    if (MODE != kAdapters) pdl_wait();
-    bool waited = false;
-
-    TileWalk walk(MODE == kAdapters ? nullptr : p.offsets, p.M, MODE == kAdapters ? 1 : p.n_groups, n_tiles, lane);
-    RowsTile tile;
-
-    if (warp == 0) {
-        // ------------------------------------------------------------ producer
-        int stage = 0;
-        uint32_t ph = 0;
-        bool ok = true;
-        for (long long t = blockIdx.x; ok && walk.find(t, BN, tile); t += gridDim.x) {
-            const int w_row = tile.group * p.N + tile.col0;
-            if constexpr (MODE == kGathered) {
-                const int count = tile.row1 - tile.row0, quads = (count + 3) >> 2;
-                int r[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int i = min(tile.row0 + 4 * lane + j, tile.row1 - 1);
-                    const int v = p.rows ? __ldg(p.rows + i) : i;
-                    r[j] = (unsigned)v < (unsigned long long)p.a_rows ? v : 0;
-                }
-                for (int kt = 0; kt < k_tiles; ++kt) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(empty_bar(stage), ph ^ 1, abort_flag));
-                    if (!ok) break;
-                    if (elect_one()) {
-                        mbar_expect_tx(full_bar(stage), (uint32_t)(C::kBBytes + quads * 4 * kRowBytes));
-                        tma_load_2d(b_base + stage * C::kBBytes, &tma_w, full_bar(stage), kt * kStepCols, w_row);
-                    }
-                    __syncwarp();
-                    if (lane < quads)
-                        tma_gather4(a_base + stage * C::kABytes + lane * 4 * kRowBytes, &tma_a, full_bar(stage), kt * kStepCols, r[0], r[1], r[2], r[3]);
-                    __syncwarp();
-                    if (++stage == S) { stage = 0; ph ^= 1; }
-                }
-            } else {
-                bool failed = false;
-                if (elect_one()) {
-                    int s = stage;
-                    uint32_t sp = ph;
-                    for (int kt = 0; kt < k_tiles; ++kt) {
-                        if (!mbar_wait(empty_bar(s), sp ^ 1, abort_flag)) { failed = true; break; }
-                        mbar_expect_tx(full_bar(s), C::kStageBytes);
-                        tma_load_2d(a_base + s * C::kABytes, &tma_a, full_bar(s), kt * kStepCols, tile.row0);
-                        tma_load_2d(b_base + s * C::kBBytes, &tma_w, full_bar(s), kt * kStepCols, w_row);
-                        if (++s == S) { s = 0; sp ^= 1; }
-                    }
-                }
-                ok = !__any_sync(0xffffffffu, failed);
-                stage += k_tiles;
-                ph ^= (uint32_t)(stage / S) & 1u;
-                stage %= S;
-                if constexpr (MODE == kAdapters) {
-                    if (!waited) { pdl_wait(); waited = true; }
-                    const int32_t* list = p.lists + (int64_t)(tile.row0 / kBM) * kAdapterListInts;
-                    const int count = list[0];
-                    for (int j = 0; ok && j < count; ++j) {
-                        const int u_row = list[4 + j] * p.N + tile.col0;
-                        for (int c = 0; c < rank_chunks; ++c) {
-                            ok = __all_sync(0xffffffffu, mbar_wait(empty_bar(stage), ph ^ 1, abort_flag));
-                            if (!ok) break;
-                            if (elect_one()) {
-                                mbar_arrive(go_bar(stage));
-                                mbar_expect_tx(full_bar(stage), C::kBBytes);
-                                tma_load_2d(b_base + stage * C::kBBytes, &tma_up, full_bar(stage), c * kRankChunk, u_row);
-                            }
-                            __syncwarp();
-                            if (++stage == S) { stage = 0; ph ^= 1; }
-                        }
-                    }
-                }
-            }
-        }
-        if (!ok) {
-            // copies already in flight land before the CTA exits
-            const long long t0 = clock64();
-            while (clock64() - t0 < 2000000) {}
-        }
-    } else if (warp == 1) {
-        // ------------------------------------------------------------ MMA issuer
-        const uint32_t idesc = rows_idesc<BN, FP8>();
-        int stage = 0;
-        uint32_t ph = 0, seg = 0, low_ph = 0;
-        bool ok = true;
-        for (long long t = blockIdx.x; ok && walk.find(t, BN, tile); t += gridDim.x) {
-            int kt = 0;
-            while (ok && kt < k_tiles) {
-                const int acc = seg & 1;
-                const uint32_t d_tmem = tmem_base + acc * BN;
-                const int kt_end = F32 ? min(kt + kSegment, k_tiles) : k_tiles;
-                const bool last = kt_end == k_tiles;
-                bool failed = false;
-                if (elect_one()) {
-                    int s = stage;
-                    uint32_t sp = ph;
-                    if (!mbar_wait(tempty_bar(acc), ((seg >> 1) & 1) ^ 1, abort_flag)) failed = true;
-                    tc_fence_after();
-                    for (int k = kt; k < kt_end && !failed; ++k) {
-                        if (!mbar_wait(full_bar(s), sp, abort_flag)) { failed = true; break; }
-                        tc_fence_after();
-                        const uint64_t adesc = make_smem_desc(a_base + s * C::kABytes), bdesc = make_smem_desc(b_base + s * C::kBBytes);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) tc_mma<FP8>(d_tmem, adesc + 2 * i, bdesc + 2 * i, idesc, (k > kt || i) ? 1u : 0u);
-                        tc_commit(empty_bar(s));
-                        if (++s == S) { s = 0; sp ^= 1; }
-                    }
-                    if (!failed && (MODE != kAdapters || !last)) tc_commit(tfull_bar(acc));
-                }
-                ok = !__any_sync(0xffffffffu, failed);
-                stage += kt_end - kt;
-                ph ^= (uint32_t)(stage / S) & 1u;
-                stage %= S;
-                if constexpr (MODE == kAdapters) {
-                    if (ok && last) {
-                        if (!waited) { pdl_wait(); waited = true; }
-                        const int32_t* list = p.lists + (int64_t)(tile.row0 / kBM) * kAdapterListInts;
-                        const int count = list[0];
-                        int mine[4];
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const int row = tile.row0 + q * 32 + lane;
-                            mine[q] = row < tile.row1 ? __ldg(p.row_adapter + row) : -1;
-                        }
-                        for (int j = 0; ok && j < count; ++j) {
-                            const int id = list[4 + j];
-                            uint32_t off[4];
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) off[q] = ~__ballot_sync(0xffffffffu, mine[q] == id);
-                            for (int c = 0; c < rank_chunks; ++c) {
-                                ok = __all_sync(0xffffffffu, mbar_wait(full_bar(stage), ph, abort_flag) &&
-                                                                 mbar_wait(low_bar(stage), (low_ph >> stage) & 1u, abort_flag));
-                                if (!ok) break;
-                                tc_fence_after();
-                                if (elect_one()) {
-                                    const uint64_t adesc = make_smem_desc(a_base + stage * C::kABytes);
-                                    const uint64_t bdesc = make_smem_desc(b_base + stage * C::kBBytes);
-                                    for (int i = 0; i * 16 < min(kRankChunk, p.rank - c * kRankChunk); ++i) {
-                                        tc_mma_lanes(d_tmem, adesc + 2 * i, bdesc + 2 * i, idesc, off);
-                                        tc_mma_lanes(d_tmem, adesc + 4 + 2 * i, bdesc + 2 * i, idesc, off);
-                                    }
-                                    tc_commit(empty_bar(stage));
-                                }
-                                __syncwarp();
-                                low_ph ^= 1u << stage;
-                                if (++stage == S) { stage = 0; ph ^= 1; }
-                            }
-                        }
-                        if (ok && elect_one()) tc_commit(tfull_bar(acc));
-                        __syncwarp();
-                    }
-                }
-                kt = kt_end;
-                ++seg;
-            }
-        }
-    } else if (warp < 2 + kEpiWarps) {
-        // ------------------------------------------------------------ epilogue
-        const int ew = warp - 2, quad = warp & 3, half = ew >> 2;
-        unsigned char* slab = base_ptr + S * C::kStageBytes + ew * kSlabBytes;
-        uint32_t seg = 0;
-        bool ok = true;
-        for (long long t = blockIdx.x; half < C::kHalves && ok && walk.find(t, BN, tile); t += gridDim.x) {
-            const int row = tile.row0 + quad * 32 + lane;
-            const bool live = row < tile.row1;
-            int src = row;
-            if (MODE == kGathered && p.rows && live) src = __ldg(p.rows + row);
-            const bool known = MODE != kGathered || (unsigned)src < (unsigned long long)p.a_rows;
-            const float rs = FP8 && p.row_scale && live && known ? __ldg(p.row_scale + src) : 1.0f;
-            const int cbeg = half * C::kHalfCols;
-            const bool wide = tile.row0 + quad * 32 < tile.row1;  // rows of this warp in the tile
-            auto taddr = [&]() { return tmem_base + ((uint32_t)(quad * 32) << 16) + (seg & 1) * BN + cbeg; };
-            auto release = [&]() {
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(tempty_bar(seg & 1));
-                ++seg;
-            };
-            if constexpr (F32) {
-                constexpr int kCols = C::kHalfCols;
-                float sum[kCols];
-#pragma unroll
-                for (int j = 0; j < kCols; ++j) sum[j] = 0.0f;
-                for (int kt = 0; kt < k_tiles; kt += kSegment) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(tfull_bar(seg & 1), (seg >> 1) & 1, abort_flag));
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (wide) {
-#pragma unroll
-                        for (int c = 0; c < kCols; c += 32) {
-                            uint32_t v[32];
-                            tmem_ld32(taddr() + c, v);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) sum[c + j] += __uint_as_float(v[j]);
-                        }
-                    }
-                    release();
-                }
-                if (!ok) break;
-                if (!wide) continue;
-#pragma unroll
-                for (int c = 0; c < kCols; c += 32) {
-                    const int col0 = tile.col0 + cbeg + c;
-                    if (col0 >= p.N) break;
-                    float x[32];
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) x[j] = sum[c + j];
-                    rows_finish<FP8>(x, p, tile.group, col0, rs, known);
-#pragma unroll
-                    for (int q = 0; q < 8; ++q)
-                        *reinterpret_cast<float4*>(slab + lane * 128 + ((q ^ (lane & 7)) << 4)) =
-                            make_float4(p.alpha * x[4 * q], p.alpha * x[4 * q + 1], p.alpha * x[4 * q + 2], p.alpha * x[4 * q + 3]);
-                    __syncwarp();
-                    rows_store<float, 32>(slab, p, tile.row0 + quad * 32, tile.row1, col0, lane);
-                    __syncwarp();
-                }
-            } else {
-                constexpr int kCols = C::kHalfCols < 64 ? C::kHalfCols : 64;
-                constexpr int kShift = kCols == 32 ? 1 : 0, kMask = kCols / 8 - 1;
-                ok = __all_sync(0xffffffffu, mbar_wait(tfull_bar(seg & 1), (seg >> 1) & 1, abort_flag));
-                if (!ok) break;
-                tc_fence_after();
-                if (wide) {
-#pragma unroll 1
-                    for (int c = 0; c < C::kHalfCols; c += kCols) {
-                        const int col0 = tile.col0 + cbeg + c;
-                        if (col0 >= p.N) break;
-#pragma unroll
-                        for (int sub = 0; sub < kCols / 32; ++sub) {
-                            uint32_t v[32];
-                            tmem_ld32(taddr() + c + 32 * sub, v);
-                            tmem_wait_ld();
-                            float x[32];
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) x[j] = __uint_as_float(v[j]);
-                            rows_finish<FP8>(x, p, tile.group, col0 + 32 * sub, rs, known);
-#pragma unroll
-                            for (int q = 0; q < 4; ++q)
-                                *reinterpret_cast<uint4*>(slab + lane * (kCols * 2) + (((4 * sub + q) ^ ((lane >> kShift) & kMask)) << 4)) =
-                                    make_uint4(pack_bf16(x[8 * q], x[8 * q + 1]), pack_bf16(x[8 * q + 2], x[8 * q + 3]),
-                                               pack_bf16(x[8 * q + 4], x[8 * q + 5]), pack_bf16(x[8 * q + 6], x[8 * q + 7]));
-                        }
-                        __syncwarp();
-                        rows_store<__nv_bfloat16, kCols>(slab, p, tile.row0 + quad * 32, tile.row1, col0, lane);
-                        __syncwarp();
-                    }
-                }
-                release();
-            }
-        }
-    } else if constexpr (MODE == kAdapters) {
-        // ------------------------------------------------------------ `low` into the ring, a row per thread
-        const int r = (warp - 2 - kEpiWarps) * 32 + lane;
-        int stage = 0;
-        uint32_t go_ph = 0;
-        bool ok = true;
-        pdl_wait();
-        for (long long t = blockIdx.x; ok && walk.find(t, BN, tile); t += gridDim.x) {
-            stage = (stage + k_tiles) % S;
-            const int count = p.lists[(int64_t)(tile.row0 / kBM) * kAdapterListInts];
-            const int row = tile.row0 + r;
-            uint32_t hi[kRankChunk / 2], lo[kRankChunk / 2];
-            int held = -1;  // chunk in the registers
-            for (int j = 0; ok && j < count; ++j) {
-                for (int c = 0; c < rank_chunks; ++c) {
-                    if (held != c) {
-                        held = c;
-#pragma unroll
-                        for (int i = 0; i < kRankChunk; i += 4) {
-                            float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-                            if (row < tile.row1 && c * kRankChunk + i < p.rank)
-                                f = *reinterpret_cast<const float4*>(p.low + (int64_t)row * p.rank + c * kRankChunk + i);
-                            hi[i / 2] = pack_bf16(f.x, f.y);
-                            hi[i / 2 + 1] = pack_bf16(f.z, f.w);
-                            // what the first term leaves; nothing where it is not finite (inf - inf)
-                            auto rest = [](float v) {
-                                const float d = v - __bfloat162float(__float2bfloat16_rn(v));
-                                return fabsf(d) < INFINITY ? d : 0.0f;
-                            };
-                            lo[i / 2] = pack_bf16(rest(f.x), rest(f.y));
-                            lo[i / 2 + 1] = pack_bf16(rest(f.z), rest(f.w));
-                        }
-                    }
-                    ok = __all_sync(0xffffffffu, mbar_wait(go_bar(stage), (go_ph >> stage) & 1u, abort_flag));
-                    if (!ok) break;
-                    unsigned char* dst = base_ptr + stage * C::kABytes + r * kRowBytes;
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        *reinterpret_cast<uint4*>(dst + ((q ^ (r & 7)) << 4)) = make_uint4(hi[4 * q], hi[4 * q + 1], hi[4 * q + 2], hi[4 * q + 3]);
-                        *reinterpret_cast<uint4*>(dst + (((4 + q) ^ (r & 7)) << 4)) = make_uint4(lo[4 * q], lo[4 * q + 1], lo[4 * q + 2], lo[4 * q + 3]);
-                    }
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(low_bar(stage));
-                    go_ph ^= 1u << stage;
-                    if (++stage == S) stage = 0;
-                }
-            }
-        }
-    }
-
-    tc_fence_before();
-    __syncthreads();
-    if (warp == 1) {
-        tc_fence_after();
-        tmem_dealloc(tmem_base, C::kTmemCols);
-    }
-    if (threadIdx.x == 0 && *abort_flag) atomicExch(error, 1);
-}
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeTiledFn g_rows_encode = nullptr;
 
-// 2-D row-major tensor; boxes of 128 bytes x box_rows, 128-byte swizzle.
+}  // namespace
+
 bool rows_map(CUtensorMap* map, const void* ptr, int64_t rows, int64_t cols, int64_t pitch, bool fp8, int box_rows) {
     const int eb = fp8 ? 1 : 2;
     const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
     const cuuint64_t strides[1] = {(cuuint64_t)pitch * eb};
-    const cuuint32_t box[2] = {(cuuint32_t)(kRowBytes / eb), (cuuint32_t)box_rows};
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / eb), (cuuint32_t)box_rows};
     const cuuint32_t estr[2] = {1, 1};
     return g_rows_encode(map, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides,
                          box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-
-template <int BN, bool FP8, int MODE, bool F32>
-cudaError_t rows_launch_t(const RowsArgs& g, int sm_count, int* d_error, cudaStream_t stream) {
-    alignas(64) CUtensorMap ma, mw, mu;
-    if (!rows_map(&ma, g.a, g.a_rows, g.K, g.lda, FP8, MODE == kGathered ? 1 : kBM) ||
-        !rows_map(&mw, g.w, (int64_t)g.n_groups * g.N, g.K, g.K, FP8, BN))
-        return cudaErrorInvalidValue;
-    mu = mw;
-    if (MODE == kAdapters && !rows_map(&mu, g.up, (int64_t)g.n_adapters * g.N, g.rank, g.rank, false, BN)) return cudaErrorInvalidValue;
-    const int eb = F32 ? 4 : 2;
-    RowsParams p{};
-    p.rows = g.rows; p.offsets = g.offsets; p.bias = g.bias; p.row_scale = g.row_scale; p.col_scale = g.col_scale; p.out = g.out;
-    p.a_rows = g.a_rows; p.ldo = g.ldo; p.M = g.M; p.N = g.N; p.K = g.K; p.n_groups = g.n_groups; p.act = g.act; p.out_mode = g.out_mode;
-    p.alpha = g.alpha;
-    p.out_vec = !(reinterpret_cast<uintptr_t>(g.out) & 15) && !((g.ldo * eb) & 15);
-    p.bias_vec = g.N % 4 == 0 && !((reinterpret_cast<uintptr_t>(g.bias) | reinterpret_cast<uintptr_t>(g.col_scale)) & 15);
-    p.row_adapter = g.row_adapter; p.low = g.low; p.lists = g.lists; p.rank = g.rank;
-    // at most this many tiles: a group's last one may be short
-    const int64_t n_tiles = (g.N + BN - 1) / BN;
-    const int64_t tiles = ((int64_t)(g.M + kBM - 1) / kBM + std::min(g.n_groups - 1, g.M)) * n_tiles;
-    const int grid = (int)std::min<int64_t>(tiles, sm_count);
-    return launch_pdl(rows_kernel<BN, FP8, MODE, F32>, dim3(grid), rows_threads(MODE), RCfg<BN>::kSmemBytes, stream, 1, ma, mw, mu, p, d_error);
-}
-
-template <int BN, bool FP8, int MODE, bool F32>
-cudaError_t rows_set() {
-    return cudaFuncSetAttribute(rows_kernel<BN, FP8, MODE, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, RCfg<BN>::kSmemBytes);
-}
-
-template <bool FP8, int MODE>
-cudaError_t rows_pick(const RowsArgs& g, int bn, bool f32, int sm_count, int* err, cudaStream_t st) {
-    if (f32) {
-        switch (bn) {
-            case 32: return rows_launch_t<32, FP8, MODE, true>(g, sm_count, err, st);
-            case 64: return rows_launch_t<64, FP8, MODE, true>(g, sm_count, err, st);
-            default: return rows_launch_t<128, FP8, MODE, true>(g, sm_count, err, st);
-        }
-    }
-    switch (bn) {
-        case 32: return rows_launch_t<32, FP8, MODE, false>(g, sm_count, err, st);
-        case 64: return rows_launch_t<64, FP8, MODE, false>(g, sm_count, err, st);
-        case 128: return rows_launch_t<128, FP8, MODE, false>(g, sm_count, err, st);
-        default: return rows_launch_t<256, FP8, MODE, false>(g, sm_count, err, st);
-    }
-}
-
-template <bool FP8, int MODE>
-cudaError_t rows_set_all() {
-    const cudaError_t e[7] = {rows_set<32, FP8, MODE, true>(),  rows_set<64, FP8, MODE, true>(),   rows_set<128, FP8, MODE, true>(),
-                              rows_set<32, FP8, MODE, false>(), rows_set<64, FP8, MODE, false>(),  rows_set<128, FP8, MODE, false>(),
-                              rows_set<256, FP8, MODE, false>()};
-    for (cudaError_t x : e)
-        if (x != cudaSuccess) return x;
-    return cudaSuccess;
-}
-
-}  // namespace
 
 cudaError_t rows_configure(const char** why) {
     if (!g_rows_encode) {
@@ -697,27 +39,28 @@ cudaError_t rows_configure(const char** why) {
         }
         g_rows_encode = reinterpret_cast<EncodeTiledFn>(fn);
     }
-    const cudaError_t e[5] = {rows_set_all<false, kGrouped>(), rows_set_all<false, kGathered>(), rows_set_all<false, kAdapters>(),
-                              rows_set_all<true, kGrouped>(), rows_set_all<true, kGathered>()};
-    for (cudaError_t x : e) {
-        if (x != cudaSuccess) {
+    for (cudaError_t (*set)() : {rows_grouped_configure, rows_gathered_configure, rows_adapters_configure}) {
+        const cudaError_t e = set();
+        if (e != cudaSuccess) {
             if (why) *why = "shared-memory opt-in for the row products failed";
-            return x;
+            return e;
         }
     }
     return cudaSuccess;
 }
 
+RowsTileShape rows_shape(const RowsArgs& g, int sm_count) {
+    return rows_tile(g.M, g.N, g.row_adapter ? 1 : g.n_groups, g.out_mode != kOutBf16, sm_count);
+}
+
 cudaError_t rows_launch(const RowsArgs& g, int sm_count, int* d_error, cudaStream_t stream) {
     if (!g_rows_encode) return cudaErrorNotReady;
     if (g.M <= 0) return cudaSuccess;
-    const bool f32 = g.out_mode != kOutBf16;
-    const int bn = rows_tile(g.M, g.N, g.n_groups, f32, sm_count);
-    if (g.row_adapter) return rows_pick<false, kAdapters>(g, bn, f32, sm_count, d_error, stream);
+    const RowsTileShape t = rows_shape(g, sm_count);
+    if (g.row_adapter) return rows_adapters_launch(g, t, sm_count, d_error, stream);
     // few rows a group: gathers fetch only those, a box always 128
-    const bool gather = g.rows || (int64_t)g.M < (int64_t)g.n_groups * 64;
-    if (g.fp8) return gather ? rows_pick<true, kGathered>(g, bn, f32, sm_count, d_error, stream) : rows_pick<true, kGrouped>(g, bn, f32, sm_count, d_error, stream);
-    return gather ? rows_pick<false, kGathered>(g, bn, f32, sm_count, d_error, stream) : rows_pick<false, kGrouped>(g, bn, f32, sm_count, d_error, stream);
+    if (g.rows || (int64_t)g.M < (int64_t)g.n_groups * 64) return rows_gathered_launch(g, t, sm_count, d_error, stream);
+    return rows_grouped_launch(g, t, sm_count, d_error, stream);
 }
 
 }  // namespace sb

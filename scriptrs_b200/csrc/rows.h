@@ -1,6 +1,7 @@
 // Products whose weights a row chooses: grouped products (rows.cu), the adapters' down-projection (adapter_down.cu), and
 // the router with the weighted sum of the experts' rows (route.cu).
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -26,14 +27,25 @@ struct RowsArgs {
     const int32_t* row_adapter;  // [M], ids outside [0, n_adapters): none; null: no adapters
     const void* up;              // [n_adapters x N x rank] bf16
     const float* low;            // [M x rank] f32, scaled; written by the kernel ahead in the stream
-    const int32_t* lists;        // per 128 rows: number of adapters, their ids in the order of their first rows
+    const int32_t* lists;        // per tile's rows: number of adapters, their ids in the order of their first rows
     int n_adapters, rank;
 };
-constexpr int kAdapterListInts = 132;  // a count, padding to 16 bytes, 128 ids
+constexpr int kAdapterListInts = 260;  // a count, padding to 16 bytes, an id per row of the tile
 
 cudaError_t rows_configure(const char** why);
+// The tile that rows_launch takes.
+RowsTileShape rows_shape(const RowsArgs& g, int sm_count);
 // cudaErrorInvalidValue: a tensor map was refused (alignment or size).
 cudaError_t rows_launch(const RowsArgs& g, int sm_count, int* d_error, cudaStream_t stream);
+// 2-D row-major tensor; boxes of 128 bytes x box_rows, 128-byte swizzle.
+bool rows_map(CUtensorMap* map, const void* ptr, int64_t rows, int64_t cols, int64_t pitch, bool fp8, int box_rows);
+// The forms of the kernel (rows_grouped.cu, rows_gathered.cu, rows_adapters.cu).
+cudaError_t rows_grouped_configure();
+cudaError_t rows_gathered_configure();
+cudaError_t rows_adapters_configure();
+cudaError_t rows_grouped_launch(const RowsArgs& g, RowsTileShape t, int sm_count, int* d_error, cudaStream_t stream);
+cudaError_t rows_gathered_launch(const RowsArgs& g, RowsTileShape t, int sm_count, int* d_error, cudaStream_t stream);
+cudaError_t rows_adapters_launch(const RowsArgs& g, RowsTileShape t, int sm_count, int* d_error, cudaStream_t stream);
 
 struct AdapterDownArgs {
     const void* a;    // [M x K] bf16, pitch lda
@@ -41,7 +53,8 @@ struct AdapterDownArgs {
     const float* scale;  // [n_adapters] or null
     const int32_t* row_adapter;
     float* low;          // [M x rank]
-    int32_t* lists;      // [ceil(M / 128) x kAdapterListInts]
+    int32_t* lists;      // [ceil(M / list_rows) x kAdapterListInts]
+    int list_rows;       // rows of a tile of the product: 128 or 256
     int64_t lda;
     int M, K, rank, n_adapters;
 };

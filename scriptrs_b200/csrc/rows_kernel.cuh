@@ -1,0 +1,775 @@
+// Products whose weights a row chooses, on tcgen05 tensor cores:
+//   grouped:   out[i] = alpha act(s W_e x[rows[i]] + b_e)            for offsets[e] <= i < offsets[e + 1]
+//   adapters:  out[i] = alpha act(W x[i] + U_a low[i] + b)           with the adapter a of row i, low = scale_a D_a x[i]
+//
+// One CTA per SM, warp-specialised like the shared product of gemm.cu: a TMA producer, an MMA issuer (128 rows x BN columns per
+// CTA in tensor memory, two accumulators), eight epilogue warps.  What differs:
+//   - The tiles are found on the device.  A tile belongs to one group: 128 consecutive rows of it per CTA (the last ones of a
+//     group may be missing) times BN columns.  Every warp walks the offsets 32 groups at a time with a prefix sum over its
+//     lanes, so no table of groups is kept and the host never learns the sizes.
+//   - Rows picked by an index arrive by TMA gathers of four rows each, issued by four warps (32 rows each) from one elected
+//     lane with the indices in its registers; a tile with few rows fetches only those.
+//   - Rows leave through a swizzled slab per warp and ordinary stores of 16 bytes a lane, predicated by row and column: the rows
+//     after a group's last one belong to its neighbour.
+//   - The low-rank addition is K = rank more columns of the same product, accumulated in the same tensor memory: `low` as bf16
+//     terms (two where the result is bf16: 2^-17 of it dropped; three where it is stored in 32 bits) against the rows of U_a.
+//     A tile may hold rows of several adapters: its MMAs run once for each, with the lanes of the other rows disabled, so that
+//     nothing of one adapter (not even a NaN) reaches rows of another, and the shared weights are read once whatever the adapters.
+//   - The tensor core adds into its accumulator by truncation, 1e-6 of the result at K = 1024 and 4.4e-6 at 4096 (measured).
+//     Where the result is stored in 32 bits, it is collected in registers every kSegment stages, rounded to nearest (2e-7).
+// Every wait on an mbarrier is bounded; when one runs out the kernel sets *error, drains, frees its tensor memory and returns.
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "gemm_tile.h"
+#include "launch.cuh"
+#include "rows.h"
+#include "tc_ptx.cuh"
+
+namespace sb {
+
+namespace {
+
+using namespace ptx;
+
+constexpr int kBM = 128;
+constexpr int kRowBytes = 128;  // of an operand row in a stage: one swizzle row
+constexpr int kEpiWarps = 8;
+constexpr int kSlabBytes = 32 * 128;
+constexpr int kSegment = 4;     // stages (64 bf16 or 128 e4m3 columns of K each) between two collections of a 32-bit result
+
+enum RowsMode : int { kGrouped = 0, kGathered = 1, kAdapters = 2 };
+
+// CTAS = 2: a cluster of two CTAs on 256 rows x BN columns (tcgen05 cta_group::2); each stages its own 128 rows of A and its own
+// half of the W rows.
+template <int BN, int CTAS>
+struct RCfg {
+    static constexpr int kABytes = kBM * kRowBytes;
+    static constexpr int kBBytes = BN / CTAS * kRowBytes;
+    static constexpr int kStageBytes = kABytes + kBBytes;
+    static constexpr int kStages = kStageBytes <= 24576 ? 8 : (kStageBytes <= 32768 ? 6 : 4);
+    static constexpr int kHalves = gemm_halves(BN);
+    static constexpr int kHalfCols = BN / kHalves;
+    static constexpr int kIndexBytes = kBM * 4;
+    static constexpr int kBarBytes = 384;
+    static constexpr int kSmemBytes = kStages * kStageBytes + kEpiWarps * kSlabBytes + kIndexBytes + kBarBytes + 1024;
+    static constexpr uint32_t kTmemCols = 2 * BN;
+};
+
+// Four warps more where rows are picked (gathers) or have adapters (`low`).
+constexpr int rows_threads(int mode) { return mode == kGrouped ? 320 : 448; }
+
+template <int BN, int CTAS, bool FP8>
+__device__ __forceinline__ uint32_t rows_idesc() {
+    const uint32_t fmt = FP8 ? 0u : 1u;  // e4m3 / bf16; fp32 accumulate, both operands K-major
+    return (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)((kBM * CTAS) >> 4) << 24);
+}
+
+// Four rows of the map (box one row high) to four consecutive 128-byte rows; CTAS = 2: `bar` is a shared::cluster address.
+template <int CTAS>
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int r0, int r1, int r2, int r3) {
+    if constexpr (CTAS == 2) {
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+            ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(r0), "r"(r1), "r"(r2), "r"(r3)
+            : "memory");
+    } else {
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+            ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(r0), "r"(r1), "r"(r2), "r"(r3)
+            : "memory");
+    }
+}
+template <int CTAS>
+__device__ __forceinline__ void rows_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+    if constexpr (CTAS == 2) tma_load_2d_pair(dst, map, bar, c0, c1);
+    else tma_load_2d(dst, map, bar, c0, c1);
+}
+template <int CTAS, bool FP8>
+__device__ __forceinline__ void rows_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (CTAS == 2) tc_mma_pair<FP8>(d, a, b, idesc, accumulate);
+    else tc_mma<FP8>(d, a, b, idesc, accumulate);
+}
+// The product is added in the tensor-memory lanes whose bit in `off` is clear (the pair's second CTA: words 4 to 7).
+template <int CTAS>
+__device__ __forceinline__ void rows_mma_lanes(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, const uint32_t (&off)[4 * CTAS]) {
+    if constexpr (CTAS == 2) {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, 1, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]), "r"(off[4]), "r"(off[5]), "r"(off[6]),
+              "r"(off[7])
+            : "memory");
+    } else {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, 1, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7}, p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3])
+            : "memory");
+    }
+}
+template <int CTAS>
+__device__ __forceinline__ void rows_commit(uint32_t bar) {
+    if constexpr (CTAS == 2) tc_commit_both(bar);
+    else tc_commit(bar);
+}
+// Bounded wait for a barrier on which the other CTA of the pair arrives after writing its shared memory.
+template <int CTAS>
+__device__ __forceinline__ bool rows_wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    if (!mbar_wait(bar, parity, abort_flag)) return false;
+    if constexpr (CTAS == 2) asm volatile("fence.acq_rel.cluster;" ::: "memory");
+    return true;
+}
+
+struct RowsParams {
+    const int32_t* rows;
+    const int32_t* offsets;
+    const float* bias;
+    const float* row_scale;
+    const float* col_scale;
+    void* out;
+    int64_t a_rows, ldo;
+    int M, N, K, n_groups, act, out_mode;
+    float alpha;
+    bool out_vec;    // output rows on 16-byte boundaries
+    bool bias_vec;   // bias and column scales of every group on 16-byte boundaries
+    // adapters
+    const int32_t* row_adapter;
+    const float* low;
+    const int32_t* lists;
+    int rank;
+};
+
+// A tile: rows [row0, row1) of the output, columns from col0, weights of group `group`.
+struct RowsTile {
+    int group, row0, row1, col0;
+};
+
+// Finds tile t.  All lanes of a warp call it together, with ascending t.
+template <int ROWS>
+struct TileWalk {
+    const int32_t* offsets;
+    int M, n_groups, n_tiles, lane;
+    int first_group;      // of the 32 groups that the lanes hold
+    long long first_tile; // tiles of the groups before them
+    int lo, hi, upto;     // this lane's group: rows, tiles of the groups up to and including it
+    int total;            // tiles of the 32 groups
+
+    __device__ __forceinline__ TileWalk(const int32_t* off, int m, int groups, int nt, int ln)
+        : offsets(off), M(m), n_groups(groups), n_tiles(nt), lane(ln), first_group(0), first_tile(0) {
+        load();
+    }
+    __device__ __forceinline__ void load() {
+        const int g = first_group + lane;
+        lo = hi = 0;
+        if (g < n_groups) {
+            // whatever the offsets hold, rows stay inside [0, M)
+            lo = offsets ? min(max(__ldg(offsets + g), 0), M) : 0;
+            hi = offsets ? max(min(__ldg(offsets + g + 1), M), lo) : M;
+        }
+        upto = (hi - lo + ROWS - 1) / ROWS * n_tiles;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += v;
+        }
+        total = __shfl_sync(0xffffffffu, upto, 31);
+    }
+    __device__ __forceinline__ bool find(long long t, int bn, RowsTile& out) {
+        while (t >= first_tile + total) {
+            if (first_group + 32 >= n_groups) return false;
+            first_tile += total;
+            first_group += 32;
+            load();
+        }
+        const int r = (int)(t - first_tile);
+        const int src = __ffs(__ballot_sync(0xffffffffu, upto > r)) - 1;
+        const int before = src ? __shfl_sync(0xffffffffu, upto, src ? src - 1 : 0) : 0;
+        const int glo = __shfl_sync(0xffffffffu, lo, src), ghi = __shfl_sync(0xffffffffu, hi, src);
+        const int mt = (r - before) / n_tiles, nt = (r - before) % n_tiles;
+        out.group = first_group + src;
+        out.row0 = glo + mt * ROWS;
+        out.row1 = min(ghi, out.row0 + ROWS);
+        out.col0 = nt * bn;
+        return true;
+    }
+};
+
+__device__ __forceinline__ float rows_act(float x, int act) {
+    if (act == kActSilu) return __fdividef(x, 1.0f + __expf(-x));
+    return act == kActRelu ? fmaxf(x, 0.0f) : x;
+}
+
+// 32 accumulator columns -> scales, bias, activation.
+template <bool FP8>
+__device__ __forceinline__ void rows_finish(float (&x)[32], const RowsParams& p, int group, int col0, float rs, bool known) {
+    const int64_t at = (int64_t)group * p.N + col0;
+    if (!known) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) x[j] = 0.0f;
+    }
+    if (p.bias_vec) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+            if (col0 + j >= p.N) break;
+            if (FP8) {
+                const float4 cs = p.col_scale ? __ldg(reinterpret_cast<const float4*>(p.col_scale + at + j)) : make_float4(1.f, 1.f, 1.f, 1.f);
+                x[j] *= rs * cs.x; x[j + 1] *= rs * cs.y; x[j + 2] *= rs * cs.z; x[j + 3] *= rs * cs.w;
+            }
+            if (p.bias) {
+                const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + at + j));
+                x[j] += b.x; x[j + 1] += b.y; x[j + 2] += b.z; x[j + 3] += b.w;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            if (col0 + j >= p.N) break;
+            if (FP8) x[j] *= rs * (p.col_scale ? __ldg(p.col_scale + at + j) : 1.0f);
+            if (p.bias) x[j] += __ldg(p.bias + at + j);
+        }
+    }
+    if (p.act != kActNone) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) x[j] = rows_act(x[j], p.act);
+    }
+}
+
+// The slab's 32 rows x COLS columns to memory, the rows below row1 and the columns below N.
+template <typename T, int COLS>
+__device__ __forceinline__ void rows_store(const unsigned char* slab, const RowsParams& p, int row0, int row1, int col0, int lane) {
+    constexpr int kBytes = COLS * (int)sizeof(T), kChunks = kBytes / 16, kPer = 16 / (int)sizeof(T), kStep = 32 / kChunks;
+    constexpr int kShift = kBytes == 64 ? 1 : 0, kMask = kChunks - 1;
+    T* out = static_cast<T*>(p.out);
+    const bool add = sizeof(T) == 4 && p.out_mode == kOutResidual;
+    if (p.out_vec) {
+        const int ch = lane % kChunks, col = col0 + ch * kPer;
+#pragma unroll
+        for (int i = 0; i < 32; i += kStep) {
+            const int r = i + lane / kChunks;
+            if (row0 + r >= row1 || col >= p.N) continue;
+            const uint4 v = *reinterpret_cast<const uint4*>(slab + r * kBytes + ((ch ^ ((r >> kShift) & kMask)) << 4));
+            T* dst = out + (int64_t)(row0 + r) * p.ldo + col;
+            if (col + kPer <= p.N) {
+                if constexpr (sizeof(T) == 4) {
+                    float4 f = make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+                    if (add) {
+                        const float4 o = *reinterpret_cast<const float4*>(dst);
+                        f = make_float4(o.x + f.x, o.y + f.y, o.z + f.z, o.w + f.w);
+                    }
+                    *reinterpret_cast<float4*>(dst) = f;
+                } else {
+                    *reinterpret_cast<uint4*>(dst) = v;
+                }
+            } else {
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) {
+                    if (col + j >= p.N) break;
+                    if constexpr (sizeof(T) == 4) dst[j] = __uint_as_float(w[j]) + (add ? dst[j] : 0.0f);
+                    else dst[j] = __ushort_as_bfloat16((unsigned short)(w[j / 2] >> (16 * (j & 1))));
+                }
+            }
+        }
+    } else {
+        for (int r = 0; r < 32 && row0 + r < row1; ++r) {
+#pragma unroll
+            for (int c = 0; c < COLS; c += 32) {
+                const int cc = c + lane;
+                if (col0 + cc >= p.N) continue;
+                const int byte = cc * (int)sizeof(T);
+                const T v = *reinterpret_cast<const T*>(slab + r * kBytes + (((byte >> 4) ^ ((r >> kShift) & kMask)) << 4) + (byte & 15));
+                T* dst = out + (int64_t)(row0 + r) * p.ldo + col0 + cc;
+                if constexpr (sizeof(T) == 4) *dst = add ? *dst + v : v;
+                else *dst = v;
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&v);
+}
+// What rounding to bf16 leaves of v; nothing where that is not finite (inf - inf).
+__device__ __forceinline__ float bf16_rest(float v) {
+    const float d = v - __bfloat162float(__float2bfloat16_rn(v));
+    return fabsf(d) < INFINITY ? d : 0.0f;
+}
+
+template <int BN, int CTAS, bool FP8, int MODE, bool F32>
+__global__ void __launch_bounds__(rows_threads(MODE), 1)
+rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_w,
+            const __grid_constant__ CUtensorMap tma_up, const RowsParams p, int* __restrict__ error) {
+    using C = RCfg<BN, CTAS>;
+    constexpr int S = C::kStages;
+    constexpr int kStepCols = FP8 ? 128 : 64;
+    constexpr int kTerms = F32 ? 3 : 2;        // bf16 terms of `low`
+    constexpr int kRankChunk = F32 ? 16 : 32;  // its columns in a stage: kTerms x kRankChunk of the 64
+    // rank of this CTA in its pair (the leader, rank 0, owns the barriers that the MMAs wait on)
+    const uint32_t rank = CTAS == 2 ? __shfl_sync(0xffffffffu, cluster_ctarank(), 0) : 0u;
+    extern __shared__ unsigned char smem_dyn[];
+    const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
+    unsigned char* base_ptr = smem_dyn + (base - smem_u32(smem_dyn));
+    const uint32_t a_base = base, b_base = base + S * C::kABytes;
+    constexpr int kSlabAt = S * C::kStageBytes, kIndexAt = kSlabAt + kEpiWarps * kSlabBytes, kBarAt = kIndexAt + C::kIndexBytes;
+    const uint32_t bar_base = base + kBarAt;
+    auto full_bar = [&](int s) { return bar_base + 8u * s; };
+    auto empty_bar = [&](int s) { return bar_base + 8u * (S + s); };
+    auto go_bar = [&](int s) { return bar_base + 8u * (2 * S + s); };        // slot free for `low`
+    auto low_bar = [&](int s) { return bar_base + 8u * (3 * S + s); };       // `low` is there
+    auto tfull_bar = [&](int a) { return bar_base + 8u * (4 * S + a); };
+    auto tempty_bar = [&](int a) { return bar_base + 8u * (4 * S + 2 + a); };
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + kBarAt + 8 * (4 * S + 4));
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    // full barriers of the leader, as its own or as the pair's address
+    auto lead = [&](uint32_t bar) { return CTAS == 2 ? mapa(bar, 0) : bar; };
+
+    const int warp = warp_index(), lane = threadIdx.x & 31;
+    const int n_tiles = (p.N + BN - 1) / BN;
+    const int k_tiles = (p.K + kStepCols - 1) / kStepCols;
+    const int rank_chunks = MODE == kAdapters ? (p.rank + kRankChunk - 1) / kRankChunk : 0;
+    const long long tile0 = blockIdx.x / CTAS, tile_step = gridDim.x / CTAS;
+    const int cta_row = (int)rank * kBM;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+            mbar_init(go_bar(s), 1);
+            mbar_init(low_bar(s), 4 * CTAS);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(tfull_bar(a), 1);
+            mbar_init(tempty_bar(a), 4 * C::kHalves * CTAS);
+        }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        if constexpr (CTAS == 2) {
+            tmem_alloc_pair(smem_u32(tmem_slot), C::kTmemCols);
+            tmem_relinquish_pair();
+        } else {
+            tmem_alloc(smem_u32(tmem_slot), C::kTmemCols);
+            tmem_relinquish();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if constexpr (CTAS == 2) cluster_sync();  // the peer's barriers exist before anything arrives on them
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    pdl_trigger();
+    // The adapters' kernel ahead in the stream waits for everything before it and lets this one start after that: only what
+    // it writes itself (low, lists) has to be waited for here, by the warps that read it.
+    if (MODE != kAdapters) pdl_wait();
+    bool waited = false;
+
+    TileWalk<kBM * CTAS> walk(MODE == kAdapters ? nullptr : p.offsets, p.M, MODE == kAdapters ? 1 : p.n_groups, n_tiles, lane);
+    RowsTile tile;
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ producer
+        int stage = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (long long t = tile0; ok && walk.find(t, BN, tile); t += tile_step) {
+            const int w_col = tile.col0 + (int)rank * (BN / CTAS);
+            const int w_row = tile.group * p.N + w_col;
+            // bytes of A that the pair fetches: whole boxes, or the quads of rows that the gathers bring
+            uint32_t a_bytes = CTAS * C::kABytes;
+            if (MODE == kGathered) {
+                a_bytes = 0;
+#pragma unroll
+                for (int c = 0; c < CTAS; ++c) a_bytes += (uint32_t)((min(max(tile.row1 - tile.row0 - c * kBM, 0), kBM) + 3) >> 2) * (4 * kRowBytes);
+            }
+            bool failed = false;
+            if (elect_one()) {
+                int s = stage;
+                uint32_t sp = ph;
+                for (int kt = 0; kt < k_tiles; ++kt) {
+                    if (!mbar_wait(empty_bar(s), sp ^ 1, abort_flag)) { failed = true; break; }
+                    if (rank == 0) mbar_expect_tx(full_bar(s), CTAS * C::kBBytes + a_bytes);
+                    if (MODE != kGathered)
+                        rows_load<CTAS>(a_base + s * C::kABytes, &tma_a, lead(full_bar(s)), kt * kStepCols, tile.row0 + cta_row);
+                    rows_load<CTAS>(b_base + s * C::kBBytes, &tma_w, lead(full_bar(s)), kt * kStepCols, w_row);
+                    if (++s == S) { s = 0; sp ^= 1; }
+                }
+            }
+            ok = !__any_sync(0xffffffffu, failed);
+            stage += k_tiles;
+            ph ^= (uint32_t)(stage / S) & 1u;
+            stage %= S;
+            if constexpr (MODE == kAdapters) {
+                if (!waited) { pdl_wait(); waited = true; }
+                const int32_t* list = p.lists + (int64_t)(tile.row0 / (kBM * CTAS)) * kAdapterListInts;
+                const int count = list[0];
+                for (int j = 0; ok && j < count; ++j) {
+                    const int u_row = list[4 + j] * p.N + w_col;
+                    for (int c = 0; c < rank_chunks; ++c) {
+                        ok = __all_sync(0xffffffffu, mbar_wait(empty_bar(stage), ph ^ 1, abort_flag));
+                        if (!ok) break;
+                        if (elect_one()) {
+                            mbar_arrive(go_bar(stage));
+                            if (rank == 0) mbar_expect_tx(full_bar(stage), CTAS * C::kBBytes);
+                            rows_load<CTAS>(b_base + stage * C::kBBytes, &tma_up, lead(full_bar(stage)), c * kRankChunk, u_row);
+                        }
+                        __syncwarp();
+                        if (++stage == S) { stage = 0; ph ^= 1; }
+                    }
+                }
+            }
+        }
+        if (!ok) {
+            // copies already in flight land before the CTA exits
+            const long long t0 = clock64();
+            while (clock64() - t0 < 2000000) {}
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA issuer
+        const uint32_t idesc = rows_idesc<BN, CTAS, FP8>();
+        int stage = 0;
+        uint32_t ph = 0, seg = 0, low_ph = 0;
+        bool ok = true;
+        for (long long t = tile0; rank == 0 && ok && walk.find(t, BN, tile); t += tile_step) {
+            int kt = 0;
+            while (ok && kt < k_tiles) {
+                const int acc = seg & 1;
+                const uint32_t d_tmem = tmem_base + acc * BN;
+                const int kt_end = F32 ? min(kt + kSegment, k_tiles) : k_tiles;
+                const bool last = kt_end == k_tiles;
+                bool failed = false;
+                if (elect_one()) {
+                    int s = stage;
+                    uint32_t sp = ph;
+                    if (!mbar_wait(tempty_bar(acc), ((seg >> 1) & 1) ^ 1, abort_flag)) failed = true;
+                    tc_fence_after();
+                    for (int k = kt; k < kt_end && !failed; ++k) {
+                        if (!mbar_wait(full_bar(s), sp, abort_flag)) { failed = true; break; }
+                        tc_fence_after();
+                        const uint64_t adesc = make_smem_desc(a_base + s * C::kABytes), bdesc = make_smem_desc(b_base + s * C::kBBytes);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) rows_mma<CTAS, FP8>(d_tmem, adesc + 2 * i, bdesc + 2 * i, idesc, (k > kt || i) ? 1u : 0u);
+                        rows_commit<CTAS>(empty_bar(s));
+                        if (++s == S) { s = 0; sp ^= 1; }
+                    }
+                    if (!failed && (MODE != kAdapters || !last)) rows_commit<CTAS>(tfull_bar(acc));
+                }
+                ok = !__any_sync(0xffffffffu, failed);
+                stage += kt_end - kt;
+                ph ^= (uint32_t)(stage / S) & 1u;
+                stage %= S;
+                if constexpr (MODE == kAdapters) {
+                    if (ok && last) {
+                        if (!waited) { pdl_wait(); waited = true; }
+                        const int32_t* list = p.lists + (int64_t)(tile.row0 / (kBM * CTAS)) * kAdapterListInts;
+                        const int count = list[0];
+                        int mine[4 * CTAS];
+#pragma unroll
+                        for (int q = 0; q < 4 * CTAS; ++q) {
+                            const int row = tile.row0 + q * 32 + lane;
+                            mine[q] = row < tile.row1 ? __ldg(p.row_adapter + row) : -1;
+                        }
+                        for (int j = 0; ok && j < count; ++j) {
+                            const int id = list[4 + j];
+                            uint32_t off[4 * CTAS];
+#pragma unroll
+                            for (int q = 0; q < 4 * CTAS; ++q) off[q] = ~__ballot_sync(0xffffffffu, mine[q] == id);
+                            for (int c = 0; c < rank_chunks; ++c) {
+                                ok = __all_sync(0xffffffffu, mbar_wait(full_bar(stage), ph, abort_flag) &&
+                                                                 rows_wait_cluster<CTAS>(low_bar(stage), (low_ph >> stage) & 1u, abort_flag));
+                                if (!ok) break;
+                                tc_fence_after();
+                                if (elect_one()) {
+                                    const uint64_t adesc = make_smem_desc(a_base + stage * C::kABytes);
+                                    const uint64_t bdesc = make_smem_desc(b_base + stage * C::kBBytes);
+                                    for (int i = 0; i * 16 < min(kRankChunk, p.rank - c * kRankChunk); ++i) {
+#pragma unroll
+                                        for (int e = 0; e < kTerms; ++e)
+                                            rows_mma_lanes<CTAS>(d_tmem, adesc + e * (kRankChunk / 8) + 2 * i, bdesc + 2 * i, idesc, off);
+                                    }
+                                    rows_commit<CTAS>(empty_bar(stage));
+                                }
+                                __syncwarp();
+                                low_ph ^= 1u << stage;
+                                if (++stage == S) { stage = 0; ph ^= 1; }
+                            }
+                        }
+                        if (ok && elect_one()) rows_commit<CTAS>(tfull_bar(acc));
+                        __syncwarp();
+                    }
+                }
+                kt = kt_end;
+                ++seg;
+            }
+        }
+    } else if (warp < 2 + kEpiWarps) {
+        // ------------------------------------------------------------ epilogue
+        const int ew = warp - 2, quad = warp & 3, half = ew >> 2;
+        unsigned char* slab = base_ptr + kSlabAt + ew * kSlabBytes;
+        uint32_t seg = 0;
+        bool ok = true;
+        for (long long t = tile0; half < C::kHalves && ok && walk.find(t, BN, tile); t += tile_step) {
+            const int row0 = tile.row0 + cta_row + quad * 32;  // of this warp
+            const int row = row0 + lane;
+            const bool live = row < tile.row1;
+            int src = row;
+            if (MODE == kGathered && p.rows && live) src = __ldg(p.rows + row);
+            const bool known = MODE != kGathered || (unsigned)src < (unsigned long long)p.a_rows;
+            const float rs = FP8 && p.row_scale && live && known ? __ldg(p.row_scale + src) : 1.0f;
+            const int cbeg = half * C::kHalfCols;
+            const bool any = row0 < tile.row1;  // rows of this warp in the tile
+            auto taddr = [&]() { return tmem_base + ((uint32_t)(quad * 32) << 16) + (seg & 1) * BN + cbeg; };
+            auto release = [&]() {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (CTAS == 2) mbar_arrive_cluster(mapa(tempty_bar(seg & 1), 0));
+                    else mbar_arrive(tempty_bar(seg & 1));
+                }
+                ++seg;
+            };
+            if constexpr (F32) {
+                constexpr int kCols = C::kHalfCols;
+                float sum[kCols];
+#pragma unroll
+                for (int j = 0; j < kCols; ++j) sum[j] = 0.0f;
+                for (int kt = 0; kt < k_tiles; kt += kSegment) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(tfull_bar(seg & 1), (seg >> 1) & 1, abort_flag));
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (any) {
+#pragma unroll
+                        for (int c = 0; c < kCols; c += 32) {
+                            uint32_t v[32];
+                            tmem_ld32(taddr() + c, v);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) sum[c + j] += __uint_as_float(v[j]);
+                        }
+                    }
+                    release();
+                }
+                if (!ok) break;
+                if (!any) continue;
+#pragma unroll
+                for (int c = 0; c < kCols; c += 32) {
+                    const int col0 = tile.col0 + cbeg + c;
+                    if (col0 >= p.N) break;
+                    float x[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) x[j] = sum[c + j];
+                    rows_finish<FP8>(x, p, tile.group, col0, rs, known);
+#pragma unroll
+                    for (int q = 0; q < 8; ++q)
+                        *reinterpret_cast<float4*>(slab + lane * 128 + ((q ^ (lane & 7)) << 4)) =
+                            make_float4(p.alpha * x[4 * q], p.alpha * x[4 * q + 1], p.alpha * x[4 * q + 2], p.alpha * x[4 * q + 3]);
+                    __syncwarp();
+                    rows_store<float, 32>(slab, p, row0, tile.row1, col0, lane);
+                    __syncwarp();
+                }
+            } else {
+                constexpr int kCols = C::kHalfCols < 64 ? C::kHalfCols : 64;
+                constexpr int kShift = kCols == 32 ? 1 : 0, kMask = kCols / 8 - 1;
+                ok = __all_sync(0xffffffffu, mbar_wait(tfull_bar(seg & 1), (seg >> 1) & 1, abort_flag));
+                if (!ok) break;
+                tc_fence_after();
+                if (any) {
+#pragma unroll 1
+                    for (int c = 0; c < C::kHalfCols; c += kCols) {
+                        const int col0 = tile.col0 + cbeg + c;
+                        if (col0 >= p.N) break;
+#pragma unroll
+                        for (int sub = 0; sub < kCols / 32; ++sub) {
+                            uint32_t v[32];
+                            tmem_ld32(taddr() + c + 32 * sub, v);
+                            tmem_wait_ld();
+                            float x[32];
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) x[j] = __uint_as_float(v[j]);
+                            rows_finish<FP8>(x, p, tile.group, col0 + 32 * sub, rs, known);
+#pragma unroll
+                            for (int q = 0; q < 4; ++q)
+                                *reinterpret_cast<uint4*>(slab + lane * (kCols * 2) + (((4 * sub + q) ^ ((lane >> kShift) & kMask)) << 4)) =
+                                    make_uint4(pack_bf16(x[8 * q], x[8 * q + 1]), pack_bf16(x[8 * q + 2], x[8 * q + 3]),
+                                               pack_bf16(x[8 * q + 4], x[8 * q + 5]), pack_bf16(x[8 * q + 6], x[8 * q + 7]));
+                        }
+                        __syncwarp();
+                        rows_store<__nv_bfloat16, kCols>(slab, p, row0, tile.row1, col0, lane);
+                        __syncwarp();
+                    }
+                }
+                release();
+            }
+        }
+    } else if constexpr (MODE == kGathered) {
+        // ------------------------------------------------------------ gathers, 32 rows a warp
+        const int gw = warp - 2 - kEpiWarps;
+        int32_t* index = reinterpret_cast<int32_t*>(base_ptr + kIndexAt) + gw * 32;
+        int stage = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (long long t = tile0; ok && walk.find(t, BN, tile); t += tile_step) {
+            const int first = tile.row0 + cta_row + gw * 32;
+            const int count = min(tile.row1 - first, 32);
+            const int i = min(first + lane, tile.row1 - 1);
+            const int v = p.rows ? __ldg(p.rows + i) : i;
+            index[lane] = (unsigned)v < (unsigned long long)p.a_rows ? v : 0;
+            __syncwarp();
+            bool failed = false;
+            if (elect_one()) {
+                int4 r[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) r[j] = reinterpret_cast<const int4*>(index)[j];
+                int s = stage;
+                uint32_t sp = ph;
+                for (int kt = 0; kt < k_tiles; ++kt) {
+                    if (!mbar_wait(empty_bar(s), sp ^ 1, abort_flag)) { failed = true; break; }
+                    const uint32_t dst = a_base + s * C::kABytes + gw * 32 * kRowBytes, bar = lead(full_bar(s));
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (4 * j < count) tma_gather4<CTAS>(dst + j * 4 * kRowBytes, &tma_a, bar, kt * kStepCols, r[j].x, r[j].y, r[j].z, r[j].w);
+                    if (++s == S) { s = 0; sp ^= 1; }
+                }
+            }
+            ok = !__any_sync(0xffffffffu, failed);
+            stage += k_tiles;
+            ph ^= (uint32_t)(stage / S) & 1u;
+            stage %= S;
+        }
+        if (!ok) {
+            const long long t0 = clock64();
+            while (clock64() - t0 < 2000000) {}
+        }
+    } else if constexpr (MODE == kAdapters) {
+        // ------------------------------------------------------------ `low` into the ring, a row per thread
+        const int r = (warp - 2 - kEpiWarps) * 32 + lane;
+        int stage = 0;
+        uint32_t go_ph = 0;
+        bool ok = true;
+        pdl_wait();
+        for (long long t = tile0; ok && walk.find(t, BN, tile); t += tile_step) {
+            stage = (stage + k_tiles) % S;
+            const int count = p.lists[(int64_t)(tile.row0 / (kBM * CTAS)) * kAdapterListInts];
+            const int row = tile.row0 + cta_row + r;
+            uint32_t term[kTerms][kRankChunk / 2];
+            int held = -1;  // chunk in the registers
+            for (int j = 0; ok && j < count; ++j) {
+                for (int c = 0; c < rank_chunks; ++c) {
+                    if (held != c) {
+                        held = c;
+#pragma unroll
+                        for (int i = 0; i < kRankChunk; i += 4) {
+                            float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (row < tile.row1 && c * kRankChunk + i < p.rank)
+                                f = *reinterpret_cast<const float4*>(p.low + (int64_t)row * p.rank + c * kRankChunk + i);
+#pragma unroll
+                            for (int e = 0; e < kTerms; ++e) {
+                                term[e][i / 2] = pack_bf16(f.x, f.y);
+                                term[e][i / 2 + 1] = pack_bf16(f.z, f.w);
+                                f = make_float4(bf16_rest(f.x), bf16_rest(f.y), bf16_rest(f.z), bf16_rest(f.w));
+                            }
+                        }
+                    }
+                    ok = __all_sync(0xffffffffu, mbar_wait(go_bar(stage), (go_ph >> stage) & 1u, abort_flag));
+                    if (!ok) break;
+                    unsigned char* dst = base_ptr + stage * C::kABytes + r * kRowBytes;
+#pragma unroll
+                    for (int e = 0; e < kTerms; ++e)
+#pragma unroll
+                        for (int q = 0; q < kRankChunk / 8; ++q)
+                            *reinterpret_cast<uint4*>(dst + (((e * (kRankChunk / 8) + q) ^ (r & 7)) << 4)) =
+                                make_uint4(term[e][4 * q], term[e][4 * q + 1], term[e][4 * q + 2], term[e][4 * q + 3]);
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if constexpr (CTAS == 2) mbar_arrive_cluster(mapa(low_bar(stage), 0));
+                        else mbar_arrive(low_bar(stage));
+                    }
+                    go_ph ^= 1u << stage;
+                    if (++stage == S) stage = 0;
+                }
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if constexpr (CTAS == 2) cluster_sync();  // neither CTA leaves while the other may still touch its memory
+    if (warp == 1) {
+        tc_fence_after();
+        if constexpr (CTAS == 2) tmem_dealloc_pair(tmem_base, C::kTmemCols);
+        else tmem_dealloc(tmem_base, C::kTmemCols);
+    }
+    if (threadIdx.x == 0 && *abort_flag) atomicExch(error, 1);
+}
+
+template <int BN, int CTAS, bool FP8, int MODE, bool F32>
+cudaError_t rows_launch_t(const RowsArgs& g, int sm_count, int* d_error, cudaStream_t stream) {
+    alignas(64) CUtensorMap ma, mw, mu;
+    if (!rows_map(&ma, g.a, g.a_rows, g.K, g.lda, FP8, MODE == kGathered ? 1 : kBM) ||
+        !rows_map(&mw, g.w, (int64_t)g.n_groups * g.N, g.K, g.K, FP8, BN / CTAS))
+        return cudaErrorInvalidValue;
+    mu = mw;
+    if (MODE == kAdapters && !rows_map(&mu, g.up, (int64_t)g.n_adapters * g.N, g.rank, g.rank, false, BN / CTAS)) return cudaErrorInvalidValue;
+    const int eb = F32 ? 4 : 2;
+    RowsParams p{};
+    p.rows = g.rows; p.offsets = g.offsets; p.bias = g.bias; p.row_scale = g.row_scale; p.col_scale = g.col_scale; p.out = g.out;
+    p.a_rows = g.a_rows; p.ldo = g.ldo; p.M = g.M; p.N = g.N; p.K = g.K; p.n_groups = g.n_groups; p.act = g.act; p.out_mode = g.out_mode;
+    p.alpha = g.alpha;
+    p.out_vec = !(reinterpret_cast<uintptr_t>(g.out) & 15) && !((g.ldo * eb) & 15);
+    p.bias_vec = g.N % 4 == 0 && !((reinterpret_cast<uintptr_t>(g.bias) | reinterpret_cast<uintptr_t>(g.col_scale)) & 15);
+    p.row_adapter = g.row_adapter; p.low = g.low; p.lists = g.lists; p.rank = g.rank;
+    // at most this many tiles: a group's last one may be short
+    const int64_t n_tiles = (g.N + BN - 1) / BN;
+    const int64_t tiles = ((int64_t)(g.M + kBM * CTAS - 1) / (kBM * CTAS) + std::min(g.n_groups - 1, g.M)) * n_tiles;
+    const int grid = CTAS * (int)std::min<int64_t>(tiles, sm_count / CTAS);
+    return launch_pdl(rows_kernel<BN, CTAS, FP8, MODE, F32>, dim3(grid), rows_threads(MODE), RCfg<BN, CTAS>::kSmemBytes, stream, CTAS, ma, mw, mu, p,
+                      d_error);
+}
+
+template <int BN, int CTAS, bool FP8, int MODE, bool F32>
+cudaError_t rows_set() {
+    return cudaFuncSetAttribute(rows_kernel<BN, CTAS, FP8, MODE, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, RCfg<BN, CTAS>::kSmemBytes);
+}
+
+// The tiles of one form of the product: columns per tile, CTAs per tile.  A 32-bit result keeps its sums in registers, 64 a
+// thread at most, so its widest tile has 128 columns.
+template <bool FP8, int MODE>
+cudaError_t rows_pick(const RowsArgs& g, RowsTileShape t, int sm_count, int* err, cudaStream_t st) {
+    if (g.out_mode != kOutBf16) {
+        if (t.ctas == 2) return rows_launch_t<128, 2, FP8, MODE, true>(g, sm_count, err, st);
+        switch (t.bn) {
+            case 32: return rows_launch_t<32, 1, FP8, MODE, true>(g, sm_count, err, st);
+            case 64: return rows_launch_t<64, 1, FP8, MODE, true>(g, sm_count, err, st);
+            default: return rows_launch_t<128, 1, FP8, MODE, true>(g, sm_count, err, st);
+        }
+    }
+    if (t.ctas == 2) return rows_launch_t<256, 2, FP8, MODE, false>(g, sm_count, err, st);
+    switch (t.bn) {
+        case 32: return rows_launch_t<32, 1, FP8, MODE, false>(g, sm_count, err, st);
+        case 64: return rows_launch_t<64, 1, FP8, MODE, false>(g, sm_count, err, st);
+        case 128: return rows_launch_t<128, 1, FP8, MODE, false>(g, sm_count, err, st);
+        default: return rows_launch_t<256, 1, FP8, MODE, false>(g, sm_count, err, st);
+    }
+}
+
+template <bool FP8, int MODE>
+cudaError_t rows_set_all() {
+    const cudaError_t e[9] = {rows_set<32, 1, FP8, MODE, true>(),  rows_set<64, 1, FP8, MODE, true>(),   rows_set<128, 1, FP8, MODE, true>(),
+                              rows_set<128, 2, FP8, MODE, true>(), rows_set<32, 1, FP8, MODE, false>(),  rows_set<64, 1, FP8, MODE, false>(),
+                              rows_set<128, 1, FP8, MODE, false>(), rows_set<256, 1, FP8, MODE, false>(), rows_set<256, 2, FP8, MODE, false>()};
+    for (cudaError_t x : e)
+        if (x != cudaSuccess) return x;
+    return cudaSuccess;
+}
+
+}  // namespace
+
+}  // namespace sb

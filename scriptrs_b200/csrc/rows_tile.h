@@ -1,4 +1,5 @@
-// Which tile a product of rows.cu takes.  Host arithmetic only (plain C++, no CUDA types), so that it can be swept without a GPU.
+// Which tile a product of rows_kernel.cuh takes.  Host arithmetic only (plain C++, no CUDA types), so that it can be swept
+// without a GPU.
 #pragma once
 #include <stdint.h>
 
@@ -6,19 +7,30 @@
 
 namespace sb {
 
-// Columns of a tile (128 rows): the width with the least waves x cost of a step of K.  The groups' sizes are on the device;
-// the rows are taken as spread evenly over the groups.
-inline int rows_tile(int64_t M, int N, int n_groups, bool f32, int sm_count) {
+struct RowsTileShape {
+    int bn;    // columns (128 rows per CTA)
+    int ctas;  // 2: a pair of CTAs on 256 rows
+};
+
+// The tile with the least waves x cost of a step of K (64 columns, 0.01 us; of gemm_tile.h).  The groups' sizes are on the
+// device; the rows are taken as spread evenly over the groups, half a tile of each lost.
+inline RowsTileShape rows_tile(int64_t M, int N, int n_groups, bool f32, int sm_count) {
     const int64_t groups = std::min<int64_t>(n_groups, M);
-    const int64_t m_tiles = groups * ((M + groups * 128 - 1) / (groups * 128));
-    const int widths[4] = {256, 128, 64, 32};
-    const int cost[4] = {39, 22, 18, 15};  // of 64 columns of K, 0.01 us
-    int best = 128;
+    RowsTileShape best{128, 1};
     int64_t least = INT64_MAX;
-    for (int i = f32 ? 1 : 0; i < 4; ++i) {
-        const int64_t waves = (m_tiles * ((N + widths[i] - 1) / widths[i]) + sm_count - 1) / sm_count;
-        if (waves * cost[i] < least) { least = waves * cost[i]; best = widths[i]; }
-    }
+    auto offer = [&](int bn, int ctas, int cost) {
+        const int64_t rows = 128 * ctas;
+        const int64_t m_tiles = groups > 1 ? std::max(groups, (2 * M + groups * rows) / (2 * rows)) : (M + rows - 1) / rows;
+        const int64_t slots = std::max(sm_count / ctas, 1);
+        const int64_t waves = (m_tiles * ((N + bn - 1) / bn) + slots - 1) / slots;
+        if (waves * cost < least) { least = waves * cost; best = {bn, ctas}; }
+    };
+    if (!f32) offer(256, 2, 37);
+    else offer(128, 2, 21);
+    if (!f32) offer(256, 1, 39);
+    offer(128, 1, 22);
+    offer(64, 1, 18);
+    offer(32, 1, 15);
     return best;
 }
 

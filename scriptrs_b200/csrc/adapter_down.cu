@@ -1,26 +1,27 @@
 // Down-projection of the low-rank adapters: low[i] = scale_a (x[i] D_a^T) for the adapter a of row i, kept in 32 bits, and for
 // the rows of every tile of the product the list of the adapters among them, in the order of their first rows.
 //
-// Bound by reading the rows once (2 K bytes each against K * rank products), so the products run on mma.sync m16n8k16 with
-// operands straight from global memory.  A warp takes 16 rows x COLS columns and every KW-th 32 columns of K; the partial sums
-// meet in shared memory in a fixed order.  KW = 8 (16 rows a block) spreads few rows over many SMs, KW = 2 (64 rows a block)
-// reads an adapter's matrix from L1 for four row tiles.  Rows of several adapters in a tile are products of their own, of which
-// each row takes its adapter's (selected, not masked by zeros: nothing of one adapter reaches another's rows).  Where nearly
-// every row has its own adapter (live streams), 16 such products would run one after the other; there a row is a chain of dot
-// products over the lanes instead.
+// Bound by reading the rows once (2 K bytes each against K * rank products).  Two kernels:
+//   - many rows: 128 rows a CTA on tcgen05, rows and adapters through a TMA ring, one pass over K for each adapter among the rows
+//     with the lanes of the other rows disabled (nothing of one adapter reaches another's rows).
+//   - few rows: 16 rows a block on mma.sync m16n8k16 with operands straight from global memory, K over the warps, the columns over
+//     blocks; a row takes its adapter's product (selected, not masked by zeros).
+// Where nearly every row has its own adapter (live streams), such passes would run one after the other; there a row is a chain of
+// dot products over the lanes of a warp.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 #include "launch.cuh"
 #include "rows.h"
+#include "tc_ptx.cuh"
 
 namespace sb {
 
 namespace {
 
 constexpr int kDownWarps = 8;
-constexpr int kMaxProducts = 3;  // adapters in 16 rows above which the rows are taken one by one
+constexpr int kMaxProducts = 2;  // adapters in 16 rows above which the rows are taken one by one
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -33,44 +34,71 @@ __device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float s) {
     return fmaf(__uint_as_float(a & 0xffff0000u), __uint_as_float(b & 0xffff0000u), s);
 }
 
-// NT tiles of 8 columns per block; KW warps share the K of 16 rows.
-template <int NT, int KW>
+// The adapters of the list_rows rows from row0 on.
+__device__ __forceinline__ void write_list(const AdapterDownArgs& p, int row0, int lane) {
+    int ids[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int r = row0 + 8 * lane + j;
+        ids[j] = 8 * lane + j < p.list_rows && r < p.M ? __ldg(p.row_adapter + r) : -1;
+        if ((unsigned)ids[j] >= (unsigned)p.n_adapters) ids[j] = -1;
+    }
+    int32_t* list = p.lists + (int64_t)(row0 / p.list_rows) * kAdapterListInts;
+    int count = 0;
+    while (true) {
+        int first = -1;
+#pragma unroll
+        for (int j = 7; j >= 0; --j)
+            if (ids[j] >= 0) first = ids[j];
+        const uint32_t have = __ballot_sync(0xffffffffu, first >= 0);
+        if (!have) break;
+        const int cur = __shfl_sync(0xffffffffu, first, __ffs(have) - 1);
+        if (lane == 0) list[4 + count] = cur;
+        ++count;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (ids[j] == cur) ids[j] = -1;
+    }
+    if (lane == 0) list[0] = count;
+}
+
+// Eight columns of a row's product, K over the lanes; lane j < 8 returns column j.
+__device__ __forceinline__ float row_dots(const __nv_bfloat16* x, const __nv_bfloat16* d, int K, int cols, int lane) {
+    float acc[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
+#pragma unroll 2
+    for (int k = lane * 8; k < K; k += 256) {
+        const uint4 xv = __ldg(reinterpret_cast<const uint4*>(x + k));
+        uint4 w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = __ldg(reinterpret_cast<const uint4*>(d + (int64_t)min(j, cols - 1) * K + k));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] = dot2(xv.w, w[j].w, dot2(xv.z, w[j].z, dot2(xv.y, w[j].y, dot2(xv.x, w[j].x, acc[j]))));
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int s = 16; s; s >>= 1) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], s);
+    float v = acc[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j)
+        if (lane == j) v = acc[j];
+    return v;
+}
+
+// NT tiles of 8 columns of 16 rows per block; the warps share K.
+template <int NT>
 __global__ void __launch_bounds__(kDownWarps * 32) adapter_down_kernel(const AdapterDownArgs p) {
-    constexpr int kCols = NT * 8, kRows = 16 * (kDownWarps / KW);
-    __shared__ float part[KW][kRows][kCols];
+    constexpr int kCols = NT * 8, kRows = 16;
+    __shared__ float part[kDownWarps][kRows][kCols];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int block0 = blockIdx.x * kRows, col0 = blockIdx.y * kCols;
+    const int row0 = blockIdx.x * kRows, col0 = blockIdx.y * kCols;
     pdl_wait();
     pdl_trigger();  // what runs beside this block may rely on all that came before it, but not on `low` and the lists
 
-    if (blockIdx.y == 0 && block0 % p.list_rows == 0 && warp == kDownWarps - 1) {
-        int ids[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int r = block0 + 8 * lane + j;
-            ids[j] = 8 * lane + j < p.list_rows && r < p.M ? __ldg(p.row_adapter + r) : -1;
-            if ((unsigned)ids[j] >= (unsigned)p.n_adapters) ids[j] = -1;
-        }
-        int32_t* list = p.lists + (int64_t)(block0 / p.list_rows) * kAdapterListInts;
-        int count = 0;
-        while (true) {
-            int first = -1;
-#pragma unroll
-            for (int j = 7; j >= 0; --j)
-                if (ids[j] >= 0) first = ids[j];
-            const uint32_t have = __ballot_sync(0xffffffffu, first >= 0);
-            if (!have) break;
-            const int cur = __shfl_sync(0xffffffffu, first, __ffs(have) - 1);
-            if (lane == 0) list[4 + count] = cur;
-            ++count;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (ids[j] == cur) ids[j] = -1;
-        }
-        if (lane == 0) list[0] = count;
-    }
+    if (blockIdx.y == 0 && row0 % p.list_rows == 0 && warp == kDownWarps - 1) write_list(p, row0, lane);
 
-    const int kw = warp % KW, tile_row = warp / KW * 16, row0 = block0 + tile_row;
     const int my_row = row0 + (lane & 15);
     int id = my_row < p.M ? __ldg(p.row_adapter + my_row) : -1;
     if ((unsigned)id >= (unsigned)p.n_adapters) id = -1;
@@ -100,21 +128,32 @@ __global__ void __launch_bounds__(kDownWarps * 32) adapter_down_kernel(const Ada
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
             const __nv_bfloat16* d = down + (int64_t)cur * p.rank * p.K;
-            // 32 columns of K: a lane's 16 bytes are the fragments of two products, the same permutation of K on both sides
-#pragma unroll(NT >= 8 ? 2 : 4)
-            for (int k = kw * 32; k < p.K; k += KW * 32) {
-                const int kk = k + 8 * q;
-                const bool in = kk < p.K;
-                uint4 xl = make_uint4(0, 0, 0, 0), xh = xl;
-                if (in && row0 + g < p.M) xl = __ldg(reinterpret_cast<const uint4*>(a + (int64_t)(row0 + g) * p.lda + kk));
-                if (in && row0 + g + 8 < p.M) xh = __ldg(reinterpret_cast<const uint4*>(a + (int64_t)(row0 + g + 8) * p.lda + kk));
+            // 32 columns of K: a lane's 16 bytes are the fragments of two products, the same permutation of K on both sides; four
+            // steps' rows are asked for at once
+            for (int k0 = warp * 32; k0 < p.K; k0 += 4 * kDownWarps * 32) {
+                uint4 xl[4], xh[4];
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const int col = col0 + 8 * n + g;
-                    uint4 w = make_uint4(0, 0, 0, 0);
-                    if (in && col < p.rank) w = __ldg(reinterpret_cast<const uint4*>(d + (int64_t)col * p.K + kk));
-                    mma_bf16(acc[n], xl.x, xh.x, xl.y, xh.y, w.x, w.y);
-                    mma_bf16(acc[n], xl.z, xh.z, xl.w, xh.w, w.z, w.w);
+                for (int u = 0; u < 4; ++u) {
+                    const int kk = k0 + u * kDownWarps * 32 + 8 * q;
+                    xl[u] = xh[u] = make_uint4(0, 0, 0, 0);
+                    if (kk < p.K && row0 + g < p.M) xl[u] = __ldg(reinterpret_cast<const uint4*>(a + (int64_t)(row0 + g) * p.lda + kk));
+                    if (kk < p.K && row0 + g + 8 < p.M) xh[u] = __ldg(reinterpret_cast<const uint4*>(a + (int64_t)(row0 + g + 8) * p.lda + kk));
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int kk = k0 + u * kDownWarps * 32 + 8 * q;
+                    uint4 w[NT];
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const int col = col0 + 8 * n + g;
+                        w[n] = make_uint4(0, 0, 0, 0);
+                        if (kk < p.K && col < p.rank) w[n] = __ldg(reinterpret_cast<const uint4*>(d + (int64_t)col * p.K + kk));
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        mma_bf16(acc[n], xl[u].x, xh[u].x, xl[u].y, xh[u].y, w[n].x, w[n].y);
+                        mma_bf16(acc[n], xl[u].z, xh[u].z, xl[u].w, xh[u].w, w[n].z, w[n].w);
+                    }
                 }
             }
 #pragma unroll
@@ -125,76 +164,273 @@ __global__ void __launch_bounds__(kDownWarps * 32) adapter_down_kernel(const Ada
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            *reinterpret_cast<float2*>(&part[kw][tile_row + g][8 * n + 2 * q]) = make_float2(sum[n][0], sum[n][1]);
-            *reinterpret_cast<float2*>(&part[kw][tile_row + g + 8][8 * n + 2 * q]) = make_float2(sum[n][2], sum[n][3]);
+            *reinterpret_cast<float2*>(&part[warp][g][8 * n + 2 * q]) = make_float2(sum[n][0], sum[n][1]);
+            *reinterpret_cast<float2*>(&part[warp][g + 8][8 * n + 2 * q]) = make_float2(sum[n][2], sum[n][3]);
         }
     } else {
-        // rows kw, kw + KW, ... of the tile, eight columns at a time, K over the lanes
+        // every eighth row a warp, eight columns at a time
         for (int r = 0; r < 16; ++r) {
             const int cur = __shfl_sync(0xffffffffu, id, r);
-            const bool mine = r % KW == kw && cur >= 0;
+            const bool mine = r % kDownWarps == warp && cur >= 0;
             for (int c = 0; c < kCols; c += 8) {
-                float acc[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
-                if (mine) {
-                    const __nv_bfloat16* x = a + (int64_t)(row0 + r) * p.lda;
-                    const __nv_bfloat16* d = down + ((int64_t)cur * p.rank + col0 + c) * p.K;
-#pragma unroll 2
-                    for (int k = lane * 8; k < p.K; k += 256) {
-                        const uint4 xv = __ldg(reinterpret_cast<const uint4*>(x + k));
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            if (col0 + c + j >= p.rank) break;
-                            const uint4 w = __ldg(reinterpret_cast<const uint4*>(d + (int64_t)j * p.K + k));
-                            acc[j] = dot2(xv.w, w.w, dot2(xv.z, w.z, dot2(xv.y, w.y, dot2(xv.x, w.x, acc[j]))));
-                        }
-                    }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-#pragma unroll
-                        for (int s = 16; s; s >>= 1) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], s);
-                }
-                if (lane < 8) {
-                    float v = acc[0];
-#pragma unroll
-                    for (int j = 1; j < 8; ++j)
-                        if (lane == j) v = acc[j];
-                    part[kw][tile_row + r][c + lane] = v;
-                }
+                const int cols = min(p.rank - col0 - c, 8);
+                float v = 0.0f;
+                if (mine && cols > 0) v = row_dots(a + (int64_t)(row0 + r) * p.lda, down + ((int64_t)cur * p.rank + col0 + c) * p.K, p.K, cols, lane);
+                if (lane < 8) part[warp][r][c + lane] = v;
             }
         }
     }
     __syncthreads();
     for (int i = threadIdx.x; i < kRows * kCols; i += kDownWarps * 32) {
-        const int r = i / kCols, c = i % kCols, row = block0 + r;
+        const int r = i / kCols, c = i % kCols, row = row0 + r;
         if (row >= p.M || col0 + c >= p.rank) continue;
         const int who = __ldg(p.row_adapter + row);
         float s = 0.0f;
         if ((unsigned)who < (unsigned)p.n_adapters) {
 #pragma unroll
-            for (int w = 0; w < KW; ++w) s += part[w][r][c];
+            for (int w = 0; w < kDownWarps; ++w) s += part[w][r][c];
             if (p.scale) s *= __ldg(p.scale + who);
         }
         p.low[(int64_t)row * p.rank + col0 + c] = s;
     }
 }
 
-template <int NT, int KW>
+// ---------------------------------------------------------------------------------------------- many rows: tcgen05
+constexpr int kTcRows = 128, kTcStages = 4, kTcThreads = 192;
+constexpr int kTcMaxPasses = 12;  // adapters in 128 rows above which the rows are taken one by one
+
+constexpr int tc_cols(int rank) { return rank <= 16 ? 16 : (rank <= 32 ? 32 : (rank <= 64 ? 64 : 128)); }
+template <int RN>
+struct DownTc {
+    static constexpr int kABytes = kTcRows * 128, kBBytes = RN * 128, kStageBytes = kABytes + kBBytes;
+    static constexpr int kSmemBytes = kTcStages * kStageBytes + 128 + 1024;
+    static constexpr uint32_t kTmemCols = RN < 32 ? 32 : RN;
+};
+
+// The adapters among 128 rows, four rows a lane, in the order of their first rows; -1 after the last one.
+struct IdWalk {
+    int ids[4];
+    __device__ __forceinline__ IdWalk(const AdapterDownArgs& p, int row0, int lane) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int r = row0 + 4 * lane + j;
+            ids[j] = r < p.M ? __ldg(p.row_adapter + r) : -1;
+            if ((unsigned)ids[j] >= (unsigned)p.n_adapters) ids[j] = -1;
+        }
+    }
+    __device__ __forceinline__ int next() {
+        int first = -1;
+#pragma unroll
+        for (int j = 3; j >= 0; --j)
+            if (ids[j] >= 0) first = ids[j];
+        const uint32_t have = __ballot_sync(0xffffffffu, first >= 0);
+        if (!have) return -1;
+        const int cur = __shfl_sync(0xffffffffu, first, __ffs(have) - 1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (ids[j] == cur) ids[j] = -1;
+        return cur;
+    }
+};
+
+// Warp 0 loads, warp 1 issues the MMAs, warps 2 to 5 read the results, a row per thread.
+template <int RN>
+__global__ void __launch_bounds__(kTcThreads) adapter_down_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_d,
+                                                                     const AdapterDownArgs p, int* __restrict__ error) {
+    using namespace ptx;
+    using C = DownTc<RN>;
+    extern __shared__ unsigned char smem_dyn[];
+    const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
+    unsigned char* base_ptr = smem_dyn + (base - smem_u32(smem_dyn));
+    const uint32_t a_base = base, b_base = base + kTcStages * C::kABytes, bar_base = base + kTcStages * C::kStageBytes;
+    auto full_bar = [&](int s) { return bar_base + 8u * s; };
+    auto empty_bar = [&](int s) { return bar_base + 8u * (kTcStages + s); };
+    const uint32_t done_bar = bar_base + 8u * (2 * kTcStages);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + kTcStages * C::kStageBytes + 8 * (2 * kTcStages + 1));
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int warp = warp_index(), lane = threadIdx.x & 31;
+    const int row0 = blockIdx.x * kTcRows, k_tiles = (p.K + 63) / 64;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kTcStages; ++s) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        mbar_init(done_bar, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(tmem_slot), C::kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_wait();
+    pdl_trigger();
+    // every warp counts the adapters for itself
+    int passes = 0;
+    {
+        IdWalk w(p, row0, lane);
+        while (passes <= kTcMaxPasses && w.next() >= 0) ++passes;
+    }
+    const bool dots = passes > kTcMaxPasses;
+
+    if (warp == 0 && !dots) {
+        IdWalk w(p, row0, lane);
+        int stage = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int id = w.next(); ok && id >= 0; id = w.next()) {
+            bool failed = false;
+            if (elect_one()) {
+                int s = stage;
+                uint32_t sp = ph;
+                for (int kt = 0; kt < k_tiles; ++kt) {
+                    if (!mbar_wait(empty_bar(s), sp ^ 1, abort_flag)) { failed = true; break; }
+                    mbar_expect_tx(full_bar(s), C::kStageBytes);
+                    tma_load_2d(a_base + s * C::kABytes, &tma_a, full_bar(s), kt * 64, row0);
+                    tma_load_2d(b_base + s * C::kBBytes, &tma_d, full_bar(s), kt * 64, id * p.rank);
+                    if (++s == kTcStages) { s = 0; sp ^= 1; }
+                }
+            }
+            ok = !__any_sync(0xffffffffu, failed);
+            stage += k_tiles;
+            ph ^= (uint32_t)(stage / kTcStages) & 1u;
+            stage %= kTcStages;
+        }
+        if (!ok) {
+            const long long t0 = clock64();
+            while (clock64() - t0 < 2000000) {}
+        }
+    } else if (warp == 1 && !dots) {
+        // fp32 accumulate, bf16 operands, both K-major, M = 128, N = RN
+        constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(RN >> 3) << 17) | ((uint32_t)(kTcRows >> 4) << 24);
+        IdWalk w(p, row0, lane);
+        int mine[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) mine[q] = row0 + 32 * q + lane < p.M ? __ldg(p.row_adapter + row0 + 32 * q + lane) : -1;
+        int stage = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int id = w.next(); ok && id >= 0; id = w.next()) {
+            uint32_t off[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) off[q] = ~__ballot_sync(0xffffffffu, mine[q] == id);
+            bool failed = false;
+            if (elect_one()) {
+                int s = stage;
+                uint32_t sp = ph;
+                for (int kt = 0; kt < k_tiles; ++kt) {
+                    if (!mbar_wait(full_bar(s), sp, abort_flag)) { failed = true; break; }
+                    tc_fence_after();
+                    const uint64_t adesc = make_smem_desc(a_base + s * C::kABytes), bdesc = make_smem_desc(b_base + s * C::kBBytes);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) tc_mma_lanes(tmem, adesc + 2 * i, bdesc + 2 * i, idesc, off, (kt | i) ? 1u : 0u);
+                    tc_commit(empty_bar(s));
+                    if (++s == kTcStages) { s = 0; sp ^= 1; }
+                }
+            }
+            ok = !__any_sync(0xffffffffu, failed);
+            stage += k_tiles;
+            ph ^= (uint32_t)(stage / kTcStages) & 1u;
+            stage %= kTcStages;
+        }
+        if (ok && elect_one()) tc_commit(done_bar);
+        __syncwarp();
+    } else if (!dots) {
+        if (warp == 2 && row0 % p.list_rows == 0) write_list(p, row0, lane);
+        const bool ok = __all_sync(0xffffffffu, mbar_wait(done_bar, 0, abort_flag));
+        tc_fence_after();
+        const int quad = warp & 3, row = row0 + 32 * quad + lane;
+        const int id = row < p.M ? __ldg(p.row_adapter + row) : -1;
+        const bool has = (unsigned)id < (unsigned)p.n_adapters;
+        const float f = has ? (p.scale ? __ldg(p.scale + id) : 1.0f) : 0.0f;
+#pragma unroll
+        for (int c = 0; c < RN; c += 16) {
+            if (!ok || c >= p.rank) break;
+            uint32_t v[16];
+            tmem_ld16(tmem + ((uint32_t)(quad * 32) << 16) + c, v);
+            tmem_wait_ld();
+            if (row >= p.M) continue;
+            float4* out = reinterpret_cast<float4*>(p.low + (int64_t)row * p.rank + c);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                // a row without an adapter leaves the accumulator as it was found: not a number to multiply by zero
+                if (c + 4 * j < p.rank)
+                    out[j] = has ? make_float4(f * __uint_as_float(v[4 * j]), f * __uint_as_float(v[4 * j + 1]), f * __uint_as_float(v[4 * j + 2]),
+                                               f * __uint_as_float(v[4 * j + 3]))
+                                 : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        }
+    } else {
+        if (warp == 2 && row0 % p.list_rows == 0) write_list(p, row0, lane);
+        const __nv_bfloat16* a = static_cast<const __nv_bfloat16*>(p.a);
+        const __nv_bfloat16* down = static_cast<const __nv_bfloat16*>(p.down);
+        for (int r = warp; r < kTcRows && row0 + r < p.M; r += kTcThreads / 32) {
+            const int row = row0 + r, id = __ldg(p.row_adapter + row);
+            const bool has = (unsigned)id < (unsigned)p.n_adapters;
+            for (int c = 0; c < p.rank; c += 8) {
+                float v = 0.0f;
+                if (has) {
+                    v = row_dots(a + (int64_t)row * p.lda, down + ((int64_t)id * p.rank + c) * p.K, p.K, 8, lane);
+                    if (p.scale) v *= __ldg(p.scale + id);
+                }
+                if (lane < 8) p.low[(int64_t)row * p.rank + c + lane] = v;
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, C::kTmemCols);
+    }
+    if (threadIdx.x == 0 && *abort_flag) atomicExch(error, 1);
+}
+
+template <int RN>
+cudaError_t down_tc_t(const AdapterDownArgs& g, int* d_error, cudaStream_t stream) {
+    alignas(64) CUtensorMap ma, md;
+    if (!rows_map(&ma, g.a, g.M, g.K, g.lda, false, kTcRows) || !rows_map(&md, g.down, (int64_t)g.n_adapters * g.rank, g.K, g.K, false, RN))
+        return cudaErrorInvalidValue;
+    return launch_pdl(adapter_down_tc_kernel<RN>, dim3((g.M + kTcRows - 1) / kTcRows), kTcThreads, DownTc<RN>::kSmemBytes, stream, 1, ma, md, g, d_error);
+}
+
+template <int NT>
 cudaError_t down_t(const AdapterDownArgs& g, cudaStream_t stream) {
-    const int rows = 16 * (kDownWarps / KW);
-    const dim3 grid((g.M + rows - 1) / rows, (g.rank + NT * 8 - 1) / (NT * 8));
-    return launch_pdl(adapter_down_kernel<NT, KW>, grid, kDownWarps * 32, 0, stream, 1, g);
+    const dim3 grid((g.M + 15) / 16, (g.rank + NT * 8 - 1) / (NT * 8));
+    return launch_pdl(adapter_down_kernel<NT>, grid, kDownWarps * 32, 0, stream, 1, g);
 }
 
 }  // namespace
 
-cudaError_t adapter_down_launch(const AdapterDownArgs& g, int sm_count, cudaStream_t stream) {
+cudaError_t adapter_down_configure() {
+    cudaError_t e = cudaSuccess;
+    auto set = [&](auto kernel, int bytes) {
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    };
+    set(adapter_down_tc_kernel<16>, DownTc<16>::kSmemBytes);
+    set(adapter_down_tc_kernel<32>, DownTc<32>::kSmemBytes);
+    set(adapter_down_tc_kernel<64>, DownTc<64>::kSmemBytes);
+    set(adapter_down_tc_kernel<128>, DownTc<128>::kSmemBytes);
+    return e;
+}
+
+cudaError_t adapter_down_launch(const AdapterDownArgs& g, int sm_count, int* d_error, cudaStream_t stream) {
     if (g.M <= 0) return cudaSuccess;
-    // 64 rows a block once those give every SM two blocks; else 16, and few rows spread their columns over blocks too
-    if (g.M >= 128 * sm_count) return g.rank > 32 ? down_t<8, 2>(g, stream) : (g.rank > 16 ? down_t<4, 2>(g, stream) : down_t<2, 2>(g, stream));
-    if (g.M >= 16 * sm_count) return g.rank > 32 ? down_t<8, 8>(g, stream) : (g.rank > 16 ? down_t<4, 8>(g, stream) : down_t<2, 8>(g, stream));
-    return down_t<1, 8>(g, stream);
+    if (g.M >= 16 * sm_count) {
+        switch (tc_cols(g.rank)) {
+            case 16: return down_tc_t<16>(g, d_error, stream);
+            case 32: return down_tc_t<32>(g, d_error, stream);
+            case 64: return down_tc_t<64>(g, d_error, stream);
+            default: return down_tc_t<128>(g, d_error, stream);
+        }
+    }
+    // the columns are spread over blocks too, as far as that fills the SMs
+    const int blocks = (g.M + 15) / 16;
+    return blocks * 4 >= sm_count ? down_t<2>(g, stream) : down_t<1>(g, stream);
 }
 
 }  // namespace sb

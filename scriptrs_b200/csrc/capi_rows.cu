@@ -152,8 +152,9 @@ int32_t sb_adapter_gemm(sb_ctx* c, const void* d_a, int64_t lda, const void* d_w
     d.list_rows = 128 * rows_shape(g, c->sm_count).ctas;
     d.M = (int)M; d.K = (int)K; d.rank = (int)rank; d.n_adapters = (int)n_adapters;
     c->prof.begin("adapter_down", c->stream);
-    cudaError_t e = adapter_down_launch(d, c->sm_count, c->stream);
+    cudaError_t e = adapter_down_launch(d, c->sm_count, c->d_error, c->stream);
     c->prof.end(c->stream);
+    if (e == cudaErrorInvalidValue) return fail(SB_INVALID_ARGUMENT, "adapter shape or alignment not supported");
     SB_CUDA(e);
     c->prof.begin("adapter_gemm", c->stream);
     e = rows_launch(g, c->sm_count, c->d_error, c->stream);

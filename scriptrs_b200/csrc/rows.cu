@@ -28,6 +28,17 @@ bool rows_map(CUtensorMap* map, const void* ptr, int64_t rows, int64_t cols, int
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool rows_out_map(CUtensorMap* map, void* ptr, int64_t rows, int64_t cols, int64_t pitch, bool f32, int row_bytes) {
+    const int eb = f32 ? 4 : 2;
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)pitch * eb};
+    const cuuint32_t box[2] = {(cuuint32_t)(row_bytes / eb), 32};
+    const cuuint32_t estr[2] = {1, 1};
+    return g_rows_encode(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, ptr, dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, row_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 cudaError_t rows_configure(const char** why) {
     if (!g_rows_encode) {
         void* fn = nullptr;
@@ -39,7 +50,7 @@ cudaError_t rows_configure(const char** why) {
         }
         g_rows_encode = reinterpret_cast<EncodeTiledFn>(fn);
     }
-    for (cudaError_t (*set)() : {rows_grouped_configure, rows_gathered_configure, rows_adapters_configure}) {
+    for (cudaError_t (*set)() : {rows_grouped_configure, rows_gathered_configure, rows_adapters_configure, adapter_down_configure}) {
         const cudaError_t e = set();
         if (e != cudaSuccess) {
             if (why) *why = "shared-memory opt-in for the row products failed";

@@ -39,6 +39,8 @@ RowsTileShape rows_shape(const RowsArgs& g, int sm_count);
 cudaError_t rows_launch(const RowsArgs& g, int sm_count, int* d_error, cudaStream_t stream);
 // 2-D row-major tensor; boxes of 128 bytes x box_rows, 128-byte swizzle.
 bool rows_map(CUtensorMap* map, const void* ptr, int64_t rows, int64_t cols, int64_t pitch, bool fp8, int box_rows);
+// The result's map: boxes of 32 rows x row_bytes (64 or 128, swizzled over as many).
+bool rows_out_map(CUtensorMap* map, void* ptr, int64_t rows, int64_t cols, int64_t pitch, bool f32, int row_bytes);
 // The forms of the kernel (rows_grouped.cu, rows_gathered.cu, rows_adapters.cu).
 cudaError_t rows_grouped_configure();
 cudaError_t rows_gathered_configure();
@@ -58,7 +60,8 @@ struct AdapterDownArgs {
     int64_t lda;
     int M, K, rank, n_adapters;
 };
-cudaError_t adapter_down_launch(const AdapterDownArgs& g, int sm_count, cudaStream_t stream);
+cudaError_t adapter_down_configure();
+cudaError_t adapter_down_launch(const AdapterDownArgs& g, int sm_count, int* d_error, cudaStream_t stream);
 
 struct RouteArgs {
     const void* logits;  // [rows x n_experts], pitch ld

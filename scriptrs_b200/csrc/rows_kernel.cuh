@@ -9,8 +9,8 @@
 //     lanes, so no table of groups is kept and the host never learns the sizes.
 //   - Rows picked by an index arrive by TMA gathers of four rows each, issued by four warps (32 rows each) from one elected
 //     lane with the indices in its registers; a tile with few rows fetches only those.
-//   - Rows leave through a swizzled slab per warp and ordinary stores of 16 bytes a lane, predicated by row and column: the rows
-//     after a group's last one belong to its neighbour.
+//   - Rows leave through a swizzled slab per warp: 32 rows of one group by a TMA store (or reduce-add), which clips at column N;
+//     the last rows of a group, behind which its neighbour's begin, and results off the 16-byte boundaries by ordinary stores.
 //   - The low-rank addition is K = rank more columns of the same product, accumulated in the same tensor memory: `low` as bf16
 //     terms (two where the result is bf16: 2^-17 of it dropped; three where it is stored in 32 bits) against the rows of U_a.
 //     A tile may hold rows of several adapters: its MMAs run once for each, with the lanes of the other rows disabled, so that
@@ -47,17 +47,19 @@ enum RowsMode : int { kGrouped = 0, kGathered = 1, kAdapters = 2 };
 
 // CTAS = 2: a cluster of two CTAs on 256 rows x BN columns (tcgen05 cta_group::2); each stages its own 128 rows of A and its own
 // half of the W rows.
-template <int BN, int CTAS>
+template <int BN, int CTAS, int MODE>
 struct RCfg {
     static constexpr int kABytes = kBM * kRowBytes;
     static constexpr int kBBytes = BN / CTAS * kRowBytes;
     static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kStages = kStageBytes <= 24576 ? 8 : (kStageBytes <= 32768 ? 6 : 4);
+    static constexpr int kLowBytes = MODE == kAdapters ? 2 * kBM * kRowBytes : 0;  // `low` of the tile's rows: two operand tiles
+    static constexpr int kStages = std::min((231 * 1024 - 2048 - kEpiWarps * kSlabBytes - kLowBytes - kBM * 4) / kStageBytes, 8);
     static constexpr int kHalves = gemm_halves(BN);
     static constexpr int kHalfCols = BN / kHalves;
     static constexpr int kIndexBytes = kBM * 4;
-    static constexpr int kBarBytes = 384;
-    static constexpr int kSmemBytes = kStages * kStageBytes + kEpiWarps * kSlabBytes + kIndexBytes + kBarBytes + 1024;
+    static constexpr int kBarBytes = 256;
+    static constexpr int kSmemBytes = kStages * kStageBytes + kLowBytes + kEpiWarps * kSlabBytes + kIndexBytes + kBarBytes + 1024;
+    static_assert(kStages >= 3 && kSmemBytes <= 227 * 1024 && 8 * (2 * kStages + 6) + 8 <= kBarBytes, "shared memory");
     static constexpr uint32_t kTmemCols = 2 * BN;
 };
 
@@ -95,23 +97,10 @@ __device__ __forceinline__ void rows_mma(uint32_t d, uint64_t a, uint64_t b, uin
     if constexpr (CTAS == 2) tc_mma_pair<FP8>(d, a, b, idesc, accumulate);
     else tc_mma<FP8>(d, a, b, idesc, accumulate);
 }
-// The product is added in the tensor-memory lanes whose bit in `off` is clear (the pair's second CTA: words 4 to 7).
 template <int CTAS>
 __device__ __forceinline__ void rows_mma_lanes(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, const uint32_t (&off)[4 * CTAS]) {
-    if constexpr (CTAS == 2) {
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, 1, 0;\n\t"
-            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, p;\n\t}"
-            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]), "r"(off[4]), "r"(off[5]), "r"(off[6]),
-              "r"(off[7])
-            : "memory");
-    } else {
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, 1, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7}, p;\n\t}"
-            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3])
-            : "memory");
-    }
+    if constexpr (CTAS == 2) tc_mma_lanes_pair(d, a, b, idesc, off, 1u);
+    else tc_mma_lanes(d, a, b, idesc, off, 1u);
 }
 template <int CTAS>
 __device__ __forceinline__ void rows_commit(uint32_t bar) {
@@ -120,10 +109,25 @@ __device__ __forceinline__ void rows_commit(uint32_t bar) {
 }
 // Bounded wait for a barrier on which the other CTA of the pair arrives after writing its shared memory.
 template <int CTAS>
-__device__ __forceinline__ bool rows_wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-    if (!mbar_wait(bar, parity, abort_flag)) return false;
-    if constexpr (CTAS == 2) asm volatile("fence.acq_rel.cluster;" ::: "memory");
-    return true;
+__device__ __forceinline__ bool rows_wait_pair(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    if constexpr (CTAS == 1) return mbar_wait(bar, parity, abort_flag);
+    const long long t0 = clock64();
+    while (true) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if (*abort_flag) return false;
+        if (clock64() - t0 > kWaitCycles) {
+            *abort_flag = 1;
+            return false;
+        }
+    }
 }
 
 struct RowsParams {
@@ -200,43 +204,62 @@ struct TileWalk {
     }
 };
 
-__device__ __forceinline__ float rows_act(float x, int act) {
-    if (act == kActSilu) return __fdividef(x, 1.0f + __expf(-x));
-    return act == kActRelu ? fmaxf(x, 0.0f) : x;
+// Brings the bias and the column scales of a tile's columns into L1 while the accumulator is not ready yet.
+template <bool FP8>
+__device__ __forceinline__ void rows_touch(const RowsParams& p, int group, int col0, int cols, int lane) {
+    const int col = col0 + (lane & 15) * 32;
+    if ((lane & 15) * 32 >= cols || col >= p.N) return;
+    const float* from = lane < 16 ? p.bias : (FP8 ? p.col_scale : nullptr);
+    if (from) asm volatile("prefetch.global.L1 [%0];" ::"l"(from + (int64_t)group * p.N + col));
 }
 
-// 32 accumulator columns -> scales, bias, activation.
-template <bool FP8>
+// 32 accumulator columns -> scales, bias, activation.  The loads carry no branches between them: one that ended the loop at N
+// made each wait for the one before it, 5000 cycles for 32 columns.
+template <bool FP8, bool F32>
 __device__ __forceinline__ void rows_finish(float (&x)[32], const RowsParams& p, int group, int col0, float rs, bool known) {
     const int64_t at = (int64_t)group * p.N + col0;
     if (!known) {
 #pragma unroll
         for (int j = 0; j < 32; ++j) x[j] = 0.0f;
     }
-    if (p.bias_vec) {
+    if (FP8) {
+        if (p.col_scale && p.bias_vec) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-            if (col0 + j >= p.N) break;
-            if (FP8) {
-                const float4 cs = p.col_scale ? __ldg(reinterpret_cast<const float4*>(p.col_scale + at + j)) : make_float4(1.f, 1.f, 1.f, 1.f);
-                x[j] *= rs * cs.x; x[j + 1] *= rs * cs.y; x[j + 2] *= rs * cs.z; x[j + 3] *= rs * cs.w;
+            for (int j = 0; j < 32; j += 4) {
+                float4 c = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (col0 + j < p.N) c = __ldg(reinterpret_cast<const float4*>(p.col_scale + at + j));
+                x[j] *= rs * c.x; x[j + 1] *= rs * c.y; x[j + 2] *= rs * c.z; x[j + 3] *= rs * c.w;
             }
-            if (p.bias) {
-                const float4 b = __ldg(reinterpret_cast<const float4*>(p.bias + at + j));
-                x[j] += b.x; x[j + 1] += b.y; x[j + 2] += b.z; x[j + 3] += b.w;
-            }
-        }
-    } else {
+        } else {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            if (col0 + j >= p.N) break;
-            if (FP8) x[j] *= rs * (p.col_scale ? __ldg(p.col_scale + at + j) : 1.0f);
-            if (p.bias) x[j] += __ldg(p.bias + at + j);
+            for (int j = 0; j < 32; ++j) {
+                float c = 1.0f;
+                if (p.col_scale && col0 + j < p.N) c = __ldg(p.col_scale + at + j);
+                x[j] *= rs * c;
+            }
         }
     }
-    if (p.act != kActNone) {
+    if (p.bias && p.bias_vec) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) x[j] = rows_act(x[j], p.act);
+        for (int j = 0; j < 32; j += 4) {
+            float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (col0 + j < p.N) b = __ldg(reinterpret_cast<const float4*>(p.bias + at + j));
+            x[j] += b.x; x[j + 1] += b.y; x[j + 2] += b.z; x[j + 3] += b.w;
+        }
+    } else if (p.bias) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            float b = 0.0f;
+            if (col0 + j < p.N) b = __ldg(p.bias + at + j);
+            x[j] += b;
+        }
+    }
+    if (p.act == kActSilu) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) x[j] = F32 ? __fdividef(x[j], 1.0f + __expf(-x[j])) : silu_fast(x[j]);
+    } else if (p.act == kActRelu) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) x[j] = x[j] < 0.0f ? 0.0f : x[j];  // NaN stays
     }
 }
 
@@ -305,27 +328,29 @@ __device__ __forceinline__ float bf16_rest(float v) {
 template <int BN, int CTAS, bool FP8, int MODE, bool F32>
 __global__ void __launch_bounds__(rows_threads(MODE), 1)
 rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_w,
-            const __grid_constant__ CUtensorMap tma_up, const RowsParams p, int* __restrict__ error) {
-    using C = RCfg<BN, CTAS>;
+            const __grid_constant__ CUtensorMap tma_up, const __grid_constant__ CUtensorMap tma_out, const RowsParams p,
+            int* __restrict__ error) {
+    using C = RCfg<BN, CTAS, MODE>;
     constexpr int S = C::kStages;
     constexpr int kStepCols = FP8 ? 128 : 64;
-    constexpr int kTerms = F32 ? 3 : 2;        // bf16 terms of `low`
-    constexpr int kRankChunk = F32 ? 16 : 32;  // its columns in a stage: kTerms x kRankChunk of the 64
+    // `low` as bf16 terms, 16 of its columns in 32 bytes of each: eight such blocks a row fit, kGroups x kTerms of them are used
+    constexpr int kTerms = F32 ? 3 : 2, kGroups = 8 / kTerms, kPhaseCols = 16 * kGroups;
     // rank of this CTA in its pair (the leader, rank 0, owns the barriers that the MMAs wait on)
     const uint32_t rank = CTAS == 2 ? __shfl_sync(0xffffffffu, cluster_ctarank(), 0) : 0u;
     extern __shared__ unsigned char smem_dyn[];
     const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
     unsigned char* base_ptr = smem_dyn + (base - smem_u32(smem_dyn));
     const uint32_t a_base = base, b_base = base + S * C::kABytes;
-    constexpr int kSlabAt = S * C::kStageBytes, kIndexAt = kSlabAt + kEpiWarps * kSlabBytes, kBarAt = kIndexAt + C::kIndexBytes;
+    constexpr int kLowAt = S * C::kStageBytes, kSlabAt = kLowAt + C::kLowBytes, kIndexAt = kSlabAt + kEpiWarps * kSlabBytes;
+    constexpr int kBarAt = kIndexAt + C::kIndexBytes;
     const uint32_t bar_base = base + kBarAt;
     auto full_bar = [&](int s) { return bar_base + 8u * s; };
     auto empty_bar = [&](int s) { return bar_base + 8u * (S + s); };
-    auto go_bar = [&](int s) { return bar_base + 8u * (2 * S + s); };        // slot free for `low`
-    auto low_bar = [&](int s) { return bar_base + 8u * (3 * S + s); };       // `low` is there
-    auto tfull_bar = [&](int a) { return bar_base + 8u * (4 * S + a); };
-    auto tempty_bar = [&](int a) { return bar_base + 8u * (4 * S + 2 + a); };
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + kBarAt + 8 * (4 * S + 4));
+    auto tfull_bar = [&](int a) { return bar_base + 8u * (2 * S + a); };
+    auto tempty_bar = [&](int a) { return bar_base + 8u * (2 * S + 2 + a); };
+    const uint32_t low_bar = bar_base + 8u * (2 * S + 4);   // `low` of a tile is there
+    const uint32_t lowfree_bar = bar_base + 8u * (2 * S + 5);  // and has been read
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + kBarAt + 8 * (2 * S + 6));
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     // full barriers of the leader, as its own or as the pair's address
     auto lead = [&](uint32_t bar) { return CTAS == 2 ? mapa(bar, 0) : bar; };
@@ -333,7 +358,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
     const int warp = warp_index(), lane = threadIdx.x & 31;
     const int n_tiles = (p.N + BN - 1) / BN;
     const int k_tiles = (p.K + kStepCols - 1) / kStepCols;
-    const int rank_chunks = MODE == kAdapters ? (p.rank + kRankChunk - 1) / kRankChunk : 0;
+    const int phases = MODE == kAdapters ? (p.rank + kPhaseCols - 1) / kPhaseCols : 0;
     const long long tile0 = blockIdx.x / CTAS, tile_step = gridDim.x / CTAS;
     const int cta_row = (int)rank * kBM;
 
@@ -341,13 +366,13 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
         for (int s = 0; s < S; ++s) {
             mbar_init(full_bar(s), 1);
             mbar_init(empty_bar(s), 1);
-            mbar_init(go_bar(s), 1);
-            mbar_init(low_bar(s), 4 * CTAS);
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(tfull_bar(a), 1);
             mbar_init(tempty_bar(a), 4 * C::kHalves * CTAS);
         }
+        mbar_init(low_bar, 4 * CTAS);
+        mbar_init(lowfree_bar, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -389,6 +414,13 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
 #pragma unroll
                 for (int c = 0; c < CTAS; ++c) a_bytes += (uint32_t)((min(max(tile.row1 - tile.row0 - c * kBM, 0), kBM) + 3) >> 2) * (4 * kRowBytes);
             }
+            // the tile's adapters, on their way while the shared columns of K are fetched
+            const int32_t* list = nullptr;
+            int count = 0, ids = 0;
+            if (MODE == kAdapters) {
+                list = p.lists + (int64_t)(tile.row0 / (kBM * CTAS)) * kAdapterListInts;
+                if (waited) { count = list[0]; ids = list[4 + lane]; }
+            }
             bool failed = false;
             if (elect_one()) {
                 int s = stage;
@@ -407,18 +439,16 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
             ph ^= (uint32_t)(stage / S) & 1u;
             stage %= S;
             if constexpr (MODE == kAdapters) {
-                if (!waited) { pdl_wait(); waited = true; }
-                const int32_t* list = p.lists + (int64_t)(tile.row0 / (kBM * CTAS)) * kAdapterListInts;
-                const int count = list[0];
-                for (int j = 0; ok && j < count; ++j) {
-                    const int u_row = list[4 + j] * p.N + w_col;
-                    for (int c = 0; c < rank_chunks; ++c) {
+                if (!waited) { pdl_wait(); waited = true; count = list[0]; ids = list[4 + lane]; }
+                for (int c = 0; c < phases; ++c) {
+                    for (int j = 0; ok && j < count; ++j) {
+                        if (count > 32 && j % 32 == 0) ids = list[4 + j + lane];
+                        const int u_row = __shfl_sync(0xffffffffu, ids, j % 32) * p.N + w_col;
                         ok = __all_sync(0xffffffffu, mbar_wait(empty_bar(stage), ph ^ 1, abort_flag));
                         if (!ok) break;
                         if (elect_one()) {
-                            mbar_arrive(go_bar(stage));
                             if (rank == 0) mbar_expect_tx(full_bar(stage), CTAS * C::kBBytes);
-                            rows_load<CTAS>(b_base + stage * C::kBBytes, &tma_up, lead(full_bar(stage)), c * kRankChunk, u_row);
+                            rows_load<CTAS>(b_base + stage * C::kBBytes, &tma_up, lead(full_bar(stage)), c * kPhaseCols, u_row);
                         }
                         __syncwarp();
                         if (++stage == S) { stage = 0; ph ^= 1; }
@@ -438,6 +468,21 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
         uint32_t ph = 0, seg = 0, low_ph = 0;
         bool ok = true;
         for (long long t = tile0; rank == 0 && ok && walk.find(t, BN, tile); t += tile_step) {
+            const int32_t* list = nullptr;
+            int count = 0, ids = 0, mine[4 * CTAS];
+            auto fetch = [&]() {
+                count = list[0];
+                ids = list[4 + lane];
+#pragma unroll
+                for (int q = 0; q < 4 * CTAS; ++q) {
+                    const int row = tile.row0 + q * 32 + lane;
+                    mine[q] = row < tile.row1 ? __ldg(p.row_adapter + row) : -1;
+                }
+            };
+            if (MODE == kAdapters) {
+                list = p.lists + (int64_t)(tile.row0 / (kBM * CTAS)) * kAdapterListInts;
+                if (waited) fetch();
+            }
             int kt = 0;
             while (ok && kt < k_tiles) {
                 const int acc = seg & 1;
@@ -467,37 +512,36 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                 stage %= S;
                 if constexpr (MODE == kAdapters) {
                     if (ok && last) {
-                        if (!waited) { pdl_wait(); waited = true; }
-                        const int32_t* list = p.lists + (int64_t)(tile.row0 / (kBM * CTAS)) * kAdapterListInts;
-                        const int count = list[0];
-                        int mine[4 * CTAS];
+                        if (!waited) { pdl_wait(); waited = true; fetch(); }
+                        for (int c = 0; count > 0 && c < phases; ++c) {
+                            ok = ok && __all_sync(0xffffffffu, rows_wait_pair<CTAS>(low_bar, low_ph, abort_flag));
+                            low_ph ^= 1;
+                            const int groups = min(kGroups, (p.rank - c * kPhaseCols + 15) / 16);
+                            for (int j = 0; ok && j < count; ++j) {
+                                if (count > 32 && j % 32 == 0) ids = list[4 + j + lane];
+                                const int id = __shfl_sync(0xffffffffu, ids, j % 32);
+                                uint32_t off[4 * CTAS];
 #pragma unroll
-                        for (int q = 0; q < 4 * CTAS; ++q) {
-                            const int row = tile.row0 + q * 32 + lane;
-                            mine[q] = row < tile.row1 ? __ldg(p.row_adapter + row) : -1;
-                        }
-                        for (int j = 0; ok && j < count; ++j) {
-                            const int id = list[4 + j];
-                            uint32_t off[4 * CTAS];
-#pragma unroll
-                            for (int q = 0; q < 4 * CTAS; ++q) off[q] = ~__ballot_sync(0xffffffffu, mine[q] == id);
-                            for (int c = 0; c < rank_chunks; ++c) {
-                                ok = __all_sync(0xffffffffu, mbar_wait(full_bar(stage), ph, abort_flag) &&
-                                                                 rows_wait_cluster<CTAS>(low_bar(stage), (low_ph >> stage) & 1u, abort_flag));
+                                for (int q = 0; q < 4 * CTAS; ++q) off[q] = ~__ballot_sync(0xffffffffu, mine[q] == id);
+                                ok = __all_sync(0xffffffffu, mbar_wait(full_bar(stage), ph, abort_flag));
                                 if (!ok) break;
                                 tc_fence_after();
                                 if (elect_one()) {
-                                    const uint64_t adesc = make_smem_desc(a_base + stage * C::kABytes);
-                                    const uint64_t bdesc = make_smem_desc(b_base + stage * C::kBBytes);
-                                    for (int i = 0; i * 16 < min(kRankChunk, p.rank - c * kRankChunk); ++i) {
+                                    const uint64_t adesc = make_smem_desc(base + kLowAt), bdesc = make_smem_desc(b_base + stage * C::kBBytes);
 #pragma unroll
-                                        for (int e = 0; e < kTerms; ++e)
-                                            rows_mma_lanes<CTAS>(d_tmem, adesc + e * (kRankChunk / 8) + 2 * i, bdesc + 2 * i, idesc, off);
+                                    for (int g = 0; g < kGroups; ++g) {
+                                        if (g >= groups) break;
+#pragma unroll
+                                        for (int e = 0; e < kTerms; ++e) {
+                                            constexpr int kTile = kBM * kRowBytes / 16;  // in the descriptor's 16-byte units
+                                            const int at = g * kTerms + e;
+                                            rows_mma_lanes<CTAS>(d_tmem, adesc + at / 4 * kTile + 2 * (at % 4), bdesc + 2 * g, idesc, off);
+                                        }
                                     }
                                     rows_commit<CTAS>(empty_bar(stage));
+                                    if (j == count - 1) rows_commit<CTAS>(lowfree_bar);
                                 }
                                 __syncwarp();
-                                low_ph ^= 1u << stage;
                                 if (++stage == S) { stage = 0; ph ^= 1; }
                             }
                         }
@@ -525,6 +569,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
             const float rs = FP8 && p.row_scale && live && known ? __ldg(p.row_scale + src) : 1.0f;
             const int cbeg = half * C::kHalfCols;
             const bool any = row0 < tile.row1;  // rows of this warp in the tile
+            rows_touch<FP8>(p, tile.group, tile.col0 + cbeg, C::kHalfCols, lane);
             auto taddr = [&]() { return tmem_base + ((uint32_t)(quad * 32) << 16) + (seg & 1) * BN + cbeg; };
             auto release = [&]() {
                 tc_fence_before();
@@ -534,6 +579,26 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                     else mbar_arrive(tempty_bar(seg & 1));
                 }
                 ++seg;
+            };
+            const bool whole = p.out_vec && row0 + 32 <= tile.row1;  // 32 rows of this group: one TMA store
+            auto ready = [&]() {  // the store before has read the slab
+                if (elect_one()) bulk_wait_read0();
+                __syncwarp();
+            };
+            auto leave = [&](int col0, auto&& store) {
+                if (whole) {
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (elect_one()) {
+                        if (F32 && p.out_mode == kOutResidual) tma_reduce_add_2d(&tma_out, smem_u32(slab), col0, row0);
+                        else tma_store_2d(&tma_out, smem_u32(slab), col0, row0);
+                        bulk_commit();
+                    }
+                } else {
+                    __syncwarp();
+                    store();
+                }
+                __syncwarp();
             };
             if constexpr (F32) {
                 constexpr int kCols = C::kHalfCols;
@@ -565,14 +630,13 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                     float x[32];
 #pragma unroll
                     for (int j = 0; j < 32; ++j) x[j] = sum[c + j];
-                    rows_finish<FP8>(x, p, tile.group, col0, rs, known);
+                    rows_finish<FP8, F32>(x, p, tile.group, col0, rs, known);
+                    ready();
 #pragma unroll
                     for (int q = 0; q < 8; ++q)
                         *reinterpret_cast<float4*>(slab + lane * 128 + ((q ^ (lane & 7)) << 4)) =
                             make_float4(p.alpha * x[4 * q], p.alpha * x[4 * q + 1], p.alpha * x[4 * q + 2], p.alpha * x[4 * q + 3]);
-                    __syncwarp();
-                    rows_store<float, 32>(slab, p, row0, tile.row1, col0, lane);
-                    __syncwarp();
+                    leave(col0, [&]() { rows_store<float, 32>(slab, p, row0, tile.row1, col0, lane); });
                 }
             } else {
                 constexpr int kCols = C::kHalfCols < 64 ? C::kHalfCols : 64;
@@ -585,6 +649,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                     for (int c = 0; c < C::kHalfCols; c += kCols) {
                         const int col0 = tile.col0 + cbeg + c;
                         if (col0 >= p.N) break;
+                        ready();
 #pragma unroll
                         for (int sub = 0; sub < kCols / 32; ++sub) {
                             uint32_t v[32];
@@ -593,21 +658,21 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                             float x[32];
 #pragma unroll
                             for (int j = 0; j < 32; ++j) x[j] = __uint_as_float(v[j]);
-                            rows_finish<FP8>(x, p, tile.group, col0 + 32 * sub, rs, known);
+                            rows_finish<FP8, F32>(x, p, tile.group, col0 + 32 * sub, rs, known);
 #pragma unroll
                             for (int q = 0; q < 4; ++q)
                                 *reinterpret_cast<uint4*>(slab + lane * (kCols * 2) + (((4 * sub + q) ^ ((lane >> kShift) & kMask)) << 4)) =
                                     make_uint4(pack_bf16(x[8 * q], x[8 * q + 1]), pack_bf16(x[8 * q + 2], x[8 * q + 3]),
                                                pack_bf16(x[8 * q + 4], x[8 * q + 5]), pack_bf16(x[8 * q + 6], x[8 * q + 7]));
                         }
-                        __syncwarp();
-                        rows_store<__nv_bfloat16, kCols>(slab, p, row0, tile.row1, col0, lane);
-                        __syncwarp();
+                        leave(col0, [&]() { rows_store<__nv_bfloat16, kCols>(slab, p, row0, tile.row1, col0, lane); });
                     }
                 }
                 release();
             }
         }
+        if (elect_one()) bulk_wait_all();
+        __syncwarp();
     } else if constexpr (MODE == kGathered) {
         // ------------------------------------------------------------ gathers, 32 rows a warp
         const int gw = warp - 2 - kEpiWarps;
@@ -648,53 +713,51 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
             while (clock64() - t0 < 2000000) {}
         }
     } else if constexpr (MODE == kAdapters) {
-        // ------------------------------------------------------------ `low` into the ring, a row per thread
+        // ------------------------------------------------------------ `low` of the tile's rows as an operand, a row per thread
         const int r = (warp - 2 - kEpiWarps) * 32 + lane;
-        int stage = 0;
-        uint32_t go_ph = 0;
+        unsigned char* dst = base_ptr + kLowAt + r * kRowBytes;
+        uint32_t ph = 0;
         bool ok = true;
         pdl_wait();
         for (long long t = tile0; ok && walk.find(t, BN, tile); t += tile_step) {
-            stage = (stage + k_tiles) % S;
             const int count = p.lists[(int64_t)(tile.row0 / (kBM * CTAS)) * kAdapterListInts];
             const int row = tile.row0 + cta_row + r;
-            uint32_t term[kTerms][kRankChunk / 2];
-            int held = -1;  // chunk in the registers
-            for (int j = 0; ok && j < count; ++j) {
-                for (int c = 0; c < rank_chunks; ++c) {
-                    if (held != c) {
-                        held = c;
+            for (int c = 0; count > 0 && c < phases; ++c) {
+                float f[kPhaseCols];
 #pragma unroll
-                        for (int i = 0; i < kRankChunk; i += 4) {
-                            float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-                            if (row < tile.row1 && c * kRankChunk + i < p.rank)
-                                f = *reinterpret_cast<const float4*>(p.low + (int64_t)row * p.rank + c * kRankChunk + i);
-#pragma unroll
-                            for (int e = 0; e < kTerms; ++e) {
-                                term[e][i / 2] = pack_bf16(f.x, f.y);
-                                term[e][i / 2 + 1] = pack_bf16(f.z, f.w);
-                                f = make_float4(bf16_rest(f.x), bf16_rest(f.y), bf16_rest(f.z), bf16_rest(f.w));
-                            }
-                        }
-                    }
-                    ok = __all_sync(0xffffffffu, mbar_wait(go_bar(stage), (go_ph >> stage) & 1u, abort_flag));
-                    if (!ok) break;
-                    unsigned char* dst = base_ptr + stage * C::kABytes + r * kRowBytes;
-#pragma unroll
-                    for (int e = 0; e < kTerms; ++e)
-#pragma unroll
-                        for (int q = 0; q < kRankChunk / 8; ++q)
-                            *reinterpret_cast<uint4*>(dst + (((e * (kRankChunk / 8) + q) ^ (r & 7)) << 4)) =
-                                make_uint4(term[e][4 * q], term[e][4 * q + 1], term[e][4 * q + 2], term[e][4 * q + 3]);
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if constexpr (CTAS == 2) mbar_arrive_cluster(mapa(low_bar(stage), 0));
-                        else mbar_arrive(low_bar(stage));
-                    }
-                    go_ph ^= 1u << stage;
-                    if (++stage == S) stage = 0;
+                for (int i = 0; i < kPhaseCols; i += 4) {
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (row < tile.row1 && c * kPhaseCols + i < p.rank)
+                        v = *reinterpret_cast<const float4*>(p.low + (int64_t)row * p.rank + c * kPhaseCols + i);
+                    f[i] = v.x; f[i + 1] = v.y; f[i + 2] = v.z; f[i + 3] = v.w;
                 }
+                ok = __all_sync(0xffffffffu, mbar_wait(lowfree_bar, ph ^ 1, abort_flag));
+                if (!ok) break;
+#pragma unroll
+                for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+                    for (int e = 0; e < kTerms; ++e) {
+                        uint32_t w[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            float& x = f[16 * g + 2 * i];
+                            float& y = f[16 * g + 2 * i + 1];
+                            w[i] = pack_bf16(x, y);
+                            x = bf16_rest(x);
+                            y = bf16_rest(y);
+                        }
+                        const int at = g * kTerms + e, chunk = 2 * (at % 4);
+                        unsigned char* d = dst + at / 4 * kBM * kRowBytes;
+                        *reinterpret_cast<uint4*>(d + ((chunk ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                        *reinterpret_cast<uint4*>(d + (((chunk + 1) ^ (r & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
+                    }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (CTAS == 2) mbar_arrive_cluster(mapa(low_bar, 0));
+                    else mbar_arrive(low_bar);
+                }
+                ph ^= 1;
             }
         }
     }
@@ -712,7 +775,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
 
 template <int BN, int CTAS, bool FP8, int MODE, bool F32>
 cudaError_t rows_launch_t(const RowsArgs& g, int sm_count, int* d_error, cudaStream_t stream) {
-    alignas(64) CUtensorMap ma, mw, mu;
+    alignas(64) CUtensorMap ma, mw, mu, mo;
     if (!rows_map(&ma, g.a, g.a_rows, g.K, g.lda, FP8, MODE == kGathered ? 1 : kBM) ||
         !rows_map(&mw, g.w, (int64_t)g.n_groups * g.N, g.K, g.K, FP8, BN / CTAS))
         return cudaErrorInvalidValue;
@@ -725,18 +788,20 @@ cudaError_t rows_launch_t(const RowsArgs& g, int sm_count, int* d_error, cudaStr
     p.alpha = g.alpha;
     p.out_vec = !(reinterpret_cast<uintptr_t>(g.out) & 15) && !((g.ldo * eb) & 15);
     p.bias_vec = g.N % 4 == 0 && !((reinterpret_cast<uintptr_t>(g.bias) | reinterpret_cast<uintptr_t>(g.col_scale)) & 15);
+    mo = mw;
+    if (p.out_vec && !rows_out_map(&mo, g.out, g.M, g.N, g.ldo, F32, F32 || RCfg<BN, CTAS, MODE>::kHalfCols >= 64 ? 128 : 64)) return cudaErrorInvalidValue;
     p.row_adapter = g.row_adapter; p.low = g.low; p.lists = g.lists; p.rank = g.rank;
     // at most this many tiles: a group's last one may be short
     const int64_t n_tiles = (g.N + BN - 1) / BN;
     const int64_t tiles = ((int64_t)(g.M + kBM * CTAS - 1) / (kBM * CTAS) + std::min(g.n_groups - 1, g.M)) * n_tiles;
     const int grid = CTAS * (int)std::min<int64_t>(tiles, sm_count / CTAS);
-    return launch_pdl(rows_kernel<BN, CTAS, FP8, MODE, F32>, dim3(grid), rows_threads(MODE), RCfg<BN, CTAS>::kSmemBytes, stream, CTAS, ma, mw, mu, p,
+    return launch_pdl(rows_kernel<BN, CTAS, FP8, MODE, F32>, dim3(grid), rows_threads(MODE), RCfg<BN, CTAS, MODE>::kSmemBytes, stream, CTAS, ma, mw, mu, mo, p,
                       d_error);
 }
 
 template <int BN, int CTAS, bool FP8, int MODE, bool F32>
 cudaError_t rows_set() {
-    return cudaFuncSetAttribute(rows_kernel<BN, CTAS, FP8, MODE, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, RCfg<BN, CTAS>::kSmemBytes);
+    return cudaFuncSetAttribute(rows_kernel<BN, CTAS, FP8, MODE, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, RCfg<BN, CTAS, MODE>::kSmemBytes);
 }
 
 // The tiles of one form of the product: columns per tile, CTAs per tile.  A 32-bit result keeps its sums in registers, 64 a

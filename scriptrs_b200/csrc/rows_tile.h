@@ -25,8 +25,8 @@ inline RowsTileShape rows_tile(int64_t M, int N, int n_groups, bool f32, int sm_
         const int64_t waves = (m_tiles * ((N + bn - 1) / bn) + slots - 1) / slots;
         if (waves * cost < least) { least = waves * cost; best = {bn, ctas}; }
     };
-    if (!f32) offer(256, 2, 37);
-    else offer(128, 2, 21);
+    if (!f32) offer(256, 2, 34);
+    else offer(128, 2, 20);
     if (!f32) offer(256, 1, 39);
     offer(128, 1, 22);
     offer(64, 1, 18);

@@ -112,6 +112,25 @@ __device__ __forceinline__ void tc_mma(uint32_t tmem_d, uint64_t adesc, uint64_t
             : "memory");
     }
 }
+// The product is added (or, without `accumulate`, put) in the tensor-memory lanes whose bit in `off` is clear; bf16 operands.
+__device__ __forceinline__ void tc_mma_lanes(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, const uint32_t (&off)[4],
+                                             uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %8, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7}, p;\n\t}"
+        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]), "r"(accumulate)
+        : "memory");
+}
+// The same over a pair of CTAs; words 4 to 7 are the lanes of the second one.
+__device__ __forceinline__ void tc_mma_lanes_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, const uint32_t (&off)[8],
+                                                  uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %12, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, p;\n\t}"
+        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]), "r"(off[4]), "r"(off[5]),
+          "r"(off[6]), "r"(off[7]), "r"(accumulate)
+        : "memory");
+}
 // ---- thread-block clusters of two CTAs (tcgen05 cta_group::2: one MMA spans the tensor cores of both SMs)
 __device__ __forceinline__ uint32_t cluster_ctarank() {
     uint32_t r;

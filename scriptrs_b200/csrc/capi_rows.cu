@@ -1,6 +1,7 @@
 // extern "C" layer: products whose weights a row chooses.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <string>
 
 #include "context.h"
@@ -40,7 +41,7 @@ extern "C" {
 
 int64_t sb_route_topk_workspace(int64_t rows, int64_t n_experts, int64_t top_k) {
     if (rows <= 0 || n_experts <= 0 || n_experts > kMaxRouteExperts || top_k <= 0 || rows > kLimit / top_k) return 0;
-    return route_work_bytes(rows, n_experts, top_k);
+    return std::max<int64_t>(route_work_bytes(rows, n_experts, top_k), 16);
 }
 
 int64_t sb_adapter_gemm_workspace(int64_t M, int64_t rank) {
@@ -61,8 +62,8 @@ int32_t sb_route_topk(sb_ctx* c, const void* d_logits, int32_t logits_bf16, int6
         if (off_boundary(d_logits, logits_bf16 ? 2 : 4) || off_boundary(d_experts, 4) || off_boundary(d_weights, 4) || off_boundary(d_order, 4) ||
             off_boundary(d_slots, 4) || off_boundary(d_work, 16))
             return fail(SB_INVALID_ARGUMENT, "arrays lie on the boundaries of their types, the workspace on a 16-byte one");
-        const int64_t need = route_work_bytes(rows, n_experts, top_k);
-        if (work_bytes < need || (need > 0 && !d_work)) return fail(SB_BUFFER_TOO_SMALL, "workspace of " + std::to_string(need) + " bytes needed");
+        const int64_t need = sb_route_topk_workspace(rows, n_experts, top_k);
+        if (work_bytes < need || !d_work) return fail(SB_BUFFER_TOO_SMALL, "workspace of " + std::to_string(need) + " bytes needed");
     }
     if (!c) return fail(SB_INVALID_ARGUMENT, "ctx is null");
     SB_CUDA(cudaSetDevice(c->device));

@@ -15,9 +15,18 @@ namespace sb {
 
 namespace {
 
-constexpr int kRouteWarps = 8;
-constexpr int kRouteRows = 128;  // per block of the choice and of the placement
+constexpr int kRouteThreads = 512, kRouteWarps = kRouteThreads / 32;
+constexpr int kRouteRows = 512;     // most rows of a block
+constexpr int kRouteOneBlock = 128; // rows up to which one block does everything
+constexpr int kRouteSums = 256;     // blocks up to which each sums the counts of those before it by itself
 constexpr int kMaxExperts = 1024, kMaxTopK = 16;
+
+// Rows per block: as many blocks as there are SMs to fill with a pass of 64 rows or more.
+int route_block_rows(int64_t rows) {
+    if (rows <= kRouteOneBlock) return kRouteOneBlock;
+    return (int)std::min<int64_t>(kRouteRows, (rows + 147) / 148 <= 64 ? 64 : ((rows + 147) / 148 + 63) / 64 * 64);
+}
+int64_t route_blocks(int64_t rows) { return (rows + route_block_rows(rows) - 1) / route_block_rows(rows); }
 
 // Order-preserving image of a float; 0 for what is never chosen (-inf, NaN).  +inf counts as the largest finite value, -0 as 0.
 __device__ __forceinline__ uint32_t route_key(float x) {
@@ -29,167 +38,289 @@ __device__ __forceinline__ float route_value(uint32_t k) {
     return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
 
-// A warp per row, the row's experts in registers (PER a lane, expert = 32 i + lane).  Each of the k rounds takes the largest
-// key and, among equal ones, the lowest expert.
-template <int PER, typename T>
-__device__ __forceinline__ void route_row(const RouteArgs& p, int row, int lane, int32_t* chosen) {
-    const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.ld;
+// LANES lanes take a row, PER neighbouring experts each, in registers.  Each of the k rounds takes the largest key and, among
+// equal ones, the lowest expert.  `live`: the row exists (its lanes take part in the shuffles either way).
+template <int LANES, int PER, typename T>
+__device__ __forceinline__ void route_row(const RouteArgs& p, int row, bool live, int lane, int16_t* chosen) {
+    const int l = lane % LANES;
     uint32_t key[PER];
+    if (live) {
+        const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.ld;
+        constexpr int kVec = 16 / (int)sizeof(T);
+        if (PER % kVec == 0 && p.vec) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int e = 32 * i + lane;
-        float v = -INFINITY;
-        if (e < p.n_experts) {
-            if constexpr (sizeof(T) == 2) v = __bfloat162float(x[e]);
-            else v = x[e];
+            for (int i = 0; i < PER; i += kVec) {
+                uint32_t w[4] = {0, 0, 0, 0};
+                const bool in = l * PER + i < p.n_experts;
+                if (in) {
+                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(x + l * PER + i));
+                    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+                }
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) {
+                    float f;
+                    if constexpr (sizeof(T) == 2) f = __uint_as_float(j % 2 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+                    else f = __uint_as_float(w[j]);
+                    key[(i + j) % PER] = in ? route_key(f) : 0u;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) key[i] = l * PER + i < p.n_experts ? route_key((float)x[l * PER + i]) : 0u;
         }
-        key[i] = route_key(v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) key[i] = 0u;
     }
-    uint32_t most = 0;
+    float top = 0.0f, total = 0.0f;
+    constexpr int kKeep = (kMaxTopK + LANES - 1) / LANES;  // lane l keeps the choices l, l + LANES, ...
+    float mine[kKeep];
+    int who[kKeep];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) most = max(most, key[i]);
-    most = __reduce_max_sync(0xffffffffu, most);
-    const float top = most ? route_value(most) : 0.0f;
-    float total = 0.0f;
-    if (!p.normalize) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-            if (key[i]) total += expf(route_value(key[i]) - top);
-#pragma unroll
-        for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
-    }
-    float mine = 0.0f;  // lane j: the j-th choice
-    int who = -1;
+    for (int i = 0; i < kKeep; ++i) { mine[i] = 0.0f; who[i] = -1; }
     for (int j = 0; j < p.top_k; ++j) {
         uint32_t best = 0;
         int at = 0;
 #pragma unroll
         for (int i = 0; i < PER; ++i)
-            if (key[i] > best) { best = key[i]; at = 32 * i + lane; }
-        const uint32_t all = __reduce_max_sync(0xffffffffu, best);
-        if (!all) break;
-        const int e = (int)__reduce_min_sync(0xffffffffu, best == all ? (uint32_t)at : 0xffffffffu);
+            if (key[i] > best) { best = key[i]; at = l * PER + i; }
 #pragma unroll
-        for (int i = 0; i < PER; ++i)
-            if (32 * i + lane == e) key[i] = 0;
-        const float w = expf(route_value(all) - top);
-        if (p.normalize) total += w;
-        if (lane == j) { mine = w; who = e; }
+        for (int d = LANES / 2; d; d >>= 1) {
+            const uint32_t ob = __shfl_xor_sync(0xffffffffu, best, d);
+            const int oa = __shfl_xor_sync(0xffffffffu, at, d);
+            if (ob > best || (ob == best && oa < at)) { best = ob; at = oa; }
+        }
+        if (j == 0) {
+            top = best ? route_value(best) : 0.0f;
+            if (!p.normalize) {
+#pragma unroll
+                for (int i = 0; i < PER; ++i)
+                    if (key[i]) total += expf(route_value(key[i]) - top);
+#pragma unroll
+                for (int d = LANES / 2; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+            }
+        }
+        if (best) {
+            const float w = expf(route_value(best) - top);
+            if (p.normalize) total += w;
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (l * PER + i == at) key[i] = 0;
+#pragma unroll
+            for (int i = 0; i < kKeep; ++i)
+                if (l + i * LANES == j) { mine[i] = w; who[i] = at; }
+        }
     }
-    if (lane < p.top_k) {
-        p.experts[(int64_t)row * p.top_k + lane] = who;
-        p.weights[(int64_t)row * p.top_k + lane] = who >= 0 ? mine / total : 0.0f;
-        chosen[lane] = who;
+    if (!live) return;
+    const int64_t out = (int64_t)row * p.top_k;
+#pragma unroll
+    for (int i = 0; i < kKeep; ++i) {
+        const int j = l + i * LANES;
+        if (j >= p.top_k) break;
+        p.experts[out + j] = who[i];
+        p.weights[out + j] = who[i] >= 0 ? mine[i] / total : 0.0f;
+        chosen[j] = (int16_t)who[i];
     }
 }
 
-// The choice, and how often each expert was chosen in this block's rows: counts[block][expert].
-template <int PER, typename T>
-__global__ void __launch_bounds__(kRouteWarps * 32) route_choose_kernel(const RouteArgs p) {
-    __shared__ int32_t chosen[kRouteRows * kMaxTopK];
-    __shared__ int32_t count[kMaxExperts];
+// Exclusive sums over the block's threads (thread = expert); *all: the sum of all.
+__device__ __forceinline__ int block_before(int n, int* warp_sum, int* all) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int row0 = blockIdx.x * kRouteRows, rows = min(kRouteRows, p.rows - row0);
-    for (int e = threadIdx.x; e < p.n_experts; e += blockDim.x) count[e] = 0;
-    __syncthreads();
-    pdl_wait();
-    pdl_trigger();
-    for (int r = warp; r < rows; r += kRouteWarps) route_row<PER, T>(p, row0 + r, lane, chosen + r * p.top_k);
-    __syncthreads();
-    for (int i = threadIdx.x; i < rows * p.top_k; i += blockDim.x)
-        if (chosen[i] >= 0) atomicAdd(&count[chosen[i]], 1);
-    __syncthreads();
-    for (int e = threadIdx.x; e < p.n_experts; e += blockDim.x) p.work[(int64_t)blockIdx.x * p.n_experts + e] = count[e];
-}
-
-// counts[block][expert] -> the place of the block's first row of that expert; offsets.
-__global__ void __launch_bounds__(1024) route_scan_kernel(const RouteArgs p, int blocks) {
-    __shared__ int32_t warp_sum[32];
-    const int e = threadIdx.x, warp = e >> 5, lane = e & 31;
-    pdl_wait();
-    pdl_trigger();
-    int total = 0;
-    if (e < p.n_experts) {
-#pragma unroll 8
-        for (int b = 0; b < blocks; ++b) total += p.work[(int64_t)b * p.n_experts + e];
-    }
-    int upto = total;
+    int upto = n;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, upto, d);
         if (lane >= d) upto += v;
     }
+    __syncthreads();
     if (lane == 31) warp_sum[warp] = upto;
     __syncthreads();
-    if (warp == 0) {
-        int s = lane < (int)(blockDim.x >> 5) ? warp_sum[lane] : 0;
+    int before = 0, sum = 0;
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, s, d);
-            if (lane >= d) s += v;
-        }
-        warp_sum[lane] = s;
+    for (int w = 0; w < kRouteWarps; ++w) {
+        if (w < warp) before += warp_sum[w];
+        sum += warp_sum[w];
+    }
+    *all = sum;
+    return before + upto - n;
+}
+
+// The block's choices (in shared memory, in order) to their places.  base[e]: the first place of the block's rows of expert e.
+// Each warp takes a run of them, 32 at a time: equal experts are ranked by their lanes, behind those of the chunks and warps
+// before.  Called by the whole block; part: [kRouteWarps][n_experts].
+__device__ __forceinline__ void route_place(const RouteArgs& p, const int16_t* chosen, const int* base, uint16_t* part, int64_t first, int n) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int run = (n + kRouteWarps * 32 - 1) / (kRouteWarps * 32) * 32, lo = min(warp * run, n), hi = min(lo + run, n);
+    for (int i = threadIdx.x; i < kRouteWarps * p.n_experts; i += kRouteThreads) part[i] = 0;
+    __syncthreads();
+    uint16_t* count = part + warp * p.n_experts;
+    for (int i0 = lo; i0 < hi; i0 += 32) {
+        const int e = i0 + lane < hi ? chosen[i0 + lane] : -1;
+        const uint32_t same = __match_any_sync(0xffffffffu, e);
+        if (e >= 0 && (same >> lane) == 1u) count[e] += (uint16_t)__popc(same);  // the last of its kind
+        __syncwarp();
     }
     __syncthreads();
-    if (warp) upto += warp_sum[warp - 1];
-    if (e < p.n_experts) {
-        int at = upto - total;
-        p.offsets[e] = at;
-        if (e == p.n_experts - 1) p.offsets[p.n_experts] = upto;
-        for (int b = 0; b < blocks; ++b) {
-            int32_t* c = p.work + (int64_t)b * p.n_experts + e;
-            const int n = *c;
-            *c = at;
-            at += n;
+    for (int e = threadIdx.x; e < p.n_experts; e += kRouteThreads) {
+        uint32_t at = 0;
+        for (int w = 0; w < kRouteWarps; ++w) {
+            const uint32_t c = part[w * p.n_experts + e];
+            part[w * p.n_experts + e] = (uint16_t)at;
+            at += c;
         }
+    }
+    __syncthreads();
+    for (int i0 = lo; i0 < hi; i0 += 32) {
+        const int e = i0 + lane < hi ? chosen[i0 + lane] : -1;
+        const uint32_t same = __match_any_sync(0xffffffffu, e);
+        int at = -1, rank = 0;
+        if (e >= 0) {
+            rank = count[e] + __popc(same & ((1u << lane) - 1u));
+            at = base[e] + rank;
+        }
+        __syncwarp();
+        if (e >= 0 && (same >> lane) == 1u) count[e] = (uint16_t)(rank + 1);
+        __syncwarp();
+        if (i0 + lane < hi) p.slots[first + i0 + lane] = at;
+        if (at >= 0) p.order[at] = (int)((first + i0 + lane) / p.top_k);
     }
 }
 
-// Rows of a block to their places, in order: one warp, 32 choices at a time, equal experts ranked by their lanes.
-__global__ void __launch_bounds__(256) route_place_kernel(const RouteArgs p) {
-    __shared__ int32_t next[kMaxExperts];
-    const int lane = threadIdx.x & 31;
+// The choice, and how often each expert was chosen by this block's rows: table[expert][block].  One block alone goes on to the
+// places.
+template <int LANES, int PER, typename T>
+__global__ void __launch_bounds__(kRouteThreads) route_choose_kernel(const RouteArgs p, int block_rows, int blocks) {
+    __shared__ int16_t chosen[kRouteRows * kMaxTopK];
+    __shared__ int32_t count[kMaxExperts];
+    __shared__ int warp_sum[kRouteWarps];
+    extern __shared__ uint16_t part[];  // one block alone
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int row0 = blockIdx.x * block_rows, rows = min(block_rows, p.rows - row0);
+    for (int e = threadIdx.x; e < p.n_experts; e += kRouteThreads) count[e] = 0;
     pdl_wait();
     pdl_trigger();
-    for (int e = threadIdx.x; e < p.n_experts; e += blockDim.x) next[e] = p.work[(int64_t)blockIdx.x * p.n_experts + e];
-    const int used = p.offsets[p.n_experts];
-    const int64_t first = (int64_t)blockIdx.x * kRouteRows * p.top_k;
-    const int64_t end = min(first + (int64_t)kRouteRows * p.top_k, (int64_t)p.rows * p.top_k);
-    for (int64_t i = first + threadIdx.x; i < end; i += blockDim.x)
-        if (i >= used) p.order[i] = -1;
-    __syncthreads();
-    if (threadIdx.x >= 32) return;
-    for (int64_t i0 = first; i0 < end; i0 += 32) {
-        const int64_t i = i0 + lane;
-        const int e = i < end ? p.experts[i] : -1;
-        const uint32_t same = __match_any_sync(0xffffffffu, e);
-        int at = -1;
-        if (e >= 0) at = next[e] + __popc(same & ((1u << lane) - 1u));
-        __syncwarp();
-        if (e >= 0 && (same >> lane) == 1u) next[e] = at + 1;  // the last of its kind
-        __syncwarp();
-        if (i < end) p.slots[i] = at;
-        if (at >= 0) p.order[at] = (int)(i / p.top_k);
+    constexpr int kPer = 32 / LANES;  // rows of a warp at once
+    for (int r0 = warp * kPer; r0 < rows; r0 += kRouteWarps * kPer) {
+        const int r = r0 + lane / LANES;
+        route_row<LANES, PER, T>(p, row0 + r, r < rows, lane, chosen + min(r, rows - 1) * p.top_k);
     }
+    __syncthreads();
+    const int n = rows * p.top_k;
+    for (int i = threadIdx.x; i < n; i += kRouteThreads)
+        if (chosen[i] >= 0) atomicAdd(&count[chosen[i]], 1);
+    __syncthreads();
+    if (blocks > 1) {
+        for (int e = threadIdx.x; e < p.n_experts; e += kRouteThreads) p.work[(int64_t)e * (blocks + 1) + blockIdx.x] = count[e];
+        return;
+    }
+    int used = 0;
+    for (int e0 = 0; e0 < p.n_experts; e0 += kRouteThreads) {
+        const int e = e0 + threadIdx.x;
+        int all;
+        const int at = used + block_before(e < p.n_experts ? count[e] : 0, warp_sum, &all);
+        if (e < p.n_experts) {
+            p.offsets[e] = at;
+            count[e] = at;
+        }
+        used += all;
+    }
+    if (threadIdx.x == 0) p.offsets[p.n_experts] = used;
+    for (int i = used + threadIdx.x; i < n; i += kRouteThreads) p.order[i] = -1;
+    __syncthreads();
+    route_place(p, chosen, count, part, 0, n);
 }
 
-template <typename T>
-cudaError_t route_choose(const RouteArgs& g, int blocks, cudaStream_t st) {
-    const int per = (g.n_experts + 31) / 32;
-    const int threads = kRouteWarps * 32;
-    if (per <= 1) return launch_pdl(route_choose_kernel<1, T>, dim3(blocks), threads, 0, st, 1, g);
-    if (per <= 2) return launch_pdl(route_choose_kernel<2, T>, dim3(blocks), threads, 0, st, 1, g);
-    if (per <= 4) return launch_pdl(route_choose_kernel<4, T>, dim3(blocks), threads, 0, st, 1, g);
-    if (per <= 8) return launch_pdl(route_choose_kernel<8, T>, dim3(blocks), threads, 0, st, 1, g);
-    return launch_pdl(route_choose_kernel<32, T>, dim3(blocks), threads, 0, st, 1, g);
+// Many blocks: table[expert][block] -> the sums of the blocks before, [blocks] the sum of all; a warp per expert.
+__global__ void __launch_bounds__(256) route_sums_kernel(const RouteArgs p, int blocks) {
+    const int e = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    pdl_wait();
+    pdl_trigger();
+    if (e >= p.n_experts) return;
+    int32_t* row = p.work + (int64_t)e * (blocks + 1);
+    int before = 0;
+    for (int b0 = 0; b0 < blocks; b0 += 32) {
+        const int n = b0 + lane < blocks ? row[b0 + lane] : 0;
+        int upto = n;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += v;
+        }
+        if (b0 + lane < blocks) row[b0 + lane] = before + upto - n;
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    if (lane == 0) row[blocks] = before;
 }
+
+// The places of a block's rows: what the blocks before it hold of every expert, what all hold, then the block's own order.
+__global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteArgs p, int block_rows, int blocks) {
+    __shared__ int16_t chosen[kRouteRows * kMaxTopK];
+    __shared__ int32_t base[kMaxExperts], total[kMaxExperts];
+    __shared__ int warp_sum[kRouteWarps];
+    extern __shared__ uint16_t part[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, block = blockIdx.x;
+    const int64_t first = (int64_t)block * block_rows * p.top_k;
+    const int n = (int)min((int64_t)block_rows * p.top_k, (int64_t)p.rows * p.top_k - first);
+    pdl_wait();
+    pdl_trigger();
+    for (int i = threadIdx.x; i < n; i += kRouteThreads) chosen[i] = (int16_t)p.experts[first + i];
+    if (blocks > kRouteSums) {
+        for (int e = threadIdx.x; e < p.n_experts; e += kRouteThreads) {
+            base[e] = p.work[(int64_t)e * (blocks + 1) + block];
+            total[e] = p.work[(int64_t)e * (blocks + 1) + blocks];
+        }
+    } else {
+        for (int e = warp; e < p.n_experts; e += kRouteWarps) {
+            const int32_t* row = p.work + (int64_t)e * (blocks + 1);
+            int before = 0, all = 0;
+#pragma unroll
+            for (int i = 0; i < kRouteSums / 32; ++i) {
+                const int b = i * 32 + lane;
+                const int c = b < blocks ? row[b] : 0;
+                all += c;
+                if (b < block) before += c;
+            }
+            before = __reduce_add_sync(0xffffffffu, before);
+            all = __reduce_add_sync(0xffffffffu, all);
+            if (lane == 0) { base[e] = before; total[e] = all; }
+        }
+    }
+    __syncthreads();
+    int used = 0;
+    for (int e0 = 0; e0 < p.n_experts; e0 += kRouteThreads) {
+        const int e = e0 + threadIdx.x;
+        int all;
+        const int at = used + block_before(e < p.n_experts ? total[e] : 0, warp_sum, &all);
+        if (e < p.n_experts) {
+            base[e] += at;
+            if (block == 0) p.offsets[e] = at;
+        }
+        used += all;
+    }
+    if (block == 0 && threadIdx.x == 0) p.offsets[p.n_experts] = used;
+    for (int64_t i = max(first, (int64_t)used) + threadIdx.x; i < first + n; i += kRouteThreads) p.order[i] = -1;
+    __syncthreads();
+    route_place(p, chosen, base, part, first, n);
+}
+
+// fn(kernel) for the form of the choice that a number of experts takes
+template <typename T, typename Fn>
+cudaError_t route_form(int n_experts, Fn fn) {
+    if (n_experts <= 32) return fn(route_choose_kernel<4, 8, T>);
+    if (n_experts <= 64) return fn(route_choose_kernel<8, 8, T>);
+    if (n_experts <= 128) return fn(route_choose_kernel<8, 16, T>);
+    if (n_experts <= 256) return fn(route_choose_kernel<16, 16, T>);
+    return fn(route_choose_kernel<32, 32, T>);
+}
+size_t route_part_bytes(int n_experts) { return (size_t)kRouteWarps * n_experts * sizeof(uint16_t); }
 
 // out[row] (+)= alpha sum_j weights[row][j] y[slots[row][j]], in 32 bits in the order of j, rounded once.  A thread takes eight
-// columns where rows lie on 16-byte boundaries, else one.
+// columns where rows lie on 16-byte boundaries, else one; four results' pieces are asked for at once.
 template <typename Y, int PER>
 __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs p) {
     pdl_wait();
     pdl_trigger();
+    constexpr int kAhead = 4, kWords = PER * (int)sizeof(Y) / 16 > 0 ? PER * (int)sizeof(Y) / 16 : 1;
     const int groups = (p.cols + PER - 1) / PER;
     const int64_t total = (int64_t)p.rows * groups;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
@@ -197,28 +328,48 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs p) {
         float sum[PER];
 #pragma unroll
         for (int c = 0; c < PER; ++c) sum[c] = 0.0f;
-        for (int j = 0; j < p.top_k; ++j) {
-            const int at = __ldg(p.slots + (int64_t)row * p.top_k + j);
-            if ((unsigned)at >= (unsigned long long)p.y_rows) continue;
-            const float w = p.weights ? __ldg(p.weights + (int64_t)row * p.top_k + j) : 1.0f;
-            const Y* y = static_cast<const Y*>(p.y) + (int64_t)at * p.ldy + col;
-            if constexpr (PER == 8 && sizeof(Y) == 2) {
-                const uint4 v = __ldg(reinterpret_cast<const uint4*>(y));
-                const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+        for (int j0 = 0; j0 < p.top_k; j0 += kAhead) {
+            int at[kAhead];
+            float w[kAhead];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    sum[2 * c] = fmaf(w, __uint_as_float(u[c] << 16), sum[2 * c]);
-                    sum[2 * c + 1] = fmaf(w, __uint_as_float(u[c] & 0xffff0000u), sum[2 * c + 1]);
-                }
-            } else if constexpr (PER == 8) {
+            for (int j = 0; j < kAhead; ++j) {
+                const int64_t k = (int64_t)row * p.top_k + j0 + j;
+                at[j] = j0 + j < p.top_k ? __ldg(p.slots + k) : -1;
+                if ((unsigned)at[j] >= (unsigned long long)p.y_rows) at[j] = -1;
+                w[j] = at[j] >= 0 ? (p.weights ? __ldg(p.weights + k) : 1.0f) : 0.0f;
+            }
+            if constexpr (PER == 8) {
+                uint4 v[kAhead][kWords];
 #pragma unroll
-                for (int c = 0; c < 8; c += 4) {
-                    const float4 v = __ldg(reinterpret_cast<const float4*>(y + c));
-                    sum[c] = fmaf(w, v.x, sum[c]); sum[c + 1] = fmaf(w, v.y, sum[c + 1]);
-                    sum[c + 2] = fmaf(w, v.z, sum[c + 2]); sum[c + 3] = fmaf(w, v.w, sum[c + 3]);
+                for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+                    for (int q = 0; q < kWords; ++q) {
+                        v[j][q] = make_uint4(0, 0, 0, 0);
+                        if (at[j] >= 0) v[j][q] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const Y*>(p.y) + (int64_t)at[j] * p.ldy + col) + q);
+                    }
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) {
+                    if (at[j] < 0) continue;
+                    if constexpr (sizeof(Y) == 2) {
+                        const uint32_t u[4] = {v[j][0].x, v[j][0].y, v[j][0].z, v[j][0].w};
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            sum[2 * c] = fmaf(w[j], __uint_as_float(u[c] << 16), sum[2 * c]);
+                            sum[2 * c + 1] = fmaf(w[j], __uint_as_float(u[c] & 0xffff0000u), sum[2 * c + 1]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < kWords; ++q) {
+                            const uint32_t u[4] = {v[j][q].x, v[j][q].y, v[j][q].z, v[j][q].w};
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) sum[4 * q + c] = fmaf(w[j], __uint_as_float(u[c]), sum[4 * q + c]);
+                        }
+                    }
                 }
             } else {
-                sum[0] = fmaf(w, (float)y[0], sum[0]);
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j)
+                    if (at[j] >= 0) sum[0] = fmaf(w[j], (float)static_cast<const Y*>(p.y)[(int64_t)at[j] * p.ldy + col], sum[0]);
             }
         }
         if (p.out_mode == kOutBf16) {
@@ -256,18 +407,40 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs p) {
 }  // namespace
 
 int64_t route_work_bytes(int64_t rows, int64_t n_experts, int64_t) {
-    return (rows + kRouteRows - 1) / kRouteRows * n_experts * (int64_t)sizeof(int32_t);
+    const int64_t blocks = route_blocks(rows);
+    return blocks > 1 ? n_experts * (blocks + 1) * (int64_t)sizeof(int32_t) : 0;
 }
 
-cudaError_t route_launch(const RouteArgs& g, cudaStream_t stream, int64_t* launches) {
-    if (g.rows <= 0) return cudaMemsetAsync(g.offsets, 0, sizeof(int32_t) * (g.n_experts + 1), stream);
-    const int blocks = (g.rows + kRouteRows - 1) / kRouteRows;
-    cudaError_t e = g.bf16 ? route_choose<__nv_bfloat16>(g, blocks, stream) : route_choose<float>(g, blocks, stream);
-    if (e != cudaSuccess) return e;
-    e = launch_pdl(route_scan_kernel, dim3(1), (g.n_experts + 31) / 32 * 32, 0, stream, 1, g, blocks);
-    if (e != cudaSuccess) return e;
-    *launches += 3;
-    return launch_pdl(route_place_kernel, dim3(blocks), 256, 0, stream, 1, g);
+cudaError_t route_configure() {
+    const int most = (int)route_part_bytes(kMaxExperts);
+    cudaError_t e = cudaFuncSetAttribute(route_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    auto set = [&](auto kernel) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most); };
+    for (int n : {32, 64, 128, 256, 1024}) {
+        if (e == cudaSuccess) e = route_form<float>(n, set);
+        if (e == cudaSuccess) e = route_form<__nv_bfloat16>(n, set);
+    }
+    return e;
+}
+
+cudaError_t route_launch(const RouteArgs& args, cudaStream_t stream, int64_t* launches) {
+    if (args.rows <= 0) return cudaMemsetAsync(args.offsets, 0, sizeof(int32_t) * (args.n_experts + 1), stream);
+    RouteArgs g = args;
+    const int eb = g.bf16 ? 2 : 4;
+    g.vec = !(reinterpret_cast<uintptr_t>(g.logits) & 15) && !((g.ld * eb) & 15) && !((g.n_experts * eb) & 15);
+    const int block_rows = route_block_rows(g.rows), blocks = (int)route_blocks(g.rows);
+    auto choose = [&](auto kernel) {
+        return launch_pdl(kernel, dim3(blocks), kRouteThreads, blocks == 1 ? route_part_bytes(g.n_experts) : 0, stream, 1, g, block_rows, blocks);
+    };
+    cudaError_t e = g.bf16 ? route_form<__nv_bfloat16>(g.n_experts, choose) : route_form<float>(g.n_experts, choose);
+    *launches += 1;
+    if (e != cudaSuccess || blocks == 1) return e;
+    if (blocks > kRouteSums) {
+        e = launch_pdl(route_sums_kernel, dim3((g.n_experts + 7) / 8), 256, 0, stream, 1, g, blocks);
+        *launches += 1;
+        if (e != cudaSuccess) return e;
+    }
+    *launches += 1;
+    return launch_pdl(route_place_kernel, dim3(blocks), kRouteThreads, route_part_bytes(g.n_experts), stream, 1, g, block_rows, blocks);
 }
 
 cudaError_t combine_launch(const CombineArgs& g, cudaStream_t stream) {

@@ -68,10 +68,12 @@ struct RouteArgs {
     int64_t ld;
     int rows, n_experts, top_k;
     bool bf16, normalize;
+    bool vec;  // rows and their parts lie on 16-byte boundaries (set by route_launch)
     int32_t *experts, *offsets, *order, *slots;
     float* weights;
     int32_t* work;
 };
+cudaError_t route_configure();
 int64_t route_work_bytes(int64_t rows, int64_t n_experts, int64_t top_k);
 cudaError_t route_launch(const RouteArgs& g, cudaStream_t stream, int64_t* launches);
 

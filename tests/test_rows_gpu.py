@@ -67,14 +67,13 @@ def route_ref(x, k, normalize):
     ids = np.where(np.isneginf(top), -1, ids)
     w = np.where(ids < 0, 0.0, w)
     flat = ids.reshape(-1)
-    order, slots, offsets = [], np.full(T * k, -1), [0]
-    for e in range(E):
-        for i in np.flatnonzero(flat == e):
-            slots[i] = len(order)
-            order.append(i // k)
-        offsets.append(len(order))
-    order += [-1] * (T * k - len(order))
-    return ids, w, np.array(offsets), np.array(order), slots.reshape(T, k)
+    taken = np.flatnonzero(flat >= 0)
+    placed = taken[np.argsort(flat[taken], kind="stable")]
+    offsets = np.concatenate([[0], np.cumsum(np.bincount(flat[taken], minlength=E))])
+    order, slots = np.full(T * k, -1), np.full(T * k, -1)
+    order[:placed.size] = placed // k
+    slots[placed] = np.arange(placed.size)
+    return ids, w, offsets, order, slots.reshape(T, k)
 
 
 def run_route(ctx, x, k, normalize, ld=None):
@@ -106,7 +105,8 @@ def check_route(out, x, k, normalize):
 
 @pytest.mark.parametrize("T,E,k,bf16,normalize", [(1, 1, 1, False, True), (1, 4, 2, False, True), (24, 32, 2, False, True), (127, 33, 3, True, False),
                                                   (128, 64, 4, True, True), (129, 65, 8, False, False), (1000, 128, 4, True, False),
-                                                  (777, 300, 16, False, True), (300, 1024, 5, True, False), (5000, 7, 7, False, False)])
+                                                  (777, 300, 16, False, True), (90, 20, 16, True, False), (128, 1024, 16, False, True), (3000, 1000, 16, True, False),
+                                                  (140001, 9, 2, True, True), (20000, 256, 3, False, False), (300, 1024, 5, True, False), (5000, 7, 7, False, False)])
 def test_route(ctx, T, E, k, bf16, normalize):
     g = gen(T * 31 + E)
     x = randn(g, T, E, std=1.5).to(torch.bfloat16 if bf16 else torch.float32)

@@ -2,8 +2,8 @@
 // the rows of every tile of the product the list of the adapters among them, in the order of their first rows.
 //
 // Bound by reading the rows once (2 K bytes each against K * rank products).  Two kernels:
-//   - many rows: 128 rows a CTA on tcgen05, rows and adapters through a TMA ring, one pass over K for each adapter among the rows
-//     with the lanes of the other rows disabled (nothing of one adapter reaches another's rows).
+//   - many rows: 128 rows a CTA on tcgen05, rows and adapters through a TMA ring; a pass over K for every few adapters among the
+//     rows, each with the lanes of the other rows disabled (nothing of one adapter reaches another's rows).
 //   - few rows: 16 rows a block on mma.sync m16n8k16 with operands straight from global memory, K over the warps, the columns over
 //     blocks; a row takes its adapter's product (selected, not masked by zeros).
 // Where nearly every row has its own adapter (live streams), such passes would run one after the other; there a row is a chain of
@@ -11,6 +11,8 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+
+#include <algorithm>
 
 #include "launch.cuh"
 #include "rows.h"
@@ -196,15 +198,18 @@ __global__ void __launch_bounds__(kDownWarps * 32) adapter_down_kernel(const Ada
 }
 
 // ---------------------------------------------------------------------------------------------- many rows: tcgen05
-constexpr int kTcRows = 128, kTcStages = 4, kTcThreads = 192;
-constexpr int kTcMaxPasses = 12;  // adapters in 128 rows above which the rows are taken one by one
+constexpr int kTcRows = 128, kTcMaxStages = 8, kTcThreads = 192;
+constexpr int kTcMaxPasses = 6;  // passes above which the rows are taken one by one
 
 constexpr int tc_cols(int rank) { return rank <= 16 ? 16 : (rank <= 32 ? 32 : (rank <= 64 ? 64 : 128)); }
 template <int RN>
 struct DownTc {
-    static constexpr int kABytes = kTcRows * 128, kBBytes = RN * 128, kStageBytes = kABytes + kBBytes;
-    static constexpr int kSmemBytes = kTcStages * kStageBytes + 128 + 1024;
+    static constexpr int kAtOnce = RN <= 32 ? 4 : (RN == 64 ? 2 : 1);  // adapters of a pass
+    static constexpr int kABytes = kTcRows * 128, kOneBytes = RN * 128, kBBytes = kAtOnce * kOneBytes, kStageBytes = kABytes + kBBytes;
     static constexpr uint32_t kTmemCols = RN < 32 ? 32 : RN;
+    static constexpr int smem_bytes(int stages) { return stages * kStageBytes + 256 + 1024; }
+    // all of an SM's shared memory where every CTA has one to itself, else half of it
+    static constexpr int stages(bool alone) { return std::min((alone ? 224 : 110) * 1024 / kStageBytes, kTcMaxStages); }
 };
 
 // The adapters among 128 rows, four rows a lane, in the order of their first rows; -1 after the last one.
@@ -236,22 +241,22 @@ struct IdWalk {
 // Warp 0 loads, warp 1 issues the MMAs, warps 2 to 5 read the results, a row per thread.
 template <int RN>
 __global__ void __launch_bounds__(kTcThreads) adapter_down_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_d,
-                                                                     const AdapterDownArgs p, int* __restrict__ error) {
+                                                                     const AdapterDownArgs p, int stages, int* __restrict__ error) {
     using namespace ptx;
     using C = DownTc<RN>;
     extern __shared__ unsigned char smem_dyn[];
     const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
     unsigned char* base_ptr = smem_dyn + (base - smem_u32(smem_dyn));
-    const uint32_t a_base = base, b_base = base + kTcStages * C::kABytes, bar_base = base + kTcStages * C::kStageBytes;
+    const uint32_t a_base = base, b_base = base + stages * C::kABytes, bar_base = base + stages * C::kStageBytes;
     auto full_bar = [&](int s) { return bar_base + 8u * s; };
-    auto empty_bar = [&](int s) { return bar_base + 8u * (kTcStages + s); };
-    const uint32_t done_bar = bar_base + 8u * (2 * kTcStages);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + kTcStages * C::kStageBytes + 8 * (2 * kTcStages + 1));
+    auto empty_bar = [&](int s) { return bar_base + 8u * (kTcMaxStages + s); };
+    const uint32_t done_bar = bar_base + 8u * (2 * kTcMaxStages);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + stages * C::kStageBytes + 8 * (2 * kTcMaxStages + 1));
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = warp_index(), lane = threadIdx.x & 31;
     const int row0 = blockIdx.x * kTcRows, k_tiles = (p.K + 63) / 64;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kTcStages; ++s) {
+        for (int s = 0; s < stages; ++s) {
             mbar_init(full_bar(s), 1);
             mbar_init(empty_bar(s), 1);
         }
@@ -270,35 +275,40 @@ __global__ void __launch_bounds__(kTcThreads) adapter_down_tc_kernel(const __gri
     pdl_wait();
     pdl_trigger();
     // every warp counts the adapters for itself
-    int passes = 0;
+    int found = 0;
     {
         IdWalk w(p, row0, lane);
-        while (passes <= kTcMaxPasses && w.next() >= 0) ++passes;
+        while (found <= kTcMaxPasses * C::kAtOnce && w.next() >= 0) ++found;
     }
-    const bool dots = passes > kTcMaxPasses;
+    const bool dots = found > kTcMaxPasses * C::kAtOnce;
 
     if (warp == 0 && !dots) {
         IdWalk w(p, row0, lane);
         int stage = 0;
         uint32_t ph = 0;
         bool ok = true;
-        for (int id = w.next(); ok && id >= 0; id = w.next()) {
+        for (int left = found; ok && left > 0; left -= C::kAtOnce) {
+            int id[C::kAtOnce];
+#pragma unroll
+            for (int e = 0; e < C::kAtOnce; ++e) id[e] = w.next();
             bool failed = false;
             if (elect_one()) {
                 int s = stage;
                 uint32_t sp = ph;
                 for (int kt = 0; kt < k_tiles; ++kt) {
                     if (!mbar_wait(empty_bar(s), sp ^ 1, abort_flag)) { failed = true; break; }
-                    mbar_expect_tx(full_bar(s), C::kStageBytes);
+                    mbar_expect_tx(full_bar(s), C::kABytes + min(left, C::kAtOnce) * C::kOneBytes);
                     tma_load_2d(a_base + s * C::kABytes, &tma_a, full_bar(s), kt * 64, row0);
-                    tma_load_2d(b_base + s * C::kBBytes, &tma_d, full_bar(s), kt * 64, id * p.rank);
-                    if (++s == kTcStages) { s = 0; sp ^= 1; }
+#pragma unroll
+                    for (int e = 0; e < C::kAtOnce; ++e)
+                        if (e < left) tma_load_2d(b_base + s * C::kBBytes + e * C::kOneBytes, &tma_d, full_bar(s), kt * 64, id[e] * p.rank);
+                    if (++s == stages) { s = 0; sp ^= 1; }
                 }
             }
             ok = !__any_sync(0xffffffffu, failed);
             stage += k_tiles;
-            ph ^= (uint32_t)(stage / kTcStages) & 1u;
-            stage %= kTcStages;
+            ph ^= (uint32_t)(stage / stages) & 1u;
+            stage %= stages;
         }
         if (!ok) {
             const long long t0 = clock64();
@@ -314,10 +324,14 @@ __global__ void __launch_bounds__(kTcThreads) adapter_down_tc_kernel(const __gri
         int stage = 0;
         uint32_t ph = 0;
         bool ok = true;
-        for (int id = w.next(); ok && id >= 0; id = w.next()) {
-            uint32_t off[4];
+        for (int left = found; ok && left > 0; left -= C::kAtOnce) {
+            uint32_t off[C::kAtOnce][4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) off[q] = ~__ballot_sync(0xffffffffu, mine[q] == id);
+            for (int e = 0; e < C::kAtOnce; ++e) {
+                const int id = w.next();
+#pragma unroll
+                for (int q = 0; q < 4; ++q) off[e][q] = ~__ballot_sync(0xffffffffu, mine[q] == id);
+            }
             bool failed = false;
             if (elect_one()) {
                 int s = stage;
@@ -327,15 +341,20 @@ __global__ void __launch_bounds__(kTcThreads) adapter_down_tc_kernel(const __gri
                     tc_fence_after();
                     const uint64_t adesc = make_smem_desc(a_base + s * C::kABytes), bdesc = make_smem_desc(b_base + s * C::kBBytes);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) tc_mma_lanes(tmem, adesc + 2 * i, bdesc + 2 * i, idesc, off, (kt | i) ? 1u : 0u);
+                    for (int e = 0; e < C::kAtOnce; ++e) {
+                        if (e >= left) break;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            tc_mma_lanes(tmem, adesc + 2 * i, bdesc + e * (C::kOneBytes / 16) + 2 * i, idesc, off[e], (kt | i) ? 1u : 0u);
+                    }
                     tc_commit(empty_bar(s));
-                    if (++s == kTcStages) { s = 0; sp ^= 1; }
+                    if (++s == stages) { s = 0; sp ^= 1; }
                 }
             }
             ok = !__any_sync(0xffffffffu, failed);
             stage += k_tiles;
-            ph ^= (uint32_t)(stage / kTcStages) & 1u;
-            stage %= kTcStages;
+            ph ^= (uint32_t)(stage / stages) & 1u;
+            stage %= stages;
         }
         if (ok && elect_one()) tc_commit(done_bar);
         __syncwarp();
@@ -391,11 +410,12 @@ __global__ void __launch_bounds__(kTcThreads) adapter_down_tc_kernel(const __gri
 }
 
 template <int RN>
-cudaError_t down_tc_t(const AdapterDownArgs& g, int* d_error, cudaStream_t stream) {
+cudaError_t down_tc_t(const AdapterDownArgs& g, int sm_count, int* d_error, cudaStream_t stream) {
     alignas(64) CUtensorMap ma, md;
     if (!rows_map(&ma, g.a, g.M, g.K, g.lda, false, kTcRows) || !rows_map(&md, g.down, (int64_t)g.n_adapters * g.rank, g.K, g.K, false, RN))
         return cudaErrorInvalidValue;
-    return launch_pdl(adapter_down_tc_kernel<RN>, dim3((g.M + kTcRows - 1) / kTcRows), kTcThreads, DownTc<RN>::kSmemBytes, stream, 1, ma, md, g, d_error);
+    const int blocks = (g.M + kTcRows - 1) / kTcRows, stages = DownTc<RN>::stages(blocks <= sm_count);
+    return launch_pdl(adapter_down_tc_kernel<RN>, dim3(blocks), kTcThreads, DownTc<RN>::smem_bytes(stages), stream, 1, ma, md, g, stages, d_error);
 }
 
 template <int NT>
@@ -411,10 +431,10 @@ cudaError_t adapter_down_configure() {
     auto set = [&](auto kernel, int bytes) {
         if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     };
-    set(adapter_down_tc_kernel<16>, DownTc<16>::kSmemBytes);
-    set(adapter_down_tc_kernel<32>, DownTc<32>::kSmemBytes);
-    set(adapter_down_tc_kernel<64>, DownTc<64>::kSmemBytes);
-    set(adapter_down_tc_kernel<128>, DownTc<128>::kSmemBytes);
+    set(adapter_down_tc_kernel<16>, DownTc<16>::smem_bytes(DownTc<16>::stages(true)));
+    set(adapter_down_tc_kernel<32>, DownTc<32>::smem_bytes(DownTc<32>::stages(true)));
+    set(adapter_down_tc_kernel<64>, DownTc<64>::smem_bytes(DownTc<64>::stages(true)));
+    set(adapter_down_tc_kernel<128>, DownTc<128>::smem_bytes(DownTc<128>::stages(true)));
     return e;
 }
 
@@ -422,10 +442,10 @@ cudaError_t adapter_down_launch(const AdapterDownArgs& g, int sm_count, int* d_e
     if (g.M <= 0) return cudaSuccess;
     if (g.M >= 16 * sm_count) {
         switch (tc_cols(g.rank)) {
-            case 16: return down_tc_t<16>(g, d_error, stream);
-            case 32: return down_tc_t<32>(g, d_error, stream);
-            case 64: return down_tc_t<64>(g, d_error, stream);
-            default: return down_tc_t<128>(g, d_error, stream);
+            case 16: return down_tc_t<16>(g, sm_count, d_error, stream);
+            case 32: return down_tc_t<32>(g, sm_count, d_error, stream);
+            case 64: return down_tc_t<64>(g, sm_count, d_error, stream);
+            default: return down_tc_t<128>(g, sm_count, d_error, stream);
         }
     }
     // the columns are spread over blocks too, as far as that fills the SMs

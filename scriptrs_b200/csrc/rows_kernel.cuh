@@ -16,7 +16,8 @@
 //     A tile may hold rows of several adapters: its MMAs run once for each, with the lanes of the other rows disabled, so that
 //     nothing of one adapter (not even a NaN) reaches rows of another, and the shared weights are read once whatever the adapters.
 //   - The tensor core adds into its accumulator by truncation, 1e-6 of the result at K = 1024 and 4.4e-6 at 4096 (measured).
-//     Where the result is stored in 32 bits, it is collected in registers every kSegment stages, rounded to nearest (2e-7).
+//     Where the result is stored in 32 bits, it is collected in registers every kSegment stages, rounded to nearest (4.7e-7 at
+//     either K; every four stages: 2.5e-7, but 16384 x 1024 x 1024 then takes 48 us instead of 36, a handshake per segment).
 // Every wait on an mbarrier is bounded; when one runs out the kernel sets *error, drains, frees its tensor memory and returns.
 #pragma once
 #include <cuda.h>
@@ -41,7 +42,7 @@ constexpr int kBM = 128;
 constexpr int kRowBytes = 128;  // of an operand row in a stage: one swizzle row
 constexpr int kEpiWarps = 8;
 constexpr int kSlabBytes = 32 * 128;
-constexpr int kSegment = 4;     // stages (64 bf16 or 128 e4m3 columns of K each) between two collections of a 32-bit result
+constexpr int kSegment = 8;     // stages (64 bf16 or 128 e4m3 columns of K each) between two collections of a 32-bit result
 
 enum RowsMode : int { kGrouped = 0, kGathered = 1, kAdapters = 2 };
 

@@ -23,6 +23,7 @@ namespace sb {
 namespace {
 
 constexpr int kDownWarps = 8;
+constexpr int kDotsMost = 4096;  // rows x rank up to which every row reads its adapter for itself (8 MB from L2 at K = 1024)
 constexpr int kMaxProducts = 2;  // adapters in 16 rows above which the rows are taken one by one
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -64,19 +65,30 @@ __device__ __forceinline__ void write_list(const AdapterDownArgs& p, int row0, i
     if (lane == 0) list[0] = count;
 }
 
-// Eight columns of a row's product, K over the lanes; lane j < 8 returns column j.
+// Eight columns of a row's product, K over the lanes, AHEAD steps of 256 columns asked for at once; lane j < 8 returns column j.
+template <int AHEAD>
 __device__ __forceinline__ float row_dots(const __nv_bfloat16* x, const __nv_bfloat16* d, int K, int cols, int lane) {
     float acc[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
-#pragma unroll 2
-    for (int k = lane * 8; k < K; k += 256) {
-        const uint4 xv = __ldg(reinterpret_cast<const uint4*>(x + k));
-        uint4 w[8];
+    for (int k0 = lane * 8; k0 < K; k0 += 256 * AHEAD) {
+        uint4 xv[AHEAD], w[AHEAD][8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = __ldg(reinterpret_cast<const uint4*>(d + (int64_t)min(j, cols - 1) * K + k));
+        for (int u = 0; u < AHEAD; ++u) {
+            const int k = k0 + 256 * u;
+            xv[u] = make_uint4(0, 0, 0, 0);
+            if (k < K) xv[u] = __ldg(reinterpret_cast<const uint4*>(x + k));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] = dot2(xv.w, w[j].w, dot2(xv.z, w[j].z, dot2(xv.y, w[j].y, dot2(xv.x, w[j].x, acc[j]))));
+            for (int j = 0; j < 8; ++j) {
+                w[u][j] = make_uint4(0, 0, 0, 0);
+                if (k < K && j < cols) w[u][j] = __ldg(reinterpret_cast<const uint4*>(d + (int64_t)j * K + k));
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                acc[j] = dot2(xv[u].w, w[u][j].w, dot2(xv[u].z, w[u][j].z, dot2(xv[u].y, w[u][j].y, dot2(xv[u].x, w[u][j].x, acc[j]))));
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -89,9 +101,32 @@ __device__ __forceinline__ float row_dots(const __nv_bfloat16* x, const __nv_bfl
     return v;
 }
 
+// Very few rows: a warp per row and eight columns, one block more for the lists.
+__global__ void __launch_bounds__(kDownWarps * 32, 1) adapter_down_dots_kernel(const AdapterDownArgs p, int groups) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_wait();
+    pdl_trigger();
+    const int block = (int)blockIdx.x - 1;
+    if (block < 0) {
+        for (int r = warp * p.list_rows; r < p.M; r += kDownWarps * p.list_rows) write_list(p, r, lane);
+        return;
+    }
+    const int64_t item = (int64_t)block * kDownWarps + warp;
+    const int row = (int)(item / groups), c = (int)(item % groups) * 8;
+    if (row >= p.M) return;
+    const int id = __ldg(p.row_adapter + row);
+    float v = 0.0f;
+    if ((unsigned)id < (unsigned)p.n_adapters) {
+        v = row_dots<4>(static_cast<const __nv_bfloat16*>(p.a) + (int64_t)row * p.lda,
+                        static_cast<const __nv_bfloat16*>(p.down) + ((int64_t)id * p.rank + c) * p.K, p.K, 8, lane);
+        if (p.scale) v *= __ldg(p.scale + id);
+    }
+    if (lane < 8) p.low[(int64_t)row * p.rank + c + lane] = v;
+}
+
 // NT tiles of 8 columns of 16 rows per block; the warps share K.
 template <int NT>
-__global__ void __launch_bounds__(kDownWarps * 32) adapter_down_kernel(const AdapterDownArgs p) {
+__global__ void __launch_bounds__(kDownWarps * 32, 1) adapter_down_kernel(const AdapterDownArgs p) {
     constexpr int kCols = NT * 8, kRows = 16;
     __shared__ float part[kDownWarps][kRows][kCols];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -177,7 +212,7 @@ __global__ void __launch_bounds__(kDownWarps * 32) adapter_down_kernel(const Ada
             for (int c = 0; c < kCols; c += 8) {
                 const int cols = min(p.rank - col0 - c, 8);
                 float v = 0.0f;
-                if (mine && cols > 0) v = row_dots(a + (int64_t)(row0 + r) * p.lda, down + ((int64_t)cur * p.rank + col0 + c) * p.K, p.K, cols, lane);
+                if (mine && cols > 0) v = row_dots<2>(a + (int64_t)(row0 + r) * p.lda, down + ((int64_t)cur * p.rank + col0 + c) * p.K, p.K, cols, lane);
                 if (lane < 8) part[warp][r][c + lane] = v;
             }
         }
@@ -393,7 +428,7 @@ __global__ void __launch_bounds__(kTcThreads) adapter_down_tc_kernel(const __gri
             for (int c = 0; c < p.rank; c += 8) {
                 float v = 0.0f;
                 if (has) {
-                    v = row_dots(a + (int64_t)row * p.lda, down + ((int64_t)id * p.rank + c) * p.K, p.K, 8, lane);
+                    v = row_dots<2>(a + (int64_t)row * p.lda, down + ((int64_t)id * p.rank + c) * p.K, p.K, 8, lane);
                     if (p.scale) v *= __ldg(p.scale + id);
                 }
                 if (lane < 8) p.low[(int64_t)row * p.rank + c + lane] = v;
@@ -447,6 +482,11 @@ cudaError_t adapter_down_launch(const AdapterDownArgs& g, int sm_count, int* d_e
             case 64: return down_tc_t<64>(g, sm_count, d_error, stream);
             default: return down_tc_t<128>(g, sm_count, d_error, stream);
         }
+    }
+    if ((int64_t)g.M * g.rank <= kDotsMost) {
+        const int groups = g.rank / 8;
+        const int blocks = 1 + (g.M * groups + kDownWarps - 1) / kDownWarps;
+        return launch_pdl(adapter_down_dots_kernel, dim3(blocks), kDownWarps * 32, 0, stream, 1, g, groups);
     }
     // the columns are spread over blocks too, as far as that fills the SMs
     const int blocks = (g.M + 15) / 16;

@@ -15,7 +15,7 @@ namespace sb {
 
 namespace {
 
-constexpr int kRouteThreads = 512, kRouteWarps = kRouteThreads / 32;
+constexpr int kRouteThreads = 1024, kRouteWarps = kRouteThreads / 32;
 constexpr int kRouteRows = 512;     // most rows of a block
 constexpr int kRouteOneBlock = 128; // rows up to which one block does everything
 constexpr int kRouteSums = 256;     // blocks up to which each sums the counts of those before it by itself
@@ -79,17 +79,27 @@ __device__ __forceinline__ void route_row(const RouteArgs& p, int row, bool live
 #pragma unroll
     for (int i = 0; i < kKeep; ++i) { mine[i] = 0.0f; who[i] = -1; }
     for (int j = 0; j < p.top_k; ++j) {
-        uint32_t best = 0;
-        int at = 0;
+        // the largest key, then the lowest expert that has it: trees instead of chains
+        uint32_t m[PER];
 #pragma unroll
-        for (int i = 0; i < PER; ++i)
-            if (key[i] > best) { best = key[i]; at = l * PER + i; }
+        for (int i = 0; i < PER; ++i) m[i] = key[i];
 #pragma unroll
-        for (int d = LANES / 2; d; d >>= 1) {
-            const uint32_t ob = __shfl_xor_sync(0xffffffffu, best, d);
-            const int oa = __shfl_xor_sync(0xffffffffu, at, d);
-            if (ob > best || (ob == best && oa < at)) { best = ob; at = oa; }
-        }
+        for (int d = PER / 2; d; d >>= 1)
+#pragma unroll
+            for (int i = 0; i < d; ++i) m[i] = max(m[i], m[i + d]);
+        uint32_t best = m[0];
+#pragma unroll
+        for (int d = LANES / 2; d; d >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, d));
+#pragma unroll
+        for (int i = 0; i < PER; ++i) m[i] = key[i] == best ? (uint32_t)(l * PER + i) : 0xffffu;
+#pragma unroll
+        for (int d = PER / 2; d; d >>= 1)
+#pragma unroll
+            for (int i = 0; i < d; ++i) m[i] = min(m[i], m[i + d]);
+        uint32_t low = m[0];
+#pragma unroll
+        for (int d = LANES / 2; d; d >>= 1) low = min(low, __shfl_xor_sync(0xffffffffu, low, d));
+        const int at = (int)low;
         if (j == 0) {
             top = best ? route_value(best) : 0.0f;
             if (!p.normalize) {
@@ -270,19 +280,24 @@ __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteA
             total[e] = p.work[(int64_t)e * (blocks + 1) + blocks];
         }
     } else {
-        for (int e = warp; e < p.n_experts; e += kRouteWarps) {
-            const int32_t* row = p.work + (int64_t)e * (blocks + 1);
-            int before = 0, all = 0;
+        // four experts a warp at a time, all their counts asked for at once
+        for (int e0 = warp * 4; e0 < p.n_experts; e0 += kRouteWarps * 4) {
+            int before[4] = {0, 0, 0, 0}, all[4] = {0, 0, 0, 0};
 #pragma unroll
             for (int i = 0; i < kRouteSums / 32; ++i) {
                 const int b = i * 32 + lane;
-                const int c = b < blocks ? row[b] : 0;
-                all += c;
-                if (b < block) before += c;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int c = b < blocks && e0 + j < p.n_experts ? p.work[(int64_t)(e0 + j) * (blocks + 1) + b] : 0;
+                    all[j] += c;
+                    if (b < block) before[j] += c;
+                }
             }
-            before = __reduce_add_sync(0xffffffffu, before);
-            all = __reduce_add_sync(0xffffffffu, all);
-            if (lane == 0) { base[e] = before; total[e] = all; }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int x = __reduce_add_sync(0xffffffffu, before[j]), y = __reduce_add_sync(0xffffffffu, all[j]);
+                if (lane == 0 && e0 + j < p.n_experts) { base[e0 + j] = x; total[e0 + j] = y; }
+            }
         }
     }
     __syncthreads();

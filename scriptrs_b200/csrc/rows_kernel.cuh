@@ -8,7 +8,7 @@
 //     group may be missing) times BN columns.  Every warp walks the offsets 32 groups at a time with a prefix sum over its
 //     lanes, so no table of groups is kept and the host never learns the sizes.
 //   - Rows picked by an index arrive by TMA gathers of four rows each, issued by four warps (32 rows each) from one elected
-//     lane with the indices in its registers; a tile with few rows fetches only those.
+//     lane (from every lane by turns a gather takes ten times as long); a tile with few rows fetches only those.
 //   - Rows leave through a swizzled slab per warp: 32 rows of one group by a TMA store (or reduce-add), which clips at column N;
 //     the last rows of a group, behind which its neighbour's begin, and results off the 16-byte boundaries by ordinary stores.
 //   - The low-rank addition is K = rank more columns of the same product, accumulated in the same tensor memory: `low` as bf16
@@ -54,18 +54,22 @@ struct RCfg {
     static constexpr int kBBytes = BN / CTAS * kRowBytes;
     static constexpr int kStageBytes = kABytes + kBBytes;
     static constexpr int kLowBytes = MODE == kAdapters ? 2 * kBM * kRowBytes : 0;  // `low` of the tile's rows: two operand tiles
-    static constexpr int kStages = std::min((231 * 1024 - 2048 - kEpiWarps * kSlabBytes - kLowBytes - kBM * 4) / kStageBytes, 8);
+    static constexpr int kColumnBytes = 2 * BN * 4;                                // bias and column scales of the tile
+    static constexpr int kIndexBytes = MODE == kGathered ? kBM * 4 : 0;
+    static constexpr int kBarBytes = 256;
+    static constexpr int kFixedBytes = kLowBytes + kEpiWarps * kSlabBytes + kColumnBytes + kIndexBytes + kBarBytes;
+    static constexpr int kStages = std::min((227 * 1024 - kFixedBytes) / kStageBytes, 8);
+    static constexpr int kSmemBytes = kStages * kStageBytes + kFixedBytes;
+    static_assert(kStages >= 3 && 8 * (2 * kStages + 6) + 16 <= kBarBytes, "shared memory");
+    static constexpr int kUps = kStageBytes / kBBytes;  // adapters' tiles of `up` in a stage
     static constexpr int kHalves = gemm_halves(BN);
     static constexpr int kHalfCols = BN / kHalves;
-    static constexpr int kIndexBytes = kBM * 4;
-    static constexpr int kBarBytes = 256;
-    static constexpr int kSmemBytes = kStages * kStageBytes + kLowBytes + kEpiWarps * kSlabBytes + kIndexBytes + kBarBytes + 1024;
-    static_assert(kStages >= 3 && kSmemBytes <= 227 * 1024 && 8 * (2 * kStages + 6) + 8 <= kBarBytes, "shared memory");
     static constexpr uint32_t kTmemCols = 2 * BN;
 };
 
-// Four warps more where rows are picked (gathers) or have adapters (`low`).
-constexpr int rows_threads(int mode) { return mode == kGrouped ? 320 : 448; }
+// Four warps more where rows are picked (gathers) or have adapters (`low`), 32 rows each.
+constexpr int kAuxWarps = 4;
+constexpr int rows_threads(int mode) { return 32 * (2 + kEpiWarps + (mode == kGrouped ? 0 : kAuxWarps)); }
 
 template <int BN, int CTAS, bool FP8>
 __device__ __forceinline__ uint32_t rows_idesc() {
@@ -131,6 +135,26 @@ __device__ __forceinline__ bool rows_wait_pair(uint32_t bar, uint32_t parity, vo
     }
 }
 
+// The gathering warps go by a count of the stages that the producer has begun.  They do not wait on the barriers themselves: a
+// warp without rows in a tile holds up nobody, could fall two turns of the ring behind, and would then wait for the parity of
+// another turn.  (Arriving on every stage instead, across the pair, costs twice the product's time.)
+__device__ __forceinline__ void rows_set_turn(uint32_t at, uint32_t n) {
+    asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(at), "r"(n) : "memory");
+}
+__device__ __forceinline__ bool rows_wait_turn(uint32_t at, uint32_t n, volatile int* abort_flag) {
+    const long long t0 = clock64();
+    while (true) {
+        uint32_t now;
+        asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(now) : "r"(at) : "memory");
+        if ((int32_t)(now - n) >= 0) return true;
+        if (*abort_flag) return false;
+        if (clock64() - t0 > kWaitCycles) {
+            *abort_flag = 1;
+            return false;
+        }
+    }
+}
+
 struct RowsParams {
     const int32_t* rows;
     const int32_t* offsets;
@@ -142,7 +166,6 @@ struct RowsParams {
     int M, N, K, n_groups, act, out_mode;
     float alpha;
     bool out_vec;    // output rows on 16-byte boundaries
-    bool bias_vec;   // bias and column scales of every group on 16-byte boundaries
     // adapters
     const int32_t* row_adapter;
     const float* low;
@@ -205,54 +228,27 @@ struct TileWalk {
     }
 };
 
-// Brings the bias and the column scales of a tile's columns into L1 while the accumulator is not ready yet.
-template <bool FP8>
-__device__ __forceinline__ void rows_touch(const RowsParams& p, int group, int col0, int cols, int lane) {
-    const int col = col0 + (lane & 15) * 32;
-    if ((lane & 15) * 32 >= cols || col >= p.N) return;
-    const float* from = lane < 16 ? p.bias : (FP8 ? p.col_scale : nullptr);
-    if (from) asm volatile("prefetch.global.L1 [%0];" ::"l"(from + (int64_t)group * p.N + col));
-}
-
-// 32 accumulator columns -> scales, bias, activation.  The loads carry no branches between them: one that ended the loop at N
-// made each wait for the one before it, 5000 cycles for 32 columns.
+// 32 accumulator columns -> scales, bias, activation.  bias, scale: of these columns, in shared memory.  (From global memory the
+// same loads cost a trip to L2 every 32 columns even where they had been touched before: 28 us of 75 in a product of 16384 x 4096
+// with K = 64; handed round by shuffles 7 us, but as many again for the scales.)
 template <bool FP8, bool F32>
-__device__ __forceinline__ void rows_finish(float (&x)[32], const RowsParams& p, int group, int col0, float rs, bool known) {
-    const int64_t at = (int64_t)group * p.N + col0;
+__device__ __forceinline__ void rows_finish(float (&x)[32], const RowsParams& p, const float4* bias, const float4* scale, float rs, bool known) {
     if (!known) {
 #pragma unroll
         for (int j = 0; j < 32; ++j) x[j] = 0.0f;
     }
     if (FP8) {
-        if (p.col_scale && p.bias_vec) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-                float4 c = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (col0 + j < p.N) c = __ldg(reinterpret_cast<const float4*>(p.col_scale + at + j));
-                x[j] *= rs * c.x; x[j + 1] *= rs * c.y; x[j + 2] *= rs * c.z; x[j + 3] *= rs * c.w;
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-                float c = 1.0f;
-                if (p.col_scale && col0 + j < p.N) c = __ldg(p.col_scale + at + j);
-                x[j] *= rs * c;
-            }
+        for (int j = 0; j < 8; ++j) {
+            const float4 c = scale[j];
+            x[4 * j] *= rs * c.x; x[4 * j + 1] *= rs * c.y; x[4 * j + 2] *= rs * c.z; x[4 * j + 3] *= rs * c.w;
         }
     }
-    if (p.bias && p.bias_vec) {
+    if (p.bias) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-            float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (col0 + j < p.N) b = __ldg(reinterpret_cast<const float4*>(p.bias + at + j));
-            x[j] += b.x; x[j + 1] += b.y; x[j + 2] += b.z; x[j + 3] += b.w;
-        }
-    } else if (p.bias) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            float b = 0.0f;
-            if (col0 + j < p.N) b = __ldg(p.bias + at + j);
-            x[j] += b;
+        for (int j = 0; j < 8; ++j) {
+            const float4 b = bias[j];
+            x[4 * j] += b.x; x[4 * j + 1] += b.y; x[4 * j + 2] += b.z; x[4 * j + 3] += b.w;
         }
     }
     if (p.act == kActSilu) {
@@ -301,16 +297,29 @@ __device__ __forceinline__ void rows_store(const unsigned char* slab, const Rows
             }
         }
     } else {
-        for (int r = 0; r < 32 && row0 + r < row1; ++r) {
+        // eight rows' pieces out of the slab at once: a load that waits for the store before it costs 60 cycles a row
+        const int rows = min(row1 - row0, 32);
+        for (int r0 = 0; r0 < rows; r0 += 8) {
 #pragma unroll
             for (int c = 0; c < COLS; c += 32) {
-                const int cc = c + lane;
-                if (col0 + cc >= p.N) continue;
-                const int byte = cc * (int)sizeof(T);
-                const T v = *reinterpret_cast<const T*>(slab + r * kBytes + (((byte >> 4) ^ ((r >> kShift) & kMask)) << 4) + (byte & 15));
-                T* dst = out + (int64_t)(row0 + r) * p.ldo + col0 + cc;
-                if constexpr (sizeof(T) == 4) *dst = add ? *dst + v : v;
-                else *dst = v;
+                const int cc = c + lane, byte = cc * (int)sizeof(T);
+                T* dst = out + (int64_t)(row0 + r0) * p.ldo + col0 + cc;
+                const bool in = col0 + cc < p.N;
+                T v[8];
+                float o[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int r = r0 + i;
+                    v[i] = *reinterpret_cast<const T*>(slab + r * kBytes + (((byte >> 4) ^ ((r >> kShift) & kMask)) << 4) + (byte & 15));
+                    o[i] = 0.0f;
+                    if (add && in && r < rows) o[i] = (float)dst[i * p.ldo];
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if (!in || r0 + i >= rows) continue;
+                    if constexpr (sizeof(T) == 4) dst[i * p.ldo] = v[i] + o[i];
+                    else dst[i * p.ldo] = v[i];
+                }
             }
         }
     }
@@ -338,11 +347,12 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
     constexpr int kTerms = F32 ? 3 : 2, kGroups = 8 / kTerms, kPhaseCols = 16 * kGroups;
     // rank of this CTA in its pair (the leader, rank 0, owns the barriers that the MMAs wait on)
     const uint32_t rank = CTAS == 2 ? __shfl_sync(0xffffffffu, cluster_ctarank(), 0) : 0u;
-    extern __shared__ unsigned char smem_dyn[];
-    const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
-    unsigned char* base_ptr = smem_dyn + (base - smem_u32(smem_dyn));
-    const uint32_t a_base = base, b_base = base + S * C::kABytes;
-    constexpr int kLowAt = S * C::kStageBytes, kSlabAt = kLowAt + C::kLowBytes, kIndexAt = kSlabAt + kEpiWarps * kSlabBytes;
+    extern __shared__ __align__(1024) unsigned char smem_dyn[];  // the operands' swizzle wants 1024-byte boundaries
+    const uint32_t base = smem_u32(smem_dyn);
+    unsigned char* base_ptr = smem_dyn;
+    const uint32_t a_base = base, b_base = base + C::kABytes;  // of stage 0; a stage holds its A and its W side by side
+    constexpr int kLowAt = S * C::kStageBytes, kSlabAt = kLowAt + C::kLowBytes, kColumnAt = kSlabAt + kEpiWarps * kSlabBytes;
+    constexpr int kIndexAt = kColumnAt + C::kColumnBytes;
     constexpr int kBarAt = kIndexAt + C::kIndexBytes;
     const uint32_t bar_base = base + kBarAt;
     auto full_bar = [&](int s) { return bar_base + 8u * s; };
@@ -353,6 +363,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
     const uint32_t lowfree_bar = bar_base + 8u * (2 * S + 5);  // and has been read
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + kBarAt + 8 * (2 * S + 6));
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const uint32_t turn_at = bar_base + 8u * (2 * S + 6) + 8;  // stages that the producer has begun, counted from the kernel's start
     // full barriers of the leader, as its own or as the pair's address
     auto lead = [&](uint32_t bar) { return CTAS == 2 ? mapa(bar, 0) : bar; };
 
@@ -363,6 +374,10 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
     const long long tile0 = blockIdx.x / CTAS, tile_step = gridDim.x / CTAS;
     const int cta_row = (int)rank * kBM;
 
+    if (base & 1023u) {  // dynamic shared memory begins on such a boundary where there is no static one
+        if (threadIdx.x == 0) atomicExch(error, 1);
+        return;
+    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
             mbar_init(full_bar(s), 1);
@@ -372,9 +387,10 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
             mbar_init(tfull_bar(a), 1);
             mbar_init(tempty_bar(a), 4 * C::kHalves * CTAS);
         }
-        mbar_init(low_bar, 4 * CTAS);
+        mbar_init(low_bar, kAuxWarps * CTAS);
         mbar_init(lowfree_bar, 1);
         *abort_flag = 0;
+        rows_set_turn(turn_at, 0);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -403,7 +419,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
     if (warp == 0) {
         // ------------------------------------------------------------ producer
         int stage = 0;
-        uint32_t ph = 0;
+        uint32_t ph = 0, begun = 0;
         bool ok = true;
         for (long long t = tile0; ok && walk.find(t, BN, tile); t += tile_step) {
             const int w_col = tile.col0 + (int)rank * (BN / CTAS);
@@ -428,28 +444,35 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                 uint32_t sp = ph;
                 for (int kt = 0; kt < k_tiles; ++kt) {
                     if (!mbar_wait(empty_bar(s), sp ^ 1, abort_flag)) { failed = true; break; }
+                    if (MODE == kGathered) rows_set_turn(turn_at, begun + (uint32_t)kt + 1);
                     if (rank == 0) mbar_expect_tx(full_bar(s), CTAS * C::kBBytes + a_bytes);
                     if (MODE != kGathered)
-                        rows_load<CTAS>(a_base + s * C::kABytes, &tma_a, lead(full_bar(s)), kt * kStepCols, tile.row0 + cta_row);
-                    rows_load<CTAS>(b_base + s * C::kBBytes, &tma_w, lead(full_bar(s)), kt * kStepCols, w_row);
+                        rows_load<CTAS>(a_base + s * C::kStageBytes, &tma_a, lead(full_bar(s)), kt * kStepCols, tile.row0 + cta_row);
+                    rows_load<CTAS>(b_base + s * C::kStageBytes, &tma_w, lead(full_bar(s)), kt * kStepCols, w_row);
                     if (++s == S) { s = 0; sp ^= 1; }
                 }
             }
             ok = !__any_sync(0xffffffffu, failed);
+            begun += k_tiles;
             stage += k_tiles;
             ph ^= (uint32_t)(stage / S) & 1u;
             stage %= S;
             if constexpr (MODE == kAdapters) {
                 if (!waited) { pdl_wait(); waited = true; count = list[0]; ids = list[4 + lane]; }
                 for (int c = 0; c < phases; ++c) {
-                    for (int j = 0; ok && j < count; ++j) {
-                        if (count > 32 && j % 32 == 0) ids = list[4 + j + lane];
-                        const int u_row = __shfl_sync(0xffffffffu, ids, j % 32) * p.N + w_col;
+                    for (int j0 = 0; ok && j0 < count; j0 += C::kUps) {
+                        const int n = min(C::kUps, count - j0);
+                        if (count > 32) ids = list[4 + j0 + (lane < n ? lane : 0)];  // else lane j holds adapter j
                         ok = __all_sync(0xffffffffu, mbar_wait(empty_bar(stage), ph ^ 1, abort_flag));
                         if (!ok) break;
+                        int u_row[C::kUps];
+#pragma unroll
+                        for (int u = 0; u < C::kUps; ++u) u_row[u] = __shfl_sync(0xffffffffu, ids, (count > 32 ? u : j0 + u) & 31) * p.N + w_col;
                         if (elect_one()) {
-                            if (rank == 0) mbar_expect_tx(full_bar(stage), CTAS * C::kBBytes);
-                            rows_load<CTAS>(b_base + stage * C::kBBytes, &tma_up, lead(full_bar(stage)), c * kPhaseCols, u_row);
+                            if (rank == 0) mbar_expect_tx(full_bar(stage), CTAS * C::kBBytes * n);
+#pragma unroll
+                            for (int u = 0; u < C::kUps; ++u)
+                                if (u < n) rows_load<CTAS>(a_base + stage * C::kStageBytes + u * C::kBBytes, &tma_up, lead(full_bar(stage)), c * kPhaseCols, u_row[u]);
                         }
                         __syncwarp();
                         if (++stage == S) { stage = 0; ph ^= 1; }
@@ -499,7 +522,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                     for (int k = kt; k < kt_end && !failed; ++k) {
                         if (!mbar_wait(full_bar(s), sp, abort_flag)) { failed = true; break; }
                         tc_fence_after();
-                        const uint64_t adesc = make_smem_desc(a_base + s * C::kABytes), bdesc = make_smem_desc(b_base + s * C::kBBytes);
+                        const uint64_t adesc = make_smem_desc(a_base + s * C::kStageBytes), bdesc = make_smem_desc(b_base + s * C::kStageBytes);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) rows_mma<CTAS, FP8>(d_tmem, adesc + 2 * i, bdesc + 2 * i, idesc, (k > kt || i) ? 1u : 0u);
                         rows_commit<CTAS>(empty_bar(s));
@@ -518,29 +541,38 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                             ok = ok && __all_sync(0xffffffffu, rows_wait_pair<CTAS>(low_bar, low_ph, abort_flag));
                             low_ph ^= 1;
                             const int groups = min(kGroups, (p.rank - c * kPhaseCols + 15) / 16);
-                            for (int j = 0; ok && j < count; ++j) {
-                                if (count > 32 && j % 32 == 0) ids = list[4 + j + lane];
-                                const int id = __shfl_sync(0xffffffffu, ids, j % 32);
-                                uint32_t off[4 * CTAS];
-#pragma unroll
-                                for (int q = 0; q < 4 * CTAS; ++q) off[q] = ~__ballot_sync(0xffffffffu, mine[q] == id);
+                            for (int j0 = 0; ok && j0 < count; j0 += C::kUps) {
+                                const int n = min(C::kUps, count - j0);
+                                if (count > 32) ids = list[4 + j0 + (lane < n ? lane : 0)];
                                 ok = __all_sync(0xffffffffu, mbar_wait(full_bar(stage), ph, abort_flag));
                                 if (!ok) break;
                                 tc_fence_after();
-                                if (elect_one()) {
-                                    const uint64_t adesc = make_smem_desc(base + kLowAt), bdesc = make_smem_desc(b_base + stage * C::kBBytes);
 #pragma unroll
-                                    for (int g = 0; g < kGroups; ++g) {
-                                        if (g >= groups) break;
+                                for (int u = 0; u < C::kUps; ++u) {
+                                    if (u >= n) break;
+                                    const int id = __shfl_sync(0xffffffffu, ids, (count > 32 ? u : j0 + u) & 31);
+                                    uint32_t off[4 * CTAS];
 #pragma unroll
-                                        for (int e = 0; e < kTerms; ++e) {
-                                            constexpr int kTile = kBM * kRowBytes / 16;  // in the descriptor's 16-byte units
-                                            const int at = g * kTerms + e;
-                                            rows_mma_lanes<CTAS>(d_tmem, adesc + at / 4 * kTile + 2 * (at % 4), bdesc + 2 * g, idesc, off);
+                                    for (int q = 0; q < 4 * CTAS; ++q) off[q] = ~__ballot_sync(0xffffffffu, mine[q] == id);
+                                    if (elect_one()) {
+                                        const uint64_t adesc = make_smem_desc(base + kLowAt);
+                                        const uint64_t bdesc = make_smem_desc(a_base + stage * C::kStageBytes + u * C::kBBytes);
+#pragma unroll
+                                        for (int g = 0; g < kGroups; ++g) {
+                                            if (g >= groups) break;
+#pragma unroll
+                                            for (int e = 0; e < kTerms; ++e) {
+                                                constexpr int kTile = kBM * kRowBytes / 16;  // in the descriptor's 16-byte units
+                                                const int at = g * kTerms + e;
+                                                rows_mma_lanes<CTAS>(d_tmem, adesc + at / 4 * kTile + 2 * (at % 4), bdesc + 2 * g, idesc, off);
+                                            }
                                         }
                                     }
+                                    __syncwarp();
+                                }
+                                if (elect_one()) {
                                     rows_commit<CTAS>(empty_bar(stage));
-                                    if (j == count - 1) rows_commit<CTAS>(lowfree_bar);
+                                    if (j0 + n == count) rows_commit<CTAS>(lowfree_bar);
                                 }
                                 __syncwarp();
                                 if (++stage == S) { stage = 0; ph ^= 1; }
@@ -560,7 +592,39 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
         unsigned char* slab = base_ptr + kSlabAt + ew * kSlabBytes;
         uint32_t seg = 0;
         bool ok = true;
-        for (long long t = tile0; half < C::kHalves && ok && walk.find(t, BN, tile); t += tile_step) {
+        const int cbeg = half * C::kHalfCols;
+        float* columns = reinterpret_cast<float*>(base_ptr + kColumnAt) + cbeg;  // bias; the scales BN further on
+        // the four warps of a half bring in its columns' bias and scales, fetched a tile ahead
+        float next_bias = 0.0f, next_scale = 1.0f;
+        auto fetch_columns = [&](const RowsTile& at) {
+            const int c = quad * 32 + lane, col = at.col0 + cbeg + c;
+            const bool in = c < C::kHalfCols && col < p.N;
+            next_bias = p.bias && in ? __ldg(p.bias + (int64_t)at.group * p.N + col) : 0.0f;
+            if (FP8) next_scale = p.col_scale && in ? __ldg(p.col_scale + (int64_t)at.group * p.N + col) : 1.0f;
+        };
+        static_assert(C::kHalfCols <= 128, "a thread brings in one column");
+        auto half_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory"); };
+        bool more = half < C::kHalves && walk.find(tile0, BN, tile);
+        RowsTile ahead;
+        if (more) fetch_columns(tile);
+        for (long long t = tile0; more; t += tile_step, tile = ahead) {
+            // the tile before has been read; where a wait ran out in one of the four warps, all of them leave here
+            uint32_t all_ok;
+            asm volatile(
+                "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %2, 0;\n\t"
+                "barrier.cta.red.and.pred p, %1, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                : "=r"(all_ok)
+                : "r"(1 + half), "r"(ok ? 1u : 0u)
+                : "memory");
+            ok = all_ok != 0;
+            if (!ok) break;
+            if (quad * 32 + lane < C::kHalfCols) {
+                columns[quad * 32 + lane] = next_bias;
+                if (FP8) columns[BN + quad * 32 + lane] = next_scale;
+            }
+            half_sync();
+            more = walk.find(t + tile_step, BN, ahead);
+            if (more) fetch_columns(ahead);
             const int row0 = tile.row0 + cta_row + quad * 32;  // of this warp
             const int row = row0 + lane;
             const bool live = row < tile.row1;
@@ -568,9 +632,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
             if (MODE == kGathered && p.rows && live) src = __ldg(p.rows + row);
             const bool known = MODE != kGathered || (unsigned)src < (unsigned long long)p.a_rows;
             const float rs = FP8 && p.row_scale && live && known ? __ldg(p.row_scale + src) : 1.0f;
-            const int cbeg = half * C::kHalfCols;
             const bool any = row0 < tile.row1;  // rows of this warp in the tile
-            rows_touch<FP8>(p, tile.group, tile.col0 + cbeg, C::kHalfCols, lane);
             auto taddr = [&]() { return tmem_base + ((uint32_t)(quad * 32) << 16) + (seg & 1) * BN + cbeg; };
             auto release = [&]() {
                 tc_fence_before();
@@ -622,8 +684,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                     }
                     release();
                 }
-                if (!ok) break;
-                if (!any) continue;
+                if (!ok || !any) continue;
 #pragma unroll
                 for (int c = 0; c < kCols; c += 32) {
                     const int col0 = tile.col0 + cbeg + c;
@@ -631,7 +692,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                     float x[32];
 #pragma unroll
                     for (int j = 0; j < 32; ++j) x[j] = sum[c + j];
-                    rows_finish<FP8, F32>(x, p, tile.group, col0, rs, known);
+                    rows_finish<FP8, F32>(x, p, reinterpret_cast<const float4*>(columns + c), reinterpret_cast<const float4*>(columns + BN + c), rs, known);
                     ready();
 #pragma unroll
                     for (int q = 0; q < 8; ++q)
@@ -643,33 +704,41 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                 constexpr int kCols = C::kHalfCols < 64 ? C::kHalfCols : 64;
                 constexpr int kShift = kCols == 32 ? 1 : 0, kMask = kCols / 8 - 1;
                 ok = __all_sync(0xffffffffu, mbar_wait(tfull_bar(seg & 1), (seg >> 1) & 1, abort_flag));
-                if (!ok) break;
+                if (!ok) continue;
                 tc_fence_after();
+                bool held = true;
                 if (any) {
 #pragma unroll 1
                     for (int c = 0; c < C::kHalfCols; c += kCols) {
                         const int col0 = tile.col0 + cbeg + c;
                         if (col0 >= p.N) break;
-                        ready();
+                        uint32_t packed[kCols / 2];
 #pragma unroll
                         for (int sub = 0; sub < kCols / 32; ++sub) {
                             uint32_t v[32];
                             tmem_ld32(taddr() + c + 32 * sub, v);
                             tmem_wait_ld();
+                            if (c + 32 * (sub + 1) >= C::kHalfCols) {  // the accumulator is free for the tile after the next
+                                release();
+                                held = false;
+                            }
                             float x[32];
 #pragma unroll
                             for (int j = 0; j < 32; ++j) x[j] = __uint_as_float(v[j]);
-                            rows_finish<FP8, F32>(x, p, tile.group, col0 + 32 * sub, rs, known);
+                            rows_finish<FP8, F32>(x, p, reinterpret_cast<const float4*>(columns + c + 32 * sub),
+                                                  reinterpret_cast<const float4*>(columns + BN + c + 32 * sub), rs, known);
 #pragma unroll
-                            for (int q = 0; q < 4; ++q)
-                                *reinterpret_cast<uint4*>(slab + lane * (kCols * 2) + (((4 * sub + q) ^ ((lane >> kShift) & kMask)) << 4)) =
-                                    make_uint4(pack_bf16(x[8 * q], x[8 * q + 1]), pack_bf16(x[8 * q + 2], x[8 * q + 3]),
-                                               pack_bf16(x[8 * q + 4], x[8 * q + 5]), pack_bf16(x[8 * q + 6], x[8 * q + 7]));
+                            for (int j = 0; j < 16; ++j) packed[16 * sub + j] = pack_bf16(x[2 * j], x[2 * j + 1]);
                         }
+                        ready();
+#pragma unroll
+                        for (int q = 0; q < kCols / 8; ++q)
+                            *reinterpret_cast<uint4*>(slab + lane * (kCols * 2) + ((q ^ ((lane >> kShift) & kMask)) << 4)) =
+                                make_uint4(packed[4 * q], packed[4 * q + 1], packed[4 * q + 2], packed[4 * q + 3]);
                         leave(col0, [&]() { rows_store<__nv_bfloat16, kCols>(slab, p, row0, tile.row1, col0, lane); });
                     }
                 }
-                release();
+                if (held) release();
             }
         }
         if (elect_one()) bulk_wait_all();
@@ -678,12 +747,11 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
         // ------------------------------------------------------------ gathers, 32 rows a warp
         const int gw = warp - 2 - kEpiWarps;
         int32_t* index = reinterpret_cast<int32_t*>(base_ptr + kIndexAt) + gw * 32;
-        int stage = 0;
-        uint32_t ph = 0;
+        uint32_t begun = 0;
         bool ok = true;
-        for (long long t = tile0; ok && walk.find(t, BN, tile); t += tile_step) {
-            const int first = tile.row0 + cta_row + gw * 32;
-            const int count = min(tile.row1 - first, 32);
+        for (long long t = tile0; ok && walk.find(t, BN, tile); t += tile_step, begun += k_tiles) {
+            const int first = tile.row0 + cta_row + gw * 32, count = tile.row1 - first;
+            if (count <= 0) continue;
             const int i = min(first + lane, tile.row1 - 1);
             const int v = p.rows ? __ldg(p.rows + i) : i;
             index[lane] = (unsigned)v < (unsigned long long)p.a_rows ? v : 0;
@@ -693,21 +761,17 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                 int4 r[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) r[j] = reinterpret_cast<const int4*>(index)[j];
-                int s = stage;
-                uint32_t sp = ph;
+                int s = (int)(begun % S);
                 for (int kt = 0; kt < k_tiles; ++kt) {
-                    if (!mbar_wait(empty_bar(s), sp ^ 1, abort_flag)) { failed = true; break; }
-                    const uint32_t dst = a_base + s * C::kABytes + gw * 32 * kRowBytes, bar = lead(full_bar(s));
+                    if (!rows_wait_turn(turn_at, begun + (uint32_t)kt + 1, abort_flag)) { failed = true; break; }
+                    const uint32_t dst = a_base + s * C::kStageBytes + gw * 32 * kRowBytes, bar = lead(full_bar(s));
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
                         if (4 * j < count) tma_gather4<CTAS>(dst + j * 4 * kRowBytes, &tma_a, bar, kt * kStepCols, r[j].x, r[j].y, r[j].z, r[j].w);
-                    if (++s == S) { s = 0; sp ^= 1; }
+                    if (++s == S) s = 0;
                 }
             }
             ok = !__any_sync(0xffffffffu, failed);
-            stage += k_tiles;
-            ph ^= (uint32_t)(stage / S) & 1u;
-            stage %= S;
         }
         if (!ok) {
             const long long t0 = clock64();
@@ -788,7 +852,6 @@ cudaError_t rows_launch_t(const RowsArgs& g, int sm_count, int* d_error, cudaStr
     p.a_rows = g.a_rows; p.ldo = g.ldo; p.M = g.M; p.N = g.N; p.K = g.K; p.n_groups = g.n_groups; p.act = g.act; p.out_mode = g.out_mode;
     p.alpha = g.alpha;
     p.out_vec = !(reinterpret_cast<uintptr_t>(g.out) & 15) && !((g.ldo * eb) & 15);
-    p.bias_vec = g.N % 4 == 0 && !((reinterpret_cast<uintptr_t>(g.bias) | reinterpret_cast<uintptr_t>(g.col_scale)) & 15);
     mo = mw;
     if (p.out_vec && !rows_out_map(&mo, g.out, g.M, g.N, g.ldo, F32, F32 || RCfg<BN, CTAS, MODE>::kHalfCols >= 64 ? 128 : 64)) return cudaErrorInvalidValue;
     p.row_adapter = g.row_adapter; p.low = g.low; p.lists = g.lists; p.rank = g.rank;

@@ -251,6 +251,16 @@ def test_grouped_large(ctx, M, N, K, G, gather):
     grouped_case(ctx, sizes, N, K, gather=gather, mode=1)
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+def test_gathered_short_tiles_over_many_turns_of_the_ring(ctx, fp8):
+    """Tiles with rows for some of the gathering warps only, K of many turns of the operand ring, several tiles per CTA."""
+    r = np.random.RandomState(4)
+    for sizes in (r.randint(1, 130, 60), [33] * 50, [1, 300, 2, 257, 40, 0, 129] * 6):
+        grouped_case(ctx, list(map(int, sizes)), 2048, 4096, gather=500, fp8=fp8)
+    grouped_case(ctx, [5000, 5100, 4099, 3, 2900], 2048, 2048, gather=900, fp8=fp8)
+    grouped_case(ctx, [5000, 5100, 4099, 3, 2900], 2048, 2048, gather=900, fp8=fp8, mode=1)
+
+
 def test_grouped_empty_calls(ctx):
     import scriptrs_b200 as sb
 
@@ -446,7 +456,8 @@ def test_adapter_odd_sizes_and_strides(ctx, N, K, mode):
     adapter_case(ctx, who, 2, 16, N, K, mode=mode, bias=False, scale=False)
 
 
-@pytest.mark.parametrize("M,N,K,rank,n", [(13160, 1024, 1024, 16, 70), (20000, 2048, 512, 64, 8), (3000, 4096, 1024, 32, 300)])
+@pytest.mark.parametrize("M,N,K,rank,n", [(13160, 1024, 1024, 16, 70), (20000, 2048, 512, 64, 8), (3000, 4096, 1024, 32, 300), (5000, 512, 1000, 128, 4),
+                                            (300, 4096, 1024, 8, 3), (700, 1024, 1024, 16, 5)])
 def test_adapters_large(ctx, M, N, K, rank, n):
     r = np.random.RandomState(M)
     cuts = np.sort(r.randint(0, M, 71))
@@ -458,6 +469,15 @@ def test_adapters_large(ctx, M, N, K, rank, n):
 @pytest.mark.parametrize("mode", [0, 1])
 def test_a_broken_adapter_stays_with_its_rows(ctx, mode):
     adapter_case(ctx, runs((0, 50), (1, 20), (2, 30), (-1, 28)) + [0, 1, 2] * 10, 3, 16, 256, 128, mode=mode, poison=1)
+
+
+@pytest.mark.parametrize("mode", [0, 1])
+def test_a_broken_adapter_among_many_rows(ctx, mode):
+    """The same in products large enough for tiles of 256 rows, with up to a hundred adapters in one."""
+    r = np.random.RandomState(3)
+    who = np.repeat(r.randint(-1, 90, 700), r.randint(1, 35, 700))
+    who[5000:5600] = r.randint(-1, 90, 600)
+    adapter_case(ctx, who.tolist(), 90, 16, 1024, 64, mode=mode, poison=7)
 
 
 def test_rows_without_an_adapter_equal_the_shared_product(ctx):

@@ -605,6 +605,7 @@ int32_t sb_combine_rows(sb_ctx* ctx, const void* d_y, int32_t y_f32, int64_t ldy
  *              neighbours, but a run of 128 rows costs a pass over `up` for each adapter in it.
  *   d_out      [M x N], row pitch ldo elements
  *   d_work     sb_adapter_gemm_workspace(M, rank) bytes on a 16-byte boundary
+ * Sums are held in 32 bits; for bf16 results A[i] * down[a]^T is rounded to bf16 once, for f32 results it is not.
  * Any M, N and n_adapters (n_adapters * N < 2^31); K and rank multiples of 8, rank <= 128; alignment as for sb_grouped_gemm.
  * Nothing of one adapter, inf and NaN included, reaches rows of another. */
 int32_t sb_adapter_gemm(sb_ctx* ctx, const void* d_a, int64_t lda, const void* d_w, const float* d_bias, const void* d_down,

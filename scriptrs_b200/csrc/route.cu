@@ -10,6 +10,7 @@
 #include "gemm_tile.h"
 #include "launch.cuh"
 #include "rows.h"
+#include "tc_ptx.cuh"
 
 namespace sb {
 
@@ -30,18 +31,23 @@ int64_t route_blocks(int64_t rows) { return (rows + route_block_rows(rows) - 1) 
 
 // Order-preserving image of a float; 0 for what is never chosen (-inf, NaN).  +inf counts as the largest finite value, -0 as 0.
 __device__ __forceinline__ uint32_t route_key(float x) {
-    if (!(x > -INFINITY)) return 0u;
     const uint32_t u = __float_as_uint(fminf(x, FLT_MAX) + 0.0f);
-    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+    return x > -INFINITY ? ((u & 0x80000000u) ? ~u : (u | 0x80000000u)) : 0u;
 }
 __device__ __forceinline__ float route_value(uint32_t k) {
     return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
+// exp(x) for x <= 0: the argument's rounding is 2^-24 of it, the function's error 2^-22; what counts lies near 0.
+__device__ __forceinline__ float route_exp(float x) { return ptx::ex2_approx(x * 1.44269504f); }
 
-// LANES lanes take a row, PER neighbouring experts each, in registers.  Each of the k rounds takes the largest key and, among
-// equal ones, the lowest expert.  `live`: the row exists (its lanes take part in the shuffles either way).
+// LANES lanes take a row, PER neighbouring experts each, in registers.  A round finds the largest key below the one before as the
+// maximum of key - previous in unsigned arithmetic: what lies below wraps round to the top, nearest first.
+//   bf16: a key is 16 bits, the expert (counted down) takes the other 16: keys differ and a round yields one choice.
+//   f32:  a round yields a value; the experts that have it follow in ascending order.
+// `live`: the row exists (its lanes take part in the shuffles either way).
 template <int LANES, int PER, typename T>
 __device__ __forceinline__ void route_row(const RouteArgs& p, int row, bool live, int lane, int16_t* chosen) {
+    constexpr bool kPacked = sizeof(T) == 2;
     const int l = lane % LANES;
     uint32_t key[PER];
     if (live) {
@@ -59,7 +65,7 @@ __device__ __forceinline__ void route_row(const RouteArgs& p, int row, bool live
 #pragma unroll
                 for (int j = 0; j < kVec; ++j) {
                     float f;
-                    if constexpr (sizeof(T) == 2) f = __uint_as_float(j % 2 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+                    if constexpr (kPacked) f = __uint_as_float(j % 2 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
                     else f = __uint_as_float(w[j]);
                     key[(i + j) % PER] = in ? route_key(f) : 0u;
                 }
@@ -72,17 +78,11 @@ __device__ __forceinline__ void route_row(const RouteArgs& p, int row, bool live
 #pragma unroll
         for (int i = 0; i < PER; ++i) key[i] = 0u;
     }
-    float top = 0.0f, total = 0.0f;
-    constexpr int kKeep = (kMaxTopK + LANES - 1) / LANES;  // lane l keeps the choices l, l + LANES, ...
-    float mine[kKeep];
-    int who[kKeep];
-#pragma unroll
-    for (int i = 0; i < kKeep; ++i) { mine[i] = 0.0f; who[i] = -1; }
-    for (int j = 0; j < p.top_k; ++j) {
-        // the largest key, then the lowest expert that has it: trees instead of chains
+    // the largest of f(key) over the row
+    auto most = [&](auto f) {
         uint32_t m[PER];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) m[i] = key[i];
+        for (int i = 0; i < PER; ++i) m[i] = f(key[i]);
 #pragma unroll
         for (int d = PER / 2; d; d >>= 1)
 #pragma unroll
@@ -90,35 +90,68 @@ __device__ __forceinline__ void route_row(const RouteArgs& p, int row, bool live
         uint32_t best = m[0];
 #pragma unroll
         for (int d = LANES / 2; d; d >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, d));
+        return best;
+    };
+    float total = 0.0f;
+    const uint32_t first = most([](uint32_t k) { return k; });
+    // a packed key's lower half stands for the zeros of a bf16 value, inverted where it is negative
+    auto value = [](uint32_t k) {
+        if (kPacked) k = (k & 0xffff0000u) | ((k & 0x80000000u) ? 0u : 0xffffu);
+        return route_value(k);
+    };
+    const float top = first ? value(first) : 0.0f;
+    auto weight = [&](uint32_t k) { return route_exp(value(k) - top); };
+    if (!p.normalize) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) m[i] = key[i] == best ? (uint32_t)(l * PER + i) : 0xffffu;
+        for (int i = 0; i < PER; ++i) total += key[i] ? weight(key[i]) : 0.0f;
 #pragma unroll
-        for (int d = PER / 2; d; d >>= 1)
+        for (int d = LANES / 2; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+    }
+    constexpr int kKeep = (kMaxTopK + LANES - 1) / LANES;  // lane l keeps the choices l, l + LANES, ...
+    float mine[kKeep];
+    int who[kKeep];
 #pragma unroll
-            for (int i = 0; i < d; ++i) m[i] = min(m[i], m[i + d]);
-        uint32_t low = m[0];
+    for (int i = 0; i < kKeep; ++i) { mine[i] = 0.0f; who[i] = -1; }
+    auto keep = [&](int j, float w, int e) {
+        if (p.normalize) total += w;
 #pragma unroll
-        for (int d = LANES / 2; d; d >>= 1) low = min(low, __shfl_xor_sync(0xffffffffu, low, d));
-        const int at = (int)low;
-        if (j == 0) {
-            top = best ? route_value(best) : 0.0f;
-            if (!p.normalize) {
+        for (int i = 0; i < kKeep; ++i)
+            if (l + i * LANES == j) { mine[i] = w; who[i] = e; }
+    };
+    if constexpr (kPacked) {
 #pragma unroll
-                for (int i = 0; i < PER; ++i)
-                    if (key[i]) total += expf(route_value(key[i]) - top);
-#pragma unroll
-                for (int d = LANES / 2; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
-            }
+        for (int i = 0; i < PER; ++i)
+            if (key[i]) key[i] = (key[i] & 0xffff0000u) | (0xffffu - (uint32_t)(l * PER + i));
+        uint32_t best = most([](uint32_t k) { return k; });
+        for (int j = 0; j < p.top_k; ++j) {
+            if (best) keep(j, weight(best), (int)(0xffffu - (best & 0xffffu)));
+            const uint32_t next = most([&](uint32_t k) { return k - best; }) + best;  // shuffles: by every lane, its row over or not
+            best = best ? next : 0u;
         }
-        if (best) {
-            const float w = expf(route_value(best) - top);
-            if (p.normalize) total += w;
+    } else {
+        const int group0 = lane / LANES * LANES;
+        uint32_t best = first;
+        int j = 0;
+        while (__any_sync(0xffffffffu, best && j < p.top_k)) {
+            uint32_t has = 0;  // this lane's experts with that value
 #pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if (l * PER + i == at) key[i] = 0;
-#pragma unroll
-            for (int i = 0; i < kKeep; ++i)
-                if (l + i * LANES == j) { mine[i] = w; who[i] = at; }
+            for (int i = 0; i < PER; ++i) has |= key[i] == best ? 1u << i : 0u;
+            if (!best) has = 0;
+            const float w = best ? weight(best) : 0.0f;
+            while (true) {
+                const uint32_t lanes = (__ballot_sync(0xffffffffu, has != 0) >> group0) & (LANES == 32 ? 0xffffffffu : (1u << LANES) - 1u);
+                const bool go = lanes && j < p.top_k;
+                if (!__any_sync(0xffffffffu, go)) break;
+                const int from = group0 + (lanes ? __ffs(lanes) - 1 : 0);
+                const int at = __shfl_sync(0xffffffffu, l * PER + __ffs(has) - 1, from);
+                if (go) {
+                    keep(j, w, at);
+                    ++j;
+                    if (lane == from) has &= has - 1;
+                }
+            }
+            const uint32_t next = most([&](uint32_t k) { return k - best; }) + best;
+            best = best ? next : 0u;
         }
     }
     if (!live) return;
@@ -172,11 +205,13 @@ __device__ __forceinline__ void route_place(const RouteArgs& p, const int16_t* c
     }
     __syncthreads();
     for (int e = threadIdx.x; e < p.n_experts; e += kRouteThreads) {
-        uint32_t at = 0;
+        uint32_t at = 0, c[kRouteWarps];
+#pragma unroll
+        for (int w = 0; w < kRouteWarps; ++w) c[w] = part[w * p.n_experts + e];
+#pragma unroll
         for (int w = 0; w < kRouteWarps; ++w) {
-            const uint32_t c = part[w * p.n_experts + e];
             part[w * p.n_experts + e] = (uint16_t)at;
-            at += c;
+            at += c[w];
         }
     }
     __syncthreads();

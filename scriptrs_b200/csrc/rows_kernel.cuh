@@ -11,8 +11,10 @@
 //     lane (from every lane by turns a gather takes ten times as long); a tile with few rows fetches only those.
 //   - Rows leave through a swizzled slab per warp: 32 rows of one group by a TMA store (or reduce-add), which clips at column N;
 //     the last rows of a group, behind which its neighbour's begin, and results off the 16-byte boundaries by ordinary stores.
-//   - The low-rank addition is K = rank more columns of the same product, accumulated in the same tensor memory: `low` as bf16
-//     terms (two where the result is bf16: 2^-17 of it dropped; three where it is stored in 32 bits) against the rows of U_a.
+//   - The low-rank addition is K = rank more columns of the same product, accumulated in the same tensor memory, `low` against the
+//     rows of U_a.  Where the result is bf16, `low` is rounded to bf16 too, as between any two bf16 products: 2^-9 of the addition,
+//     below the result's own rounding (a second term, 2^-17, took 13 % of the product's time at rank 64 with two adapters a tile).
+//     Where the result is stored in 32 bits it enters as three bf16 terms (2^-26).
 //     A tile may hold rows of several adapters: its MMAs run once for each, with the lanes of the other rows disabled, so that
 //     nothing of one adapter (not even a NaN) reaches rows of another, and the shared weights are read once whatever the adapters.
 //   - The tensor core adds into its accumulator by truncation, 1e-6 of the result at K = 1024 and 4.4e-6 at 4096 (measured).
@@ -48,12 +50,14 @@ enum RowsMode : int { kGrouped = 0, kGathered = 1, kAdapters = 2 };
 
 // CTAS = 2: a cluster of two CTAs on 256 rows x BN columns (tcgen05 cta_group::2); each stages its own 128 rows of A and its own
 // half of the W rows.
-template <int BN, int CTAS, int MODE>
+template <int BN, int CTAS, int MODE, bool F32>
 struct RCfg {
     static constexpr int kABytes = kBM * kRowBytes;
     static constexpr int kBBytes = BN / CTAS * kRowBytes;
     static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kLowBytes = MODE == kAdapters ? 2 * kBM * kRowBytes : 0;  // `low` of the tile's rows: two operand tiles
+    // `low` of the tile's rows as an operand: blocks of 16 of its columns (32 bytes a row), four to an operand tile
+    static constexpr int kTerms = F32 ? 3 : 1, kGroups = F32 ? 2 : 4;  // bf16 terms, blocks of columns that are held at once
+    static constexpr int kLowBytes = MODE == kAdapters ? (kTerms * kGroups + 3) / 4 * kBM * kRowBytes : 0;
     static constexpr int kColumnBytes = 2 * BN * 4;                                // bias and column scales of the tile
     static constexpr int kIndexBytes = MODE == kGathered ? kBM * 4 : 0;
     static constexpr int kBarBytes = 256;
@@ -340,11 +344,10 @@ __global__ void __launch_bounds__(rows_threads(MODE), 1)
 rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_w,
             const __grid_constant__ CUtensorMap tma_up, const __grid_constant__ CUtensorMap tma_out, const RowsParams p,
             int* __restrict__ error) {
-    using C = RCfg<BN, CTAS, MODE>;
+    using C = RCfg<BN, CTAS, MODE, F32>;
     constexpr int S = C::kStages;
     constexpr int kStepCols = FP8 ? 128 : 64;
-    // `low` as bf16 terms, 16 of its columns in 32 bytes of each: eight such blocks a row fit, kGroups x kTerms of them are used
-    constexpr int kTerms = F32 ? 3 : 2, kGroups = 8 / kTerms, kPhaseCols = 16 * kGroups;
+    constexpr int kTerms = C::kTerms, kGroups = C::kGroups, kPhaseCols = 16 * kGroups;
     // rank of this CTA in its pair (the leader, rank 0, owns the barriers that the MMAs wait on)
     const uint32_t rank = CTAS == 2 ? __shfl_sync(0xffffffffu, cluster_ctarank(), 0) : 0u;
     extern __shared__ __align__(1024) unsigned char smem_dyn[];  // the operands' swizzle wants 1024-byte boundaries
@@ -808,8 +811,10 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                             float& x = f[16 * g + 2 * i];
                             float& y = f[16 * g + 2 * i + 1];
                             w[i] = pack_bf16(x, y);
-                            x = bf16_rest(x);
-                            y = bf16_rest(y);
+                            if (kTerms > 1) {
+                                x = bf16_rest(x);
+                                y = bf16_rest(y);
+                            }
                         }
                         const int at = g * kTerms + e, chunk = 2 * (at % 4);
                         unsigned char* d = dst + at / 4 * kBM * kRowBytes;
@@ -853,19 +858,19 @@ cudaError_t rows_launch_t(const RowsArgs& g, int sm_count, int* d_error, cudaStr
     p.alpha = g.alpha;
     p.out_vec = !(reinterpret_cast<uintptr_t>(g.out) & 15) && !((g.ldo * eb) & 15);
     mo = mw;
-    if (p.out_vec && !rows_out_map(&mo, g.out, g.M, g.N, g.ldo, F32, F32 || RCfg<BN, CTAS, MODE>::kHalfCols >= 64 ? 128 : 64)) return cudaErrorInvalidValue;
+    if (p.out_vec && !rows_out_map(&mo, g.out, g.M, g.N, g.ldo, F32, F32 || RCfg<BN, CTAS, MODE, F32>::kHalfCols >= 64 ? 128 : 64)) return cudaErrorInvalidValue;
     p.row_adapter = g.row_adapter; p.low = g.low; p.lists = g.lists; p.rank = g.rank;
     // at most this many tiles: a group's last one may be short
     const int64_t n_tiles = (g.N + BN - 1) / BN;
     const int64_t tiles = ((int64_t)(g.M + kBM * CTAS - 1) / (kBM * CTAS) + std::min(g.n_groups - 1, g.M)) * n_tiles;
     const int grid = CTAS * (int)std::min<int64_t>(tiles, sm_count / CTAS);
-    return launch_pdl(rows_kernel<BN, CTAS, FP8, MODE, F32>, dim3(grid), rows_threads(MODE), RCfg<BN, CTAS, MODE>::kSmemBytes, stream, CTAS, ma, mw, mu, mo, p,
+    return launch_pdl(rows_kernel<BN, CTAS, FP8, MODE, F32>, dim3(grid), rows_threads(MODE), RCfg<BN, CTAS, MODE, F32>::kSmemBytes, stream, CTAS, ma, mw, mu, mo, p,
                       d_error);
 }
 
 template <int BN, int CTAS, bool FP8, int MODE, bool F32>
 cudaError_t rows_set() {
-    return cudaFuncSetAttribute(rows_kernel<BN, CTAS, FP8, MODE, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, RCfg<BN, CTAS, MODE>::kSmemBytes);
+    return cudaFuncSetAttribute(rows_kernel<BN, CTAS, FP8, MODE, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, RCfg<BN, CTAS, MODE, F32>::kSmemBytes);
 }
 
 // The tiles of one form of the product: columns per tile, CTAs per tile.  A 32-bit result keeps its sums in registers, 64 a

@@ -29,15 +29,21 @@ int route_block_rows(int64_t rows) {
 }
 int64_t route_blocks(int64_t rows) { return (rows + route_block_rows(rows) - 1) / route_block_rows(rows); }
 
-// Order-preserving image of a float; 0 for what is never chosen (-inf, NaN).  +inf counts as the largest finite value, -0 as 0.
+// What a logit counts as: NaN as -inf, which is never chosen, +inf as the largest finite value of its type.
+template <typename T>
+__device__ __forceinline__ float route_logit(float x) {
+    return fminf(fmaxf(x, -INFINITY), sizeof(T) == 2 ? __uint_as_float(0x7f7f0000u) : FLT_MAX);
+}
+// Order-preserving image of a float (-0 as 0); below kRouteNone: -inf.
+constexpr uint32_t kRouteNone = 0x00800000u;
 __device__ __forceinline__ uint32_t route_key(float x) {
-    const uint32_t u = __float_as_uint(fminf(x, FLT_MAX) + 0.0f);
-    return x > -INFINITY ? ((u & 0x80000000u) ? ~u : (u | 0x80000000u)) : 0u;
+    const int s = __float_as_int(x + 0.0f);
+    return (uint32_t)(s ^ ((s >> 31) | (int)0x80000000));
 }
 __device__ __forceinline__ float route_value(uint32_t k) {
     return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
-// exp(x) for x <= 0: the argument's rounding is 2^-24 of it, the function's error 2^-22; what counts lies near 0.
+// exp(x) for x <= 0: the argument's rounding is 2^-24 of it, the function's error 2^-22, and what counts lies near 0.
 __device__ __forceinline__ float route_exp(float x) { return ptx::ex2_approx(x * 1.44269504f); }
 
 // LANES lanes take a row, PER neighbouring experts each, in registers.  A round finds the largest key below the one before as the
@@ -50,62 +56,59 @@ __device__ __forceinline__ void route_row(const RouteArgs& p, int row, bool live
     constexpr bool kPacked = sizeof(T) == 2;
     const int l = lane % LANES;
     uint32_t key[PER];
-    if (live) {
-        const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.ld;
-        constexpr int kVec = 16 / (int)sizeof(T);
-        if (PER % kVec == 0 && p.vec) {
+    float total = 0.0f, top;
+    uint32_t first;
+    // the largest of key - below (mod 2^32) over the row
+    auto most = [&](uint32_t below) {
+        uint32_t m = key[0] - below;
 #pragma unroll
-            for (int i = 0; i < PER; i += kVec) {
-                uint32_t w[4] = {0, 0, 0, 0};
-                const bool in = l * PER + i < p.n_experts;
-                if (in) {
-                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(x + l * PER + i));
-                    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-                }
+        for (int i = 1; i < PER; ++i) m = __viaddmax_u32(key[i], 0u - below, m);
 #pragma unroll
-                for (int j = 0; j < kVec; ++j) {
-                    float f;
-                    if constexpr (kPacked) f = __uint_as_float(j % 2 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
-                    else f = __uint_as_float(w[j]);
-                    key[(i + j) % PER] = in ? route_key(f) : 0u;
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < PER; ++i) key[i] = l * PER + i < p.n_experts ? route_key((float)x[l * PER + i]) : 0u;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) key[i] = 0u;
-    }
-    // the largest of f(key) over the row
-    auto most = [&](auto f) {
-        uint32_t m[PER];
-#pragma unroll
-        for (int i = 0; i < PER; ++i) m[i] = f(key[i]);
-#pragma unroll
-        for (int d = PER / 2; d; d >>= 1)
-#pragma unroll
-            for (int i = 0; i < d; ++i) m[i] = max(m[i], m[i + d]);
-        uint32_t best = m[0];
-#pragma unroll
-        for (int d = LANES / 2; d; d >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, d));
-        return best;
+        for (int d = LANES / 2; d; d >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+        return m;
     };
-    float total = 0.0f;
-    const uint32_t first = most([](uint32_t k) { return k; });
     // a packed key's lower half stands for the zeros of a bf16 value, inverted where it is negative
     auto value = [](uint32_t k) {
         if (kPacked) k = (k & 0xffff0000u) | ((k & 0x80000000u) ? 0u : 0xffffu);
         return route_value(k);
     };
-    const float top = first ? value(first) : 0.0f;
-    auto weight = [&](uint32_t k) { return route_exp(value(k) - top); };
-    if (!p.normalize) {
+    {
+        float f[PER];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) total += key[i] ? weight(key[i]) : 0.0f;
+        for (int i = 0; i < PER; ++i) f[i] = -INFINITY;
+        const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.ld;
+        constexpr int kVec = 16 / (int)sizeof(T);
+        if (PER % kVec == 0 && p.vec) {
 #pragma unroll
-        for (int d = LANES / 2; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+            for (int i = 0; i < PER; i += kVec) {
+                if (!live || l * PER + i >= p.n_experts) continue;
+                const uint4 v = __ldg(reinterpret_cast<const uint4*>(x + l * PER + i));
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) {
+                    if constexpr (kPacked) f[(i + j) % PER] = __uint_as_float(j % 2 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+                    else f[(i + j) % PER] = __uint_as_float(w[j]);
+                }
+            }
+        } else if (live) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (l * PER + i < p.n_experts) f[i] = (float)x[l * PER + i];
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            f[i] = route_logit<T>(f[i]);
+            key[i] = route_key(f[i]);
+            if (kPacked) key[i] = (key[i] & 0xffff0000u) | (0xffffu - (uint32_t)(l * PER + i));
+        }
+        first = most(0u);
+        top = first >= kRouteNone ? value(first) : 0.0f;
+        if (!p.normalize) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) total += route_exp(f[i] - top);
+#pragma unroll
+            for (int d = LANES / 2; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+        }
     }
     constexpr int kKeep = (kMaxTopK + LANES - 1) / LANES;  // lane l keeps the choices l, l + LANES, ...
     float mine[kKeep];
@@ -118,26 +121,22 @@ __device__ __forceinline__ void route_row(const RouteArgs& p, int row, bool live
         for (int i = 0; i < kKeep; ++i)
             if (l + i * LANES == j) { mine[i] = w; who[i] = e; }
     };
+    uint32_t best = first;
     if constexpr (kPacked) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-            if (key[i]) key[i] = (key[i] & 0xffff0000u) | (0xffffu - (uint32_t)(l * PER + i));
-        uint32_t best = most([](uint32_t k) { return k; });
         for (int j = 0; j < p.top_k; ++j) {
-            if (best) keep(j, weight(best), (int)(0xffffu - (best & 0xffffu)));
-            const uint32_t next = most([&](uint32_t k) { return k - best; }) + best;  // shuffles: by every lane, its row over or not
-            best = best ? next : 0u;
+            if (best >= kRouteNone) keep(j, route_exp(value(best) - top), (int)(0xffffu - (best & 0xffffu)));
+            const uint32_t next = most(best) + best;  // shuffles: by every lane, its row over or not
+            best = best >= kRouteNone ? next : 0u;
         }
     } else {
         const int group0 = lane / LANES * LANES;
-        uint32_t best = first;
         int j = 0;
-        while (__any_sync(0xffffffffu, best && j < p.top_k)) {
+        while (__any_sync(0xffffffffu, best >= kRouteNone && j < p.top_k)) {
             uint32_t has = 0;  // this lane's experts with that value
 #pragma unroll
             for (int i = 0; i < PER; ++i) has |= key[i] == best ? 1u << i : 0u;
-            if (!best) has = 0;
-            const float w = best ? weight(best) : 0.0f;
+            if (best < kRouteNone) has = 0;
+            const float w = best >= kRouteNone ? route_exp(value(best) - top) : 0.0f;
             while (true) {
                 const uint32_t lanes = (__ballot_sync(0xffffffffu, has != 0) >> group0) & (LANES == 32 ? 0xffffffffu : (1u << LANES) - 1u);
                 const bool go = lanes && j < p.top_k;
@@ -150,8 +149,8 @@ __device__ __forceinline__ void route_row(const RouteArgs& p, int row, bool live
                     if (lane == from) has &= has - 1;
                 }
             }
-            const uint32_t next = most([&](uint32_t k) { return k - best; }) + best;
-            best = best ? next : 0u;
+            const uint32_t next = most(best) + best;
+            best = best >= kRouteNone ? next : 0u;
         }
     }
     if (!live) return;
@@ -191,7 +190,8 @@ __device__ __forceinline__ int block_before(int n, int* warp_sum, int* all) {
 // The block's choices (in shared memory, in order) to their places.  base[e]: the first place of the block's rows of expert e.
 // Each warp takes a run of them, 32 at a time: equal experts are ranked by their lanes, behind those of the chunks and warps
 // before.  Called by the whole block; part: [kRouteWarps][n_experts].
-__device__ __forceinline__ void route_place(const RouteArgs& p, const int16_t* chosen, const int* base, uint16_t* part, int64_t first, int n) {
+__device__ __forceinline__ void route_place(const RouteArgs& p, const int16_t* chosen, const int* base, uint16_t* part, int row0, int n) {
+    const int64_t first = (int64_t)row0 * p.top_k;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int run = (n + kRouteWarps * 32 - 1) / (kRouteWarps * 32) * 32, lo = min(warp * run, n), hi = min(lo + run, n);
     for (int i = threadIdx.x; i < kRouteWarps * p.n_experts; i += kRouteThreads) part[i] = 0;
@@ -227,7 +227,7 @@ __device__ __forceinline__ void route_place(const RouteArgs& p, const int16_t* c
         if (e >= 0 && (same >> lane) == 1u) count[e] = (uint16_t)(rank + 1);
         __syncwarp();
         if (i0 + lane < hi) p.slots[first + i0 + lane] = at;
-        if (at >= 0) p.order[at] = (int)((first + i0 + lane) / p.top_k);
+        if (at >= 0) p.order[at] = row0 + (int)((uint32_t)(i0 + lane) / (uint32_t)p.top_k);
     }
 }
 
@@ -321,6 +321,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteA
 #pragma unroll
             for (int i = 0; i < kRouteSums / 32; ++i) {
                 const int b = i * 32 + lane;
+                if (i * 32 >= blocks) break;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int c = b < blocks && e0 + j < p.n_experts ? p.work[(int64_t)(e0 + j) * (blocks + 1) + b] : 0;
@@ -350,7 +351,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteA
     if (block == 0 && threadIdx.x == 0) p.offsets[p.n_experts] = used;
     for (int64_t i = max(first, (int64_t)used) + threadIdx.x; i < first + n; i += kRouteThreads) p.order[i] = -1;
     __syncthreads();
-    route_place(p, chosen, base, part, first, n);
+    route_place(p, chosen, base, part, block * block_rows, n);
 }
 
 // fn(kernel) for the form of the choice that a number of experts takes

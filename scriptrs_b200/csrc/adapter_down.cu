@@ -1,10 +1,10 @@
-// Down-projection of the low-rank adapters: low[i] = scale_a (x[i] D_a^T) for the adapter a of row i, kept in 32 bits, and for
-// the rows of every tile of the product the list of the adapters among them, in the order of their first rows.
+// Down-projection of the low-rank adapters: low[i] = scale_a (x[i] D_a^T) for the adapter a of row i, kept in 32 bits.
 //
-// Bound by reading the rows once (2 K bytes each against K * rank products).  Two kernels:
+// Bound by reading the rows once (2 K bytes each against K * rank products).  Three kernels:
 //   - many rows: 128 rows a CTA on tcgen05, rows and adapters through a TMA ring; a pass over K for every few adapters among the
 //     rows, each with the lanes of the other rows disabled (nothing of one adapter reaches another's rows).
-//   - few rows: 16 rows a block on mma.sync m16n8k16 with operands straight from global memory, K over the warps, the columns over
+//   - very few rows: a warp per row and eight columns, K over the lanes.
+//   - between them: 16 rows a block on mma.sync m16n8k16 with operands straight from global memory, K over the warps, the columns over
 //     blocks; a row takes its adapter's product (selected, not masked by zeros).
 // Where nearly every row has its own adapter (live streams), such passes would run one after the other; there a row is a chain of
 // dot products over the lanes of a warp.
@@ -14,6 +14,7 @@
 
 #include <algorithm>
 
+#include "adapter_ids.cuh"
 #include "launch.cuh"
 #include "rows.h"
 #include "tc_ptx.cuh"
@@ -35,34 +36,6 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
 __device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float s) {
     s = fmaf(__uint_as_float(a << 16), __uint_as_float(b << 16), s);
     return fmaf(__uint_as_float(a & 0xffff0000u), __uint_as_float(b & 0xffff0000u), s);
-}
-
-// The adapters of the list_rows rows from row0 on.
-__device__ __forceinline__ void write_list(const AdapterDownArgs& p, int row0, int lane) {
-    int ids[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int r = row0 + 8 * lane + j;
-        ids[j] = 8 * lane + j < p.list_rows && r < p.M ? __ldg(p.row_adapter + r) : -1;
-        if ((unsigned)ids[j] >= (unsigned)p.n_adapters) ids[j] = -1;
-    }
-    int32_t* list = p.lists + (int64_t)(row0 / p.list_rows) * kAdapterListInts;
-    int count = 0;
-    while (true) {
-        int first = -1;
-#pragma unroll
-        for (int j = 7; j >= 0; --j)
-            if (ids[j] >= 0) first = ids[j];
-        const uint32_t have = __ballot_sync(0xffffffffu, first >= 0);
-        if (!have) break;
-        const int cur = __shfl_sync(0xffffffffu, first, __ffs(have) - 1);
-        if (lane == 0) list[4 + count] = cur;
-        ++count;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (ids[j] == cur) ids[j] = -1;
-    }
-    if (lane == 0) list[0] = count;
 }
 
 // Eight columns of a row's product, K over the lanes, AHEAD steps of 256 columns asked for at once; lane j < 8 returns column j.
@@ -101,17 +74,12 @@ __device__ __forceinline__ float row_dots(const __nv_bfloat16* x, const __nv_bfl
     return v;
 }
 
-// Very few rows: a warp per row and eight columns, one block more for the lists.
+// Very few rows: a warp per row and eight columns.
 __global__ void __launch_bounds__(kDownWarps * 32, 1) adapter_down_dots_kernel(const AdapterDownArgs p, int groups) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_wait();
     pdl_trigger();
-    const int block = (int)blockIdx.x - 1;
-    if (block < 0) {
-        for (int r = warp * p.list_rows; r < p.M; r += kDownWarps * p.list_rows) write_list(p, r, lane);
-        return;
-    }
-    const int64_t item = (int64_t)block * kDownWarps + warp;
+    const int64_t item = (int64_t)blockIdx.x * kDownWarps + warp;
     const int row = (int)(item / groups), c = (int)(item % groups) * 8;
     if (row >= p.M) return;
     const int id = __ldg(p.row_adapter + row);
@@ -132,9 +100,7 @@ __global__ void __launch_bounds__(kDownWarps * 32, 1) adapter_down_kernel(const 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int row0 = blockIdx.x * kRows, col0 = blockIdx.y * kCols;
     pdl_wait();
-    pdl_trigger();  // what runs beside this block may rely on all that came before it, but not on `low` and the lists
-
-    if (blockIdx.y == 0 && row0 % p.list_rows == 0 && warp == kDownWarps - 1) write_list(p, row0, lane);
+    pdl_trigger();  // what runs beside this block may rely on all that came before it, but not on `low`
 
     const int my_row = row0 + (lane & 15);
     int id = my_row < p.M ? __ldg(p.row_adapter + my_row) : -1;
@@ -247,32 +213,6 @@ struct DownTc {
     static constexpr int stages(bool alone) { return std::min((alone ? 224 : 110) * 1024 / kStageBytes, kTcMaxStages); }
 };
 
-// The adapters among 128 rows, four rows a lane, in the order of their first rows; -1 after the last one.
-struct IdWalk {
-    int ids[4];
-    __device__ __forceinline__ IdWalk(const AdapterDownArgs& p, int row0, int lane) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int r = row0 + 4 * lane + j;
-            ids[j] = r < p.M ? __ldg(p.row_adapter + r) : -1;
-            if ((unsigned)ids[j] >= (unsigned)p.n_adapters) ids[j] = -1;
-        }
-    }
-    __device__ __forceinline__ int next() {
-        int first = -1;
-#pragma unroll
-        for (int j = 3; j >= 0; --j)
-            if (ids[j] >= 0) first = ids[j];
-        const uint32_t have = __ballot_sync(0xffffffffu, first >= 0);
-        if (!have) return -1;
-        const int cur = __shfl_sync(0xffffffffu, first, __ffs(have) - 1);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (ids[j] == cur) ids[j] = -1;
-        return cur;
-    }
-};
-
 // Warp 0 loads, warp 1 issues the MMAs, warps 2 to 5 read the results, a row per thread.
 template <int RN>
 __global__ void __launch_bounds__(kTcThreads) adapter_down_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_d,
@@ -312,13 +252,15 @@ __global__ void __launch_bounds__(kTcThreads) adapter_down_tc_kernel(const __gri
     // every warp counts the adapters for itself
     int found = 0;
     {
-        IdWalk w(p, row0, lane);
+        AdapterIds<kTcRows> w;
+        w.load(p.row_adapter, p.n_adapters, row0, p.M, lane);
         while (found <= kTcMaxPasses * C::kAtOnce && w.next() >= 0) ++found;
     }
     const bool dots = found > kTcMaxPasses * C::kAtOnce;
 
     if (warp == 0 && !dots) {
-        IdWalk w(p, row0, lane);
+        AdapterIds<kTcRows> w;
+        w.load(p.row_adapter, p.n_adapters, row0, p.M, lane);
         int stage = 0;
         uint32_t ph = 0;
         bool ok = true;
@@ -352,7 +294,8 @@ __global__ void __launch_bounds__(kTcThreads) adapter_down_tc_kernel(const __gri
     } else if (warp == 1 && !dots) {
         // fp32 accumulate, bf16 operands, both K-major, M = 128, N = RN
         constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(RN >> 3) << 17) | ((uint32_t)(kTcRows >> 4) << 24);
-        IdWalk w(p, row0, lane);
+        AdapterIds<kTcRows> w;
+        w.load(p.row_adapter, p.n_adapters, row0, p.M, lane);
         int mine[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) mine[q] = row0 + 32 * q + lane < p.M ? __ldg(p.row_adapter + row0 + 32 * q + lane) : -1;
@@ -394,7 +337,6 @@ __global__ void __launch_bounds__(kTcThreads) adapter_down_tc_kernel(const __gri
         if (ok && elect_one()) tc_commit(done_bar);
         __syncwarp();
     } else if (!dots) {
-        if (warp == 2 && row0 % p.list_rows == 0) write_list(p, row0, lane);
         const bool ok = __all_sync(0xffffffffu, mbar_wait(done_bar, 0, abort_flag));
         tc_fence_after();
         const int quad = warp & 3, row = row0 + 32 * quad + lane;
@@ -419,7 +361,6 @@ __global__ void __launch_bounds__(kTcThreads) adapter_down_tc_kernel(const __gri
             }
         }
     } else {
-        if (warp == 2 && row0 % p.list_rows == 0) write_list(p, row0, lane);
         const __nv_bfloat16* a = static_cast<const __nv_bfloat16*>(p.a);
         const __nv_bfloat16* down = static_cast<const __nv_bfloat16*>(p.down);
         for (int r = warp; r < kTcRows && row0 + r < p.M; r += kTcThreads / 32) {
@@ -485,7 +426,7 @@ cudaError_t adapter_down_launch(const AdapterDownArgs& g, int sm_count, int* d_e
     }
     if ((int64_t)g.M * g.rank <= kDotsMost) {
         const int groups = g.rank / 8;
-        const int blocks = 1 + (g.M * groups + kDownWarps - 1) / kDownWarps;
+        const int blocks = (g.M * groups + kDownWarps - 1) / kDownWarps;
         return launch_pdl(adapter_down_dots_kernel, dim3(blocks), kDownWarps * 32, 0, stream, 1, g, groups);
     }
     // the columns are spread over blocks too, as far as that fills the SMs

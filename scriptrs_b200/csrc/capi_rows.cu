@@ -46,8 +46,7 @@ int64_t sb_route_topk_workspace(int64_t rows, int64_t n_experts, int64_t top_k) 
 
 int64_t sb_adapter_gemm_workspace(int64_t M, int64_t rank) {
     if (M <= 0 || M > kLimit - 128 || rank <= 0 || rank > kMaxRank) return 0;
-    // low [M x rank] f32 (whole 16 bytes: rank is a multiple of 8), then a list for every 128 rows
-    return (M * rank + (M + 127) / 128 * kAdapterListInts) * 4;
+    return M * rank * 4;  // the rows' products with the adapters' first matrices, f32
 }
 
 int32_t sb_route_topk(sb_ctx* c, const void* d_logits, int32_t logits_bf16, int64_t ld, int64_t rows, int64_t n_experts, int64_t top_k,
@@ -143,14 +142,12 @@ int32_t sb_adapter_gemm(sb_ctx* c, const void* d_a, int64_t lda, const void* d_w
     if (M == 0) return SB_OK;
     SB_CUDA(cudaSetDevice(c->device));
     float* low = static_cast<float*>(d_work);
-    int32_t* lists = reinterpret_cast<int32_t*>(low + M * rank);
     RowsArgs g{};
     g.a = d_a; g.w = d_w; g.bias = d_bias; g.out = d_out; g.a_rows = M; g.lda = lda; g.ldo = ldo; g.M = (int)M; g.N = (int)N; g.K = (int)K;
     g.n_groups = 1; g.act = act; g.out_mode = out_mode; g.alpha = alpha;
-    g.row_adapter = d_row_adapter; g.up = d_up; g.low = low; g.lists = lists; g.n_adapters = (int)n_adapters; g.rank = (int)rank;
+    g.row_adapter = d_row_adapter; g.up = d_up; g.low = low; g.n_adapters = (int)n_adapters; g.rank = (int)rank;
     AdapterDownArgs d{};
-    d.a = d_a; d.down = d_down; d.scale = d_scale; d.row_adapter = d_row_adapter; d.low = low; d.lists = lists; d.lda = lda;
-    d.list_rows = 128 * rows_shape(g, c->sm_count).ctas;
+    d.a = d_a; d.down = d_down; d.scale = d_scale; d.row_adapter = d_row_adapter; d.low = low; d.lda = lda;
     d.M = (int)M; d.K = (int)K; d.rank = (int)rank; d.n_adapters = (int)n_adapters;
     c->prof.begin("adapter_down", c->stream);
     cudaError_t e = adapter_down_launch(d, c->sm_count, c->d_error, c->stream);

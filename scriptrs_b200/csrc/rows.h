@@ -27,14 +27,10 @@ struct RowsArgs {
     const int32_t* row_adapter;  // [M], ids outside [0, n_adapters): none; null: no adapters
     const void* up;              // [n_adapters x N x rank] bf16
     const float* low;            // [M x rank] f32, scaled; written by the kernel ahead in the stream
-    const int32_t* lists;        // per tile's rows: number of adapters, their ids in the order of their first rows
     int n_adapters, rank;
 };
-constexpr int kAdapterListInts = 260;  // a count, padding to 16 bytes, an id per row of the tile
 
 cudaError_t rows_configure(const char** why);
-// The tile that rows_launch takes.
-RowsTileShape rows_shape(const RowsArgs& g, int sm_count);
 // cudaErrorInvalidValue: a tensor map was refused (alignment or size).
 cudaError_t rows_launch(const RowsArgs& g, int sm_count, int* d_error, cudaStream_t stream);
 // 2-D row-major tensor; boxes of 128 bytes x box_rows, 128-byte swizzle.
@@ -55,8 +51,6 @@ struct AdapterDownArgs {
     const float* scale;  // [n_adapters] or null
     const int32_t* row_adapter;
     float* low;          // [M x rank]
-    int32_t* lists;      // [ceil(M / list_rows) x kAdapterListInts]
-    int list_rows;       // rows of a tile of the product: 128 or 256
     int64_t lda;
     int M, K, rank, n_adapters;
 };

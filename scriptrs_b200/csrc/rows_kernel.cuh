@@ -29,6 +29,7 @@
 
 #include <algorithm>
 
+#include "adapter_ids.cuh"
 #include "gemm_tile.h"
 #include "launch.cuh"
 #include "rows.h"
@@ -173,8 +174,7 @@ struct RowsParams {
     // adapters
     const int32_t* row_adapter;
     const float* low;
-    const int32_t* lists;
-    int rank;
+    int rank, n_adapters;
 };
 
 // A tile: rows [row0, row1) of the output, columns from col0, weights of group `group`.
@@ -412,11 +412,11 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
     const uint32_t tmem_base = *tmem_slot;
     pdl_trigger();
     // The adapters' kernel ahead in the stream waits for everything before it and lets this one start after that: only what
-    // it writes itself (low, lists) has to be waited for here, by the warps that read it.
+    // it writes itself (low) has to be waited for here, by the warps that read it.
     if (MODE != kAdapters) pdl_wait();
-    bool waited = false;
+    constexpr int kTileRows = kBM * CTAS;
 
-    TileWalk<kBM * CTAS> walk(MODE == kAdapters ? nullptr : p.offsets, p.M, MODE == kAdapters ? 1 : p.n_groups, n_tiles, lane);
+    TileWalk<kTileRows> walk(MODE == kAdapters ? nullptr : p.offsets, p.M, MODE == kAdapters ? 1 : p.n_groups, n_tiles, lane);
     RowsTile tile;
 
     if (warp == 0) {
@@ -434,13 +434,8 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
 #pragma unroll
                 for (int c = 0; c < CTAS; ++c) a_bytes += (uint32_t)((min(max(tile.row1 - tile.row0 - c * kBM, 0), kBM) + 3) >> 2) * (4 * kRowBytes);
             }
-            // the tile's adapters, on their way while the shared columns of K are fetched
-            const int32_t* list = nullptr;
-            int count = 0, ids = 0;
-            if (MODE == kAdapters) {
-                list = p.lists + (int64_t)(tile.row0 / (kBM * CTAS)) * kAdapterListInts;
-                if (waited) { count = list[0]; ids = list[4 + lane]; }
-            }
+            AdapterIds<kTileRows> all;  // on their way while the shared columns of K are fetched
+            if (MODE == kAdapters) all.load(p.row_adapter, p.n_adapters, tile.row0, tile.row1, lane);
             bool failed = false;
             if (elect_one()) {
                 int s = stage;
@@ -461,16 +456,19 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
             ph ^= (uint32_t)(stage / S) & 1u;
             stage %= S;
             if constexpr (MODE == kAdapters) {
-                if (!waited) { pdl_wait(); waited = true; count = list[0]; ids = list[4 + lane]; }
                 for (int c = 0; c < phases; ++c) {
-                    for (int j0 = 0; ok && j0 < count; j0 += C::kUps) {
-                        const int n = min(C::kUps, count - j0);
-                        if (count > 32) ids = list[4 + j0 + (lane < n ? lane : 0)];  // else lane j holds adapter j
+                    AdapterIds<kTileRows> ids = all;
+                    for (int id = ids.next(); ok && id >= 0;) {
+                        int u_row[C::kUps], n = 0;
+#pragma unroll
+                        for (int u = 0; u < C::kUps; ++u) {
+                            if (id < 0) continue;
+                            u_row[u] = id * p.N + w_col;
+                            n = u + 1;
+                            id = ids.next();
+                        }
                         ok = __all_sync(0xffffffffu, mbar_wait(empty_bar(stage), ph ^ 1, abort_flag));
                         if (!ok) break;
-                        int u_row[C::kUps];
-#pragma unroll
-                        for (int u = 0; u < C::kUps; ++u) u_row[u] = __shfl_sync(0xffffffffu, ids, (count > 32 ? u : j0 + u) & 31) * p.N + w_col;
                         if (elect_one()) {
                             if (rank == 0) mbar_expect_tx(full_bar(stage), CTAS * C::kBBytes * n);
 #pragma unroll
@@ -495,20 +493,15 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
         uint32_t ph = 0, seg = 0, low_ph = 0;
         bool ok = true;
         for (long long t = tile0; rank == 0 && ok && walk.find(t, BN, tile); t += tile_step) {
-            const int32_t* list = nullptr;
-            int count = 0, ids = 0, mine[4 * CTAS];
-            auto fetch = [&]() {
-                count = list[0];
-                ids = list[4 + lane];
+            AdapterIds<kTileRows> all;
+            int mine[4 * CTAS];  // of rows 32 q + lane
+            if (MODE == kAdapters) {
+                all.load(p.row_adapter, p.n_adapters, tile.row0, tile.row1, lane);
 #pragma unroll
                 for (int q = 0; q < 4 * CTAS; ++q) {
                     const int row = tile.row0 + q * 32 + lane;
                     mine[q] = row < tile.row1 ? __ldg(p.row_adapter + row) : -1;
                 }
-            };
-            if (MODE == kAdapters) {
-                list = p.lists + (int64_t)(tile.row0 / (kBM * CTAS)) * kAdapterListInts;
-                if (waited) fetch();
             }
             int kt = 0;
             while (ok && kt < k_tiles) {
@@ -539,21 +532,20 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                 stage %= S;
                 if constexpr (MODE == kAdapters) {
                     if (ok && last) {
-                        if (!waited) { pdl_wait(); waited = true; fetch(); }
-                        for (int c = 0; count > 0 && c < phases; ++c) {
-                            ok = ok && __all_sync(0xffffffffu, rows_wait_pair<CTAS>(low_bar, low_ph, abort_flag));
+                        for (int c = 0; ok && c < phases; ++c) {
+                            AdapterIds<kTileRows> ids = all;
+                            int id = ids.next();
+                            if (id < 0) break;
+                            ok = __all_sync(0xffffffffu, rows_wait_pair<CTAS>(low_bar, low_ph, abort_flag));
                             low_ph ^= 1;
                             const int groups = min(kGroups, (p.rank - c * kPhaseCols + 15) / 16);
-                            for (int j0 = 0; ok && j0 < count; j0 += C::kUps) {
-                                const int n = min(C::kUps, count - j0);
-                                if (count > 32) ids = list[4 + j0 + (lane < n ? lane : 0)];
+                            while (ok && id >= 0) {
                                 ok = __all_sync(0xffffffffu, mbar_wait(full_bar(stage), ph, abort_flag));
                                 if (!ok) break;
                                 tc_fence_after();
 #pragma unroll
                                 for (int u = 0; u < C::kUps; ++u) {
-                                    if (u >= n) break;
-                                    const int id = __shfl_sync(0xffffffffu, ids, (count > 32 ? u : j0 + u) & 31);
+                                    if (id < 0) continue;
                                     uint32_t off[4 * CTAS];
 #pragma unroll
                                     for (int q = 0; q < 4 * CTAS; ++q) off[q] = ~__ballot_sync(0xffffffffu, mine[q] == id);
@@ -572,10 +564,11 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                                         }
                                     }
                                     __syncwarp();
+                                    id = ids.next();
                                 }
                                 if (elect_one()) {
                                     rows_commit<CTAS>(empty_bar(stage));
-                                    if (j0 + n == count) rows_commit<CTAS>(lowfree_bar);
+                                    if (id < 0) rows_commit<CTAS>(lowfree_bar);
                                 }
                                 __syncwarp();
                                 if (++stage == S) { stage = 0; ph ^= 1; }
@@ -788,9 +781,11 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
         bool ok = true;
         pdl_wait();
         for (long long t = tile0; ok && walk.find(t, BN, tile); t += tile_step) {
-            const int count = p.lists[(int64_t)(tile.row0 / (kBM * CTAS)) * kAdapterListInts];
+            AdapterIds<kTileRows> ids;
+            ids.load(p.row_adapter, p.n_adapters, tile.row0, tile.row1, lane);
+            if (ids.next() < 0) continue;
             const int row = tile.row0 + cta_row + r;
-            for (int c = 0; count > 0 && c < phases; ++c) {
+            for (int c = 0; c < phases; ++c) {
                 float f[kPhaseCols];
 #pragma unroll
                 for (int i = 0; i < kPhaseCols; i += 4) {
@@ -859,7 +854,7 @@ cudaError_t rows_launch_t(const RowsArgs& g, int sm_count, int* d_error, cudaStr
     p.out_vec = !(reinterpret_cast<uintptr_t>(g.out) & 15) && !((g.ldo * eb) & 15);
     mo = mw;
     if (p.out_vec && !rows_out_map(&mo, g.out, g.M, g.N, g.ldo, F32, F32 || RCfg<BN, CTAS, MODE, F32>::kHalfCols >= 64 ? 128 : 64)) return cudaErrorInvalidValue;
-    p.row_adapter = g.row_adapter; p.low = g.low; p.lists = g.lists; p.rank = g.rank;
+    p.row_adapter = g.row_adapter; p.low = g.low; p.rank = g.rank; p.n_adapters = g.n_adapters;
     // at most this many tiles: a group's last one may be short
     const int64_t n_tiles = (g.N + BN - 1) / BN;
     const int64_t tiles = ((int64_t)(g.M + kBM * CTAS - 1) / (kBM * CTAS) + std::min(g.n_groups - 1, g.M)) * n_tiles;

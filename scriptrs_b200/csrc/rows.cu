@@ -50,7 +50,7 @@ cudaError_t rows_configure(const char** why) {
         }
         g_rows_encode = reinterpret_cast<EncodeTiledFn>(fn);
     }
-    for (cudaError_t (*set)() : {rows_grouped_configure, rows_gathered_configure, rows_adapters_configure, adapter_down_configure, route_configure}) {
+    for (cudaError_t (*set)() : {rows_grouped_configure, rows_gathered_configure, rows_adapters_configure, rows_few_configure, adapter_down_configure, route_configure}) {
         const cudaError_t e = set();
         if (e != cudaSuccess) {
             if (why) *why = "shared-memory opt-in for the row products failed";
@@ -64,6 +64,7 @@ cudaError_t rows_launch(const RowsArgs& g, int sm_count, int* d_error, cudaStrea
     if (!g_rows_encode) return cudaErrorNotReady;
     if (g.M <= 0) return cudaSuccess;
     const RowsTileShape t = rows_tile(g.M, g.N, g.n_groups, g.out_mode != kOutBf16, sm_count);
+    if (rows_few(g)) return rows_few_launch(g, t, sm_count, d_error, stream);
     if (g.row_adapter) return rows_adapters_launch(g, t, sm_count, d_error, stream);
     // few rows a group: gathers fetch only those, a box always 128
     if (g.rows || (int64_t)g.M < (int64_t)g.n_groups * 64) return rows_gathered_launch(g, t, sm_count, d_error, stream);

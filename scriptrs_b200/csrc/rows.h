@@ -37,7 +37,10 @@ cudaError_t rows_launch(const RowsArgs& g, int sm_count, int* d_error, cudaStrea
 bool rows_map(CUtensorMap* map, const void* ptr, int64_t rows, int64_t cols, int64_t pitch, bool fp8, int box_rows);
 // The result's map: boxes of 32 rows x row_bytes (64 or 128, swizzled over as many).
 bool rows_out_map(CUtensorMap* map, void* ptr, int64_t rows, int64_t cols, int64_t pitch, bool f32, int row_bytes);
-// The forms of the kernel (rows_grouped.cu, rows_gathered.cu, rows_adapters.cu).
+// The forms of the kernel (rows_grouped.cu, rows_gathered.cu, rows_adapters.cu, rows_few.cu).
+cudaError_t rows_few_configure();
+bool rows_few(const RowsArgs& g);
+cudaError_t rows_few_launch(const RowsArgs& g, RowsTileShape t, int sm_count, int* d_error, cudaStream_t stream);
 cudaError_t rows_grouped_configure();
 cudaError_t rows_gathered_configure();
 cudaError_t rows_adapters_configure();

@@ -17,6 +17,9 @@
 //     Where the result is stored in 32 bits it enters as three bf16 terms (2^-26).
 //     A tile may hold rows of several adapters: its MMAs run once for each, with the lanes of the other rows disabled, so that
 //     nothing of one adapter (not even a NaN) reaches rows of another, and the shared weights are read once whatever the adapters.
+//   - Up to 32 rows (live streams, as a rule each with an adapter of its own): an MMA per adapter would take longer than all of
+//     K, so the addition is formed on CUDA cores by the four warps that stage `low` otherwise, in 32 bits, U_a on its way before
+//     `low` is there, and the epilogue adds it (24 rows with as many adapters, rank 16, 1024 -> 4096: 14.8 -> 10.1 us).
 //   - The tensor core adds into its accumulator by truncation, 1e-6 of the result at K = 1024 and 4.4e-6 at 4096 (measured).
 //     Where the result is stored in 32 bits, it is collected in registers every kSegment stages, rounded to nearest (4.7e-7 at
 //     either K; every four stages: 2.5e-7, but 16384 x 1024 x 1024 then takes 48 us instead of 36, a handshake per segment).
@@ -45,27 +48,34 @@ constexpr int kBM = 128;
 constexpr int kRowBytes = 128;  // of an operand row in a stage: one swizzle row
 constexpr int kEpiWarps = 8;
 constexpr int kSlabBytes = 32 * 128;
+constexpr int kFewRows = 32, kFewPitch = kFewRows + 1;  // rows of the few-row forms; an odd pitch spreads both sides over the banks
 constexpr int kSegment = 8;     // stages (64 bf16 or 128 e4m3 columns of K each) between two collections of a 32-bit result
 
-enum RowsMode : int { kGrouped = 0, kGathered = 1, kAdapters = 2 };
+enum RowsMode : int { kGrouped = 0, kGathered = 1, kAdapters = 2, kFewAdapters = 3, kFewGathered = 4 };
+constexpr bool rows_few(int mode) { return mode == kFewAdapters || mode == kFewGathered; }
+constexpr bool rows_gathers(int mode) { return mode == kGathered || mode == kFewGathered; }
 
 // CTAS = 2: a cluster of two CTAs on 256 rows x BN columns (tcgen05 cta_group::2); each stages its own 128 rows of A and its own
 // half of the W rows.
 template <int BN, int CTAS, int MODE, bool F32>
 struct RCfg {
-    static constexpr int kABytes = kBM * kRowBytes;
+    // The few-row forms stage 32 rows of A.  The MMA reads 128: the others are whatever lies behind, and so are their lanes of the
+    // accumulator, which nobody reads.  What that saves goes into stages: narrow tiles are paced by the weights in flight
+    // (24 rows, 1024 -> 4096: @RING@).
+    static constexpr int kABytes = (rows_few(MODE) ? kFewRows : kBM) * kRowBytes;
     static constexpr int kBBytes = BN / CTAS * kRowBytes;
     static constexpr int kStageBytes = kABytes + kBBytes;
     // `low` of the tile's rows as an operand: blocks of 16 of its columns (32 bytes a row), four to an operand tile
     static constexpr int kTerms = F32 ? 3 : 1, kGroups = F32 ? 2 : 4;  // bf16 terms, blocks of columns that are held at once
-    static constexpr int kLowBytes = MODE == kAdapters ? (kTerms * kGroups + 3) / 4 * kBM * kRowBytes : 0;
+    static constexpr int kLowBytes = MODE == kAdapters ? (kTerms * kGroups + 3) / 4 * kBM * kRowBytes
+                                                       : (MODE == kFewAdapters ? (BN * kFewPitch * 4 + 1023) / 1024 * 1024 : 0);  // the addition, by column
     static constexpr int kColumnBytes = 2 * BN * 4;                                // bias and column scales of the tile
-    static constexpr int kIndexBytes = MODE == kGathered ? kBM * 4 : 0;
-    static constexpr int kBarBytes = 256;
+    static constexpr int kIndexBytes = rows_gathers(MODE) ? kBM * 4 : 0;
+    static constexpr int kBarBytes = 384;
     static constexpr int kFixedBytes = kLowBytes + kEpiWarps * kSlabBytes + kColumnBytes + kIndexBytes + kBarBytes;
-    static constexpr int kStages = std::min((227 * 1024 - kFixedBytes) / kStageBytes, 8);
+    static constexpr int kStages = std::min((227 * 1024 - kFixedBytes) / kStageBytes, rows_few(MODE) ? 16 : 8);
     static constexpr int kSmemBytes = kStages * kStageBytes + kFixedBytes;
-    static_assert(kStages >= 3 && 8 * (2 * kStages + 6) + 16 <= kBarBytes, "shared memory");
+    static_assert(kLowBytes % 1024 == 0 && kStages >= 3 && 8 * (2 * kStages + 6) + 16 <= kBarBytes, "shared memory");
     static constexpr int kUps = kStageBytes / kBBytes;  // adapters' tiles of `up` in a stage
     static constexpr int kHalves = gemm_halves(BN);
     static constexpr int kHalfCols = BN / kHalves;
@@ -174,6 +184,7 @@ struct RowsParams {
     // adapters
     const int32_t* row_adapter;
     const float* low;
+    const void* up;
     int rank, n_adapters;
 };
 
@@ -391,7 +402,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
             mbar_init(tempty_bar(a), 4 * C::kHalves * CTAS);
         }
         mbar_init(low_bar, kAuxWarps * CTAS);
-        mbar_init(lowfree_bar, 1);
+        mbar_init(lowfree_bar, MODE == kFewAdapters ? C::kHalves : 1);
         *abort_flag = 0;
         rows_set_turn(turn_at, 0);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -413,10 +424,11 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
     pdl_trigger();
     // The adapters' kernel ahead in the stream waits for everything before it and lets this one start after that: only what
     // it writes itself (low) has to be waited for here, by the warps that read it.
-    if (MODE != kAdapters) pdl_wait();
+    constexpr bool kHasAdapters = MODE == kAdapters || MODE == kFewAdapters;
+    if (!kHasAdapters) pdl_wait();
     constexpr int kTileRows = kBM * CTAS;
 
-    TileWalk<kTileRows> walk(MODE == kAdapters ? nullptr : p.offsets, p.M, MODE == kAdapters ? 1 : p.n_groups, n_tiles, lane);
+    TileWalk<kTileRows> walk(kHasAdapters ? nullptr : p.offsets, p.M, kHasAdapters ? 1 : p.n_groups, n_tiles, lane);
     RowsTile tile;
 
     if (warp == 0) {
@@ -429,7 +441,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
             const int w_row = tile.group * p.N + w_col;
             // bytes of A that the pair fetches: whole boxes, or the quads of rows that the gathers bring
             uint32_t a_bytes = CTAS * C::kABytes;
-            if (MODE == kGathered) {
+            if (rows_gathers(MODE)) {
                 a_bytes = 0;
 #pragma unroll
                 for (int c = 0; c < CTAS; ++c) a_bytes += (uint32_t)((min(max(tile.row1 - tile.row0 - c * kBM, 0), kBM) + 3) >> 2) * (4 * kRowBytes);
@@ -442,9 +454,9 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                 uint32_t sp = ph;
                 for (int kt = 0; kt < k_tiles; ++kt) {
                     if (!mbar_wait(empty_bar(s), sp ^ 1, abort_flag)) { failed = true; break; }
-                    if (MODE == kGathered) rows_set_turn(turn_at, begun + (uint32_t)kt + 1);
+                    if (rows_gathers(MODE)) rows_set_turn(turn_at, begun + (uint32_t)kt + 1);
                     if (rank == 0) mbar_expect_tx(full_bar(s), CTAS * C::kBBytes + a_bytes);
-                    if (MODE != kGathered)
+                    if (!rows_gathers(MODE))
                         rows_load<CTAS>(a_base + s * C::kStageBytes, &tma_a, lead(full_bar(s)), kt * kStepCols, tile.row0 + cta_row);
                     rows_load<CTAS>(b_base + s * C::kStageBytes, &tma_w, lead(full_bar(s)), kt * kStepCols, w_row);
                     if (++s == S) { s = 0; sp ^= 1; }
@@ -586,7 +598,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
         // ------------------------------------------------------------ epilogue
         const int ew = warp - 2, quad = warp & 3, half = ew >> 2;
         unsigned char* slab = base_ptr + kSlabAt + ew * kSlabBytes;
-        uint32_t seg = 0;
+        uint32_t seg = 0, tiles = 0;
         bool ok = true;
         const int cbeg = half * C::kHalfCols;
         float* columns = reinterpret_cast<float*>(base_ptr + kColumnAt) + cbeg;  // bias; the scales BN further on
@@ -625,8 +637,8 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
             const int row = row0 + lane;
             const bool live = row < tile.row1;
             int src = row;
-            if (MODE == kGathered && p.rows && live) src = __ldg(p.rows + row);
-            const bool known = MODE != kGathered || (unsigned)src < (unsigned long long)p.a_rows;
+            if (rows_gathers(MODE) && p.rows && live) src = __ldg(p.rows + row);
+            const bool known = !rows_gathers(MODE) || (unsigned)src < (unsigned long long)p.a_rows;
             const float rs = FP8 && p.row_scale && live && known ? __ldg(p.row_scale + src) : 1.0f;
             const bool any = row0 < tile.row1;  // rows of this warp in the tile
             auto taddr = [&]() { return tmem_base + ((uint32_t)(quad * 32) << 16) + (seg & 1) * BN + cbeg; };
@@ -640,6 +652,16 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                 ++seg;
             };
             const bool whole = p.out_vec && row0 + 32 <= tile.row1;  // 32 rows of this group: one TMA store
+            const float* addition = reinterpret_cast<const float*>(base_ptr + kLowAt) + lane;  // of this row; columns kFewPitch apart
+            if (MODE == kFewAdapters && any) {
+                ok = __all_sync(0xffffffffu, mbar_wait(low_bar, tiles & 1, abort_flag));
+                if (!ok) continue;
+            }
+            ++tiles;
+            auto added = [&]() {
+                __syncwarp();
+                if (MODE == kFewAdapters && lane == 0) mbar_arrive(lowfree_bar);
+            };
             auto ready = [&]() {  // the store before has read the slab
                 if (elect_one()) bulk_wait_read0();
                 __syncwarp();
@@ -681,6 +703,11 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                     release();
                 }
                 if (!ok || !any) continue;
+                if (MODE == kFewAdapters) {
+#pragma unroll
+                    for (int j = 0; j < kCols; ++j) sum[j] += addition[(cbeg + j) * kFewPitch];
+                    added();
+                }
 #pragma unroll
                 for (int c = 0; c < kCols; c += 32) {
                     const int col0 = tile.col0 + cbeg + c;
@@ -721,6 +748,10 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                             float x[32];
 #pragma unroll
                             for (int j = 0; j < 32; ++j) x[j] = __uint_as_float(v[j]);
+                            if (MODE == kFewAdapters) {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) x[j] += addition[(cbeg + c + 32 * sub + j) * kFewPitch];
+                            }
                             rows_finish<FP8, F32>(x, p, reinterpret_cast<const float4*>(columns + c + 32 * sub),
                                                   reinterpret_cast<const float4*>(columns + BN + c + 32 * sub), rs, known);
 #pragma unroll
@@ -735,11 +766,12 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                     }
                 }
                 if (held) release();
+                if (any) added();
             }
         }
         if (elect_one()) bulk_wait_all();
         __syncwarp();
-    } else if constexpr (MODE == kGathered) {
+    } else if constexpr (rows_gathers(MODE)) {
         // ------------------------------------------------------------ gathers, 32 rows a warp
         const int gw = warp - 2 - kEpiWarps;
         int32_t* index = reinterpret_cast<int32_t*>(base_ptr + kIndexAt) + gw * 32;
@@ -772,6 +804,59 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
         if (!ok) {
             const long long t0 = clock64();
             while (clock64() - t0 < 2000000) {}
+        }
+    } else if constexpr (MODE == kFewAdapters) {
+        // ------------------------------------------------------------ the addition: a column a lane, every fourth row a warp
+        const int w = warp - 2 - kEpiWarps;
+        constexpr int kEach = kFewRows / kAuxWarps;
+        float* addition = reinterpret_cast<float*>(base_ptr + kLowAt);
+        const __nv_bfloat16* up = static_cast<const __nv_bfloat16*>(p.up);
+        int ids[kEach];
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int row = w + kAuxWarps * i;
+            ids[i] = row < p.M ? __ldg(p.row_adapter + row) : -1;
+        }
+        uint32_t ph = 0;
+        bool ok = true, waited = false;
+        for (long long t = tile0; ok && walk.find(t, BN, tile); t += tile_step, ph ^= 1) {
+            for (int c = 0; ok && c < BN; c += 32) {
+                const int col = tile.col0 + c + lane;
+                float acc[kEach];
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) acc[i] = 0.0f;
+                for (int r = 0; r < p.rank; r += 8) {
+                    uint4 u[kEach];
+#pragma unroll
+                    for (int i = 0; i < kEach; ++i) {
+                        u[i] = make_uint4(0, 0, 0, 0);
+                        if ((unsigned)ids[i] < (unsigned)p.n_adapters && col < p.N)
+                            u[i] = __ldg(reinterpret_cast<const uint4*>(up + ((int64_t)ids[i] * p.N + col) * p.rank + r));
+                    }
+                    if (!waited) { pdl_wait(); waited = true; }
+                    // a row without an adapter has zeros in `low`, one beyond M borrows the last one's; no branches between the loads
+                    float4 x[kEach], y[kEach];
+#pragma unroll
+                    for (int i = 0; i < kEach; ++i) {
+                        const float4* low = reinterpret_cast<const float4*>(p.low + (int64_t)min(w + kAuxWarps * i, p.M - 1) * p.rank + r);
+                        x[i] = low[0];
+                        y[i] = low[1];
+                    }
+#pragma unroll
+                    for (int i = 0; i < kEach; ++i) {
+                        auto part = [](float a, float b, uint32_t v, float s) {
+                            return fmaf(b, __uint_as_float(v & 0xffff0000u), fmaf(a, __uint_as_float(v << 16), s));
+                        };
+                        acc[i] = part(y[i].z, y[i].w, u[i].w, part(y[i].x, y[i].y, u[i].z, part(x[i].z, x[i].w, u[i].y, part(x[i].x, x[i].y, u[i].x, acc[i]))));
+                    }
+                }
+                if (c == 0) ok = __all_sync(0xffffffffu, mbar_wait(lowfree_bar, ph ^ 1, abort_flag));
+                if (!ok) break;
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) addition[(c + lane) * kFewPitch + w + kAuxWarps * i] = acc[i];
+            }
+            __syncwarp();
+            if (ok && lane == 0) mbar_arrive(low_bar);
         }
     } else if constexpr (MODE == kAdapters) {
         // ------------------------------------------------------------ `low` of the tile's rows as an operand, a row per thread
@@ -841,7 +926,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
 template <int BN, int CTAS, bool FP8, int MODE, bool F32>
 cudaError_t rows_launch_t(const RowsArgs& g, int sm_count, int* d_error, cudaStream_t stream) {
     alignas(64) CUtensorMap ma, mw, mu, mo;
-    if (!rows_map(&ma, g.a, g.a_rows, g.K, g.lda, FP8, MODE == kGathered ? 1 : kBM) ||
+    if (!rows_map(&ma, g.a, g.a_rows, g.K, g.lda, FP8, rows_gathers(MODE) ? 1 : RCfg<BN, CTAS, MODE, F32>::kABytes / kRowBytes) ||
         !rows_map(&mw, g.w, (int64_t)g.n_groups * g.N, g.K, g.K, FP8, BN / CTAS))
         return cudaErrorInvalidValue;
     mu = mw;
@@ -854,7 +939,7 @@ cudaError_t rows_launch_t(const RowsArgs& g, int sm_count, int* d_error, cudaStr
     p.out_vec = !(reinterpret_cast<uintptr_t>(g.out) & 15) && !((g.ldo * eb) & 15);
     mo = mw;
     if (p.out_vec && !rows_out_map(&mo, g.out, g.M, g.N, g.ldo, F32, F32 || RCfg<BN, CTAS, MODE, F32>::kHalfCols >= 64 ? 128 : 64)) return cudaErrorInvalidValue;
-    p.row_adapter = g.row_adapter; p.low = g.low; p.rank = g.rank; p.n_adapters = g.n_adapters;
+    p.row_adapter = g.row_adapter; p.low = g.low; p.up = g.up; p.rank = g.rank; p.n_adapters = g.n_adapters;
     // at most this many tiles: a group's last one may be short
     const int64_t n_tiles = (g.N + BN - 1) / BN;
     const int64_t tiles = ((int64_t)(g.M + kBM * CTAS - 1) / (kBM * CTAS) + std::min(g.n_groups - 1, g.M)) * n_tiles;
@@ -872,15 +957,18 @@ cudaError_t rows_set() {
 // thread at most, so its widest tile has 128 columns.
 template <bool FP8, int MODE>
 cudaError_t rows_pick(const RowsArgs& g, RowsTileShape t, int sm_count, int* err, cudaStream_t st) {
+    if constexpr (rows_few(MODE)) t.ctas = 1;  // (a pair's tile is 256 columns wide, 128 where the result is stored in 32 bits)
     if (g.out_mode != kOutBf16) {
-        if (t.ctas == 2) return rows_launch_t<128, 2, FP8, MODE, true>(g, sm_count, err, st);
+        if constexpr (!rows_few(MODE))
+            if (t.ctas == 2) return rows_launch_t<128, 2, FP8, MODE, true>(g, sm_count, err, st);
         switch (t.bn) {
             case 32: return rows_launch_t<32, 1, FP8, MODE, true>(g, sm_count, err, st);
             case 64: return rows_launch_t<64, 1, FP8, MODE, true>(g, sm_count, err, st);
             default: return rows_launch_t<128, 1, FP8, MODE, true>(g, sm_count, err, st);
         }
     }
-    if (t.ctas == 2) return rows_launch_t<256, 2, FP8, MODE, false>(g, sm_count, err, st);
+    if constexpr (!rows_few(MODE))
+        if (t.ctas == 2) return rows_launch_t<256, 2, FP8, MODE, false>(g, sm_count, err, st);
     switch (t.bn) {
         case 32: return rows_launch_t<32, 1, FP8, MODE, false>(g, sm_count, err, st);
         case 64: return rows_launch_t<64, 1, FP8, MODE, false>(g, sm_count, err, st);
@@ -891,9 +979,14 @@ cudaError_t rows_pick(const RowsArgs& g, RowsTileShape t, int sm_count, int* err
 
 template <bool FP8, int MODE>
 cudaError_t rows_set_all() {
-    const cudaError_t e[9] = {rows_set<32, 1, FP8, MODE, true>(),  rows_set<64, 1, FP8, MODE, true>(),   rows_set<128, 1, FP8, MODE, true>(),
-                              rows_set<128, 2, FP8, MODE, true>(), rows_set<32, 1, FP8, MODE, false>(),  rows_set<64, 1, FP8, MODE, false>(),
-                              rows_set<128, 1, FP8, MODE, false>(), rows_set<256, 1, FP8, MODE, false>(), rows_set<256, 2, FP8, MODE, false>()};
+    const cudaError_t e[7] = {rows_set<32, 1, FP8, MODE, true>(),  rows_set<64, 1, FP8, MODE, true>(),   rows_set<128, 1, FP8, MODE, true>(),
+                              rows_set<32, 1, FP8, MODE, false>(), rows_set<64, 1, FP8, MODE, false>(), rows_set<128, 1, FP8, MODE, false>(),
+                              rows_set<256, 1, FP8, MODE, false>()};
+    if constexpr (!rows_few(MODE)) {
+        const cudaError_t pair[2] = {rows_set<128, 2, FP8, MODE, true>(), rows_set<256, 2, FP8, MODE, false>()};
+        for (cudaError_t x : pair)
+            if (x != cudaSuccess) return x;
+    }
     for (cudaError_t x : e)
         if (x != cudaSuccess) return x;
     return cudaSuccess;

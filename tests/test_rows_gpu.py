@@ -466,6 +466,16 @@ def test_adapters_large(ctx, M, N, K, rank, n):
     adapter_case(ctx, who, n, rank, N, K, mode=1)
 
 
+@pytest.mark.parametrize("M", [1, 7, 32, 33])
+@pytest.mark.parametrize("rank,N,K,mode", [(8, 1030, 640, 0), (24, 4096, 1024, 1), (128, 30, 72, 2), (16, 45000, 64, 0), (64, 20000, 64, 1), (40, 127, 1000, 0),
+                                           (16, 100000, 32, 0)])
+def test_adapters_of_a_few_streams(ctx, M, rank, N, K, mode):
+    """Up to 32 rows take another path; more than one tile per CTA in the wide ones."""
+    who = [(7 * i) % 12 - 1 for i in range(M)]
+    adapter_case(ctx, who, 11, rank, N, K, mode=mode, act=SILU, alpha=0.5)
+    adapter_case(ctx, who, 11, rank, N, K, mode=mode, poison=6, pad_o=3, shift=1)
+
+
 @pytest.mark.parametrize("mode", [0, 1])
 def test_a_broken_adapter_stays_with_its_rows(ctx, mode):
     adapter_case(ctx, runs((0, 50), (1, 20), (2, 30), (-1, 28)) + [0, 1, 2] * 10, 3, 16, 256, 128, mode=mode, poison=1)

@@ -937,8 +937,8 @@ cudaError_t rows_launch_t(const RowsArgs& g, int sm_count, int* d_error, cudaStr
     p.a_rows = g.a_rows; p.ldo = g.ldo; p.M = g.M; p.N = g.N; p.K = g.K; p.n_groups = g.n_groups; p.act = g.act; p.out_mode = g.out_mode;
     p.alpha = g.alpha;
     p.out_vec = !(reinterpret_cast<uintptr_t>(g.out) & 15) && !((g.ldo * eb) & 15);
-    mo = mw;
-    if (p.out_vec && !rows_out_map(&mo, g.out, g.M, g.N, g.ldo, F32, F32 || RCfg<BN, CTAS, MODE, F32>::kHalfCols >= 64 ? 128 : 64)) return cudaErrorInvalidValue;
+    mo = mw;  // stores by TMA want 32 rows of a group
+    if (p.out_vec && g.M >= 32 && !rows_out_map(&mo, g.out, g.M, g.N, g.ldo, F32, F32 || RCfg<BN, CTAS, MODE, F32>::kHalfCols >= 64 ? 128 : 64)) return cudaErrorInvalidValue;
     p.row_adapter = g.row_adapter; p.low = g.low; p.up = g.up; p.rank = g.rank; p.n_adapters = g.n_adapters;
     // at most this many tiles: a group's last one may be short
     const int64_t n_tiles = (g.N + BN - 1) / BN;

@@ -2,12 +2,12 @@
 //
 // Bound by reading the rows once (2 K bytes each against K * rank products).  Three kernels:
 //   - many rows: 128 rows a CTA on tcgen05, rows and adapters through a TMA ring; a pass over K for every few adapters among the
-//     rows, each with the lanes of the other rows disabled (nothing of one adapter reaches another's rows).
+//     rows, whose matrices lie side by side as one operand; each row takes its own adapter's columns of the accumulator (selected,
+//     not masked by zeros: nothing of one adapter reaches another's rows).
 //   - very few rows: a warp per row and eight columns, K over the lanes.
 //   - between them: 16 rows a block on mma.sync m16n8k16 with operands straight from global memory, K over the warps, the columns over
 //     blocks; a row takes its adapter's product (selected, not masked by zeros).
-// Where nearly every row has its own adapter (live streams), such passes would run one after the other; there a row is a chain of
-// dot products over the lanes of a warp.
+//     Where more than two adapters meet in the 16 rows, a row is a chain of dot products over the lanes of a warp instead.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -199,43 +199,46 @@ __global__ void __launch_bounds__(kDownWarps * 32, 1) adapter_down_kernel(const 
 }
 
 // ---------------------------------------------------------------------------------------------- many rows: tcgen05
-constexpr int kTcRows = 128, kTcMaxStages = 8, kTcThreads = 192;
-constexpr int kTcMaxPasses = 6;  // passes above which the rows are taken one by one
-
+constexpr int kTcRows = 128, kTcThreads = 192;
 constexpr int tc_cols(int rank) { return rank <= 16 ? 16 : (rank <= 32 ? 32 : (rank <= 64 ? 64 : 128)); }
 template <int RN>
 struct DownTc {
-    static constexpr int kAtOnce = RN <= 32 ? 4 : (RN == 64 ? 2 : 1);  // adapters of a pass
+    static constexpr int kAtOnce = RN == 16 ? 4 : (RN == 128 ? 1 : 2);  // adapters of a pass
+    static constexpr int kCols = kAtOnce * RN;                          // their columns of the accumulator
+    static constexpr uint32_t kTmemCols = 2 * kCols;  // two accumulators by turns, for a pass over K each
     static constexpr int kABytes = kTcRows * 128, kOneBytes = RN * 128, kBBytes = kAtOnce * kOneBytes, kStageBytes = kABytes + kBBytes;
-    static constexpr uint32_t kTmemCols = RN < 32 ? 32 : RN;
-    static constexpr int smem_bytes(int stages) { return stages * kStageBytes + 256 + 1024; }
-    // all of an SM's shared memory where every CTA has one to itself, else half of it
-    static constexpr int stages(bool alone) { return std::min((alone ? 224 : 110) * 1024 / kStageBytes, kTcMaxStages); }
+    static constexpr int kStages = std::min(224 * 1024 / kStageBytes, 8);
+    static constexpr int kSmemBytes = kStages * kStageBytes + 256 + 1024;
 };
 
-// Warp 0 loads, warp 1 issues the MMAs, warps 2 to 5 read the results, a row per thread.
+// One CTA per SM, tiles of 128 rows by turns.  Warp 0 loads, warp 1 issues the MMAs, warps 2 to 5 read the results, a row per thread.
 template <int RN>
 __global__ void __launch_bounds__(kTcThreads) adapter_down_tc_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_d,
-                                                                     const AdapterDownArgs p, int stages, int* __restrict__ error) {
+                                                                     const AdapterDownArgs p, int* __restrict__ error) {
     using namespace ptx;
     using C = DownTc<RN>;
+    constexpr int S = C::kStages;
     extern __shared__ unsigned char smem_dyn[];
     const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
     unsigned char* base_ptr = smem_dyn + (base - smem_u32(smem_dyn));
-    const uint32_t a_base = base, b_base = base + stages * C::kABytes, bar_base = base + stages * C::kStageBytes;
+    const uint32_t a_base = base, b_base = base + S * C::kABytes, bar_base = base + S * C::kStageBytes;
     auto full_bar = [&](int s) { return bar_base + 8u * s; };
-    auto empty_bar = [&](int s) { return bar_base + 8u * (kTcMaxStages + s); };
-    const uint32_t done_bar = bar_base + 8u * (2 * kTcMaxStages);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + stages * C::kStageBytes + 8 * (2 * kTcMaxStages + 1));
+    auto empty_bar = [&](int s) { return bar_base + 8u * (S + s); };
+    auto done_bar = [&](int a) { return bar_base + 8u * (2 * S + a); };
+    auto free_bar = [&](int a) { return bar_base + 8u * (2 * S + 2 + a); };
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + S * C::kStageBytes + 8 * (2 * S + 4));
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = warp_index(), lane = threadIdx.x & 31;
-    const int row0 = blockIdx.x * kTcRows, k_tiles = (p.K + 63) / 64;
+    const int k_tiles = (p.K + 63) / 64, tiles = (p.M + kTcRows - 1) / kTcRows;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < stages; ++s) {
+        for (int s = 0; s < S; ++s) {
             mbar_init(full_bar(s), 1);
             mbar_init(empty_bar(s), 1);
         }
-        mbar_init(done_bar, 1);
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(done_bar(a), 1);
+            mbar_init(free_bar(a), 4);
+        }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -249,130 +252,124 @@ __global__ void __launch_bounds__(kTcThreads) adapter_down_tc_kernel(const __gri
     const uint32_t tmem = *tmem_slot;
     pdl_wait();
     pdl_trigger();
-    // every warp counts the adapters for itself
-    int found = 0;
-    {
-        AdapterIds<kTcRows> w;
-        w.load(p.row_adapter, p.n_adapters, row0, p.M, lane);
-        while (found <= kTcMaxPasses * C::kAtOnce && w.next() >= 0) ++found;
-    }
-    const bool dots = found > kTcMaxPasses * C::kAtOnce;
+    AdapterIds<kTcRows> ids;  // of a tile; every warp goes through them by itself
 
-    if (warp == 0 && !dots) {
-        AdapterIds<kTcRows> w;
-        w.load(p.row_adapter, p.n_adapters, row0, p.M, lane);
+    if (warp == 0) {
         int stage = 0;
         uint32_t ph = 0;
         bool ok = true;
-        for (int left = found; ok && left > 0; left -= C::kAtOnce) {
-            int id[C::kAtOnce];
+        for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+            for (ids.load(p.row_adapter, p.n_adapters, t * kTcRows, p.M, lane); ok;) {
+                int id[C::kAtOnce], n = 0;
 #pragma unroll
-            for (int e = 0; e < C::kAtOnce; ++e) id[e] = w.next();
-            bool failed = false;
-            if (elect_one()) {
-                int s = stage;
-                uint32_t sp = ph;
-                for (int kt = 0; kt < k_tiles; ++kt) {
-                    if (!mbar_wait(empty_bar(s), sp ^ 1, abort_flag)) { failed = true; break; }
-                    mbar_expect_tx(full_bar(s), C::kABytes + min(left, C::kAtOnce) * C::kOneBytes);
-                    tma_load_2d(a_base + s * C::kABytes, &tma_a, full_bar(s), kt * 64, row0);
-#pragma unroll
-                    for (int e = 0; e < C::kAtOnce; ++e)
-                        if (e < left) tma_load_2d(b_base + s * C::kBBytes + e * C::kOneBytes, &tma_d, full_bar(s), kt * 64, id[e] * p.rank);
-                    if (++s == stages) { s = 0; sp ^= 1; }
+                for (int e = 0; e < C::kAtOnce; ++e) {
+                    id[e] = ids.next();
+                    n += id[e] >= 0;
                 }
+                if (n == 0) break;
+                bool failed = false;
+                if (elect_one()) {
+                    int s = stage;
+                    uint32_t sp = ph;
+                    for (int kt = 0; kt < k_tiles; ++kt) {
+                        if (!mbar_wait(empty_bar(s), sp ^ 1, abort_flag)) { failed = true; break; }
+                        mbar_expect_tx(full_bar(s), C::kABytes + n * C::kOneBytes);
+                        tma_load_2d(a_base + s * C::kABytes, &tma_a, full_bar(s), kt * 64, t * kTcRows);
+#pragma unroll
+                        for (int e = 0; e < C::kAtOnce; ++e)
+                            if (e < n) tma_load_2d(b_base + s * C::kBBytes + e * C::kOneBytes, &tma_d, full_bar(s), kt * 64, id[e] * p.rank);
+                        if (++s == S) { s = 0; sp ^= 1; }
+                    }
+                }
+                ok = !__any_sync(0xffffffffu, failed);
+                stage += k_tiles;
+                ph ^= (uint32_t)(stage / S) & 1u;
+                stage %= S;
             }
-            ok = !__any_sync(0xffffffffu, failed);
-            stage += k_tiles;
-            ph ^= (uint32_t)(stage / stages) & 1u;
-            stage %= stages;
         }
         if (!ok) {
             const long long t0 = clock64();
             while (clock64() - t0 < 2000000) {}
         }
-    } else if (warp == 1 && !dots) {
-        // fp32 accumulate, bf16 operands, both K-major, M = 128, N = RN
-        constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(RN >> 3) << 17) | ((uint32_t)(kTcRows >> 4) << 24);
-        AdapterIds<kTcRows> w;
-        w.load(p.row_adapter, p.n_adapters, row0, p.M, lane);
-        int mine[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) mine[q] = row0 + 32 * q + lane < p.M ? __ldg(p.row_adapter + row0 + 32 * q + lane) : -1;
+    } else if (warp == 1) {
         int stage = 0;
         uint32_t ph = 0;
         bool ok = true;
-        for (int left = found; ok && left > 0; left -= C::kAtOnce) {
-            uint32_t off[C::kAtOnce][4];
+        int pass = 0;
+        for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+            for (ids.load(p.row_adapter, p.n_adapters, t * kTcRows, p.M, lane); ok; ++pass) {
+                int n = 0;
 #pragma unroll
-            for (int e = 0; e < C::kAtOnce; ++e) {
-                const int id = w.next();
-#pragma unroll
-                for (int q = 0; q < 4; ++q) off[e][q] = ~__ballot_sync(0xffffffffu, mine[q] == id);
-            }
-            bool failed = false;
-            if (elect_one()) {
-                int s = stage;
-                uint32_t sp = ph;
-                for (int kt = 0; kt < k_tiles; ++kt) {
-                    if (!mbar_wait(full_bar(s), sp, abort_flag)) { failed = true; break; }
+                for (int e = 0; e < C::kAtOnce; ++e) n += ids.next() >= 0;
+                if (n == 0) break;
+                // fp32 accumulate, bf16 operands, both K-major, M = 128, N = the columns of this pass's adapters
+                const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n * RN >> 3) << 17) | ((uint32_t)(kTcRows >> 4) << 24);
+                const int acc = pass & 1;
+                bool failed = false;
+                if (elect_one()) {
+                    int s = stage;
+                    uint32_t sp = ph;
+                    if (!mbar_wait(free_bar(acc), ((pass >> 1) & 1) ^ 1, abort_flag)) failed = true;
                     tc_fence_after();
-                    const uint64_t adesc = make_smem_desc(a_base + s * C::kABytes), bdesc = make_smem_desc(b_base + s * C::kBBytes);
+                    for (int kt = 0; kt < k_tiles && !failed; ++kt) {
+                        if (!mbar_wait(full_bar(s), sp, abort_flag)) { failed = true; break; }
+                        tc_fence_after();
+                        const uint64_t adesc = make_smem_desc(a_base + s * C::kABytes), bdesc = make_smem_desc(b_base + s * C::kBBytes);
 #pragma unroll
-                    for (int e = 0; e < C::kAtOnce; ++e) {
-                        if (e >= left) break;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            tc_mma_lanes(tmem, adesc + 2 * i, bdesc + e * (C::kOneBytes / 16) + 2 * i, idesc, off[e], (kt | i) ? 1u : 0u);
+                        for (int i = 0; i < 4; ++i) tc_mma<false>(tmem + acc * C::kCols, adesc + 2 * i, bdesc + 2 * i, idesc, (kt | i) ? 1u : 0u);
+                        tc_commit(empty_bar(s));
+                        if (++s == S) { s = 0; sp ^= 1; }
                     }
-                    tc_commit(empty_bar(s));
-                    if (++s == stages) { s = 0; sp ^= 1; }
+                    if (!failed) tc_commit(done_bar(acc));
                 }
-            }
-            ok = !__any_sync(0xffffffffu, failed);
-            stage += k_tiles;
-            ph ^= (uint32_t)(stage / stages) & 1u;
-            stage %= stages;
-        }
-        if (ok && elect_one()) tc_commit(done_bar);
-        __syncwarp();
-    } else if (!dots) {
-        const bool ok = __all_sync(0xffffffffu, mbar_wait(done_bar, 0, abort_flag));
-        tc_fence_after();
-        const int quad = warp & 3, row = row0 + 32 * quad + lane;
-        const int id = row < p.M ? __ldg(p.row_adapter + row) : -1;
-        const bool has = (unsigned)id < (unsigned)p.n_adapters;
-        const float f = has ? (p.scale ? __ldg(p.scale + id) : 1.0f) : 0.0f;
-#pragma unroll
-        for (int c = 0; c < RN; c += 16) {
-            if (!ok || c >= p.rank) break;
-            uint32_t v[16];
-            tmem_ld16(tmem + ((uint32_t)(quad * 32) << 16) + c, v);
-            tmem_wait_ld();
-            if (row >= p.M) continue;
-            float4* out = reinterpret_cast<float4*>(p.low + (int64_t)row * p.rank + c);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                // a row without an adapter leaves the accumulator as it was found: not a number to multiply by zero
-                if (c + 4 * j < p.rank)
-                    out[j] = has ? make_float4(f * __uint_as_float(v[4 * j]), f * __uint_as_float(v[4 * j + 1]), f * __uint_as_float(v[4 * j + 2]),
-                                               f * __uint_as_float(v[4 * j + 3]))
-                                 : make_float4(0.f, 0.f, 0.f, 0.f);
+                ok = !__any_sync(0xffffffffu, failed);
+                stage += k_tiles;
+                ph ^= (uint32_t)(stage / S) & 1u;
+                stage %= S;
             }
         }
     } else {
-        const __nv_bfloat16* a = static_cast<const __nv_bfloat16*>(p.a);
-        const __nv_bfloat16* down = static_cast<const __nv_bfloat16*>(p.down);
-        for (int r = warp; r < kTcRows && row0 + r < p.M; r += kTcThreads / 32) {
-            const int row = row0 + r, id = __ldg(p.row_adapter + row);
+        const int quad = warp & 3;
+        bool ok = true;
+        int pass = 0;
+        for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+            const int row = t * kTcRows + 32 * quad + lane;
+            const int id = row < p.M ? __ldg(p.row_adapter + row) : -1;
             const bool has = (unsigned)id < (unsigned)p.n_adapters;
-            for (int c = 0; c < p.rank; c += 8) {
-                float v = 0.0f;
-                if (has) {
-                    v = row_dots<2>(a + (int64_t)row * p.lda, down + ((int64_t)id * p.rank + c) * p.K, p.K, 8, lane);
-                    if (p.scale) v *= __ldg(p.scale + id);
+            const float f = has ? (p.scale ? __ldg(p.scale + id) : 1.0f) : 0.0f;
+            float4* out = reinterpret_cast<float4*>(p.low + (int64_t)row * p.rank);
+            if (row < p.M && !has)
+                for (int c = 0; c < p.rank; c += 4) out[c / 4] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (ids.load(p.row_adapter, p.n_adapters, t * kTcRows, p.M, lane); ok; ++pass) {
+                int n = 0, mine = -1;  // place of this row's adapter in the pass
+#pragma unroll
+                for (int e = 0; e < C::kAtOnce; ++e) {
+                    const int next = ids.next();
+                    n += next >= 0;
+                    if (has && next == id) mine = e;
                 }
-                if (lane < 8) p.low[(int64_t)row * p.rank + c + lane] = v;
+                if (n == 0) break;
+                const int acc = pass & 1;
+                ok = __all_sync(0xffffffffu, mbar_wait(done_bar(acc), (pass >> 1) & 1, abort_flag));
+                if (!ok) break;
+                tc_fence_after();
+                for (int e = 0; e < n; ++e) {
+                    if (!__any_sync(0xffffffffu, mine == e)) continue;
+                    for (int c = 0; c < p.rank; c += 16) {
+                        uint32_t v[16];
+                        tmem_ld16(tmem + ((uint32_t)(quad * 32) << 16) + acc * C::kCols + e * RN + c, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (mine == e && c + 4 * i < p.rank)
+                                out[c / 4 + i] = make_float4(f * __uint_as_float(v[4 * i]), f * __uint_as_float(v[4 * i + 1]),
+                                                             f * __uint_as_float(v[4 * i + 2]), f * __uint_as_float(v[4 * i + 3]));
+                        __syncwarp();
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(free_bar(acc));
             }
         }
     }
@@ -390,8 +387,8 @@ cudaError_t down_tc_t(const AdapterDownArgs& g, int sm_count, int* d_error, cuda
     alignas(64) CUtensorMap ma, md;
     if (!rows_map(&ma, g.a, g.M, g.K, g.lda, false, kTcRows) || !rows_map(&md, g.down, (int64_t)g.n_adapters * g.rank, g.K, g.K, false, RN))
         return cudaErrorInvalidValue;
-    const int blocks = (g.M + kTcRows - 1) / kTcRows, stages = DownTc<RN>::stages(blocks <= sm_count);
-    return launch_pdl(adapter_down_tc_kernel<RN>, dim3(blocks), kTcThreads, DownTc<RN>::smem_bytes(stages), stream, 1, ma, md, g, stages, d_error);
+    const int blocks = std::min((g.M + kTcRows - 1) / kTcRows, sm_count);
+    return launch_pdl(adapter_down_tc_kernel<RN>, dim3(blocks), kTcThreads, DownTc<RN>::kSmemBytes, stream, 1, ma, md, g, d_error);
 }
 
 template <int NT>
@@ -407,10 +404,10 @@ cudaError_t adapter_down_configure() {
     auto set = [&](auto kernel, int bytes) {
         if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     };
-    set(adapter_down_tc_kernel<16>, DownTc<16>::smem_bytes(DownTc<16>::stages(true)));
-    set(adapter_down_tc_kernel<32>, DownTc<32>::smem_bytes(DownTc<32>::stages(true)));
-    set(adapter_down_tc_kernel<64>, DownTc<64>::smem_bytes(DownTc<64>::stages(true)));
-    set(adapter_down_tc_kernel<128>, DownTc<128>::smem_bytes(DownTc<128>::stages(true)));
+    set(adapter_down_tc_kernel<16>, DownTc<16>::kSmemBytes);
+    set(adapter_down_tc_kernel<32>, DownTc<32>::kSmemBytes);
+    set(adapter_down_tc_kernel<64>, DownTc<64>::kSmemBytes);
+    set(adapter_down_tc_kernel<128>, DownTc<128>::kSmemBytes);
     return e;
 }
 

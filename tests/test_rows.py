@@ -119,7 +119,7 @@ int main() {
                 for (int f32 = 0; f32 < 2; ++f32)
                     for (int sms : {20, 132, 148}) {
                         const sb::RowsTileShape t = sb::rows_tile(M, N, G, f32 != 0, sms); const int bn = t.bn;
-                        if (t.ctas == 2 ? bn != (f32 ? 128 : 256) : !(bn == 32 || bn == 64 || bn == 128 || (bn == 256 && !f32))) { std::printf("bad %ld %d %d %d\n", M, N, G, bn); return 1; }
+                        if (t.ctas == 2 ? (f32 || bn != 256) : !(bn == 32 || bn == 64 || bn == 128 || (bn == 256 && !f32))) { std::printf("bad %ld %d %d %d\n", M, N, G, bn); return 1; }
                         ++n;
                     }
     std::printf("%ld\n", n);

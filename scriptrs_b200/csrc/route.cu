@@ -160,7 +160,7 @@ __device__ __forceinline__ void route_row(const RouteArgs& p, int row, bool live
         const int j = l + i * LANES;
         if (j >= p.top_k) break;
         p.experts[out + j] = who[i];
-        p.weights[out + j] = who[i] >= 0 ? mine[i] / total : 0.0f;
+        p.weights[out + j] = who[i] >= 0 ? __fdividef(mine[i], total) : 0.0f;  // 1 <= total <= 1024
         chosen[j] = (int16_t)who[i];
     }
 }

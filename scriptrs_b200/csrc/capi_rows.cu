@@ -131,7 +131,7 @@ int32_t sb_adapter_gemm(sb_ctx* c, const void* d_a, int64_t lda, const void* d_w
                         int64_t M, int64_t N, int64_t K, int32_t act, int32_t out_mode, float alpha, void* d_work, int64_t work_bytes) {
     int32_t st = check_product(d_a, lda, d_w, d_bias, d_out, ldo, M, N, K, 1, false, act, out_mode);
     if (st != SB_OK) return st;
-    if (n_adapters <= 0 || n_adapters > kLimit / N || rank <= 0 || rank > kMaxRank || rank % 8)
+    if (n_adapters <= 0 || n_adapters > kLimit / std::max(N, kMaxRank) || rank <= 0 || rank > kMaxRank || rank % 8)
         return fail(SB_INVALID_ARGUMENT, "adapters: at least one, rank a multiple of 8 up to 128");
     if (M > 0 && (!d_down || !d_up || !d_row_adapter)) return fail(SB_INVALID_ARGUMENT, "null argument");
     if (off_boundary(d_down, 16) || off_boundary(d_up, 16) || off_boundary(d_work, 16) || off_boundary(d_scale, 4) || off_boundary(d_row_adapter, 4))

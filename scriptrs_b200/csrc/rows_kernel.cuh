@@ -5,7 +5,7 @@
 // One CTA per SM, warp-specialised like the shared product of gemm.cu: a TMA producer, an MMA issuer (128 rows x BN columns per
 // CTA in tensor memory, two accumulators), eight epilogue warps.  What differs:
 //   - The tiles are found on the device.  A tile belongs to one group: 128 consecutive rows of it per CTA (the last ones of a
-//     group may be missing) times BN columns.  Every warp walks the offsets 32 groups at a time with a prefix sum over its
+//     group may be missing) times BN columns.  Every warp walks the offsets 128 groups at a time with a prefix sum over its
 //     lanes, so no table of groups is kept and the host never learns the sizes.
 //   - Rows picked by an index arrive by TMA gathers of four rows each, issued by four warps (32 rows each) from one elected
 //     lane (from every lane by turns a gather takes ten times as long); a tile with few rows fetches only those.
@@ -193,29 +193,36 @@ struct RowsTile {
     int group, row0, row1, col0;
 };
 
-// Finds tile t.  All lanes of a warp call it together, with ascending t.
+// Finds tile t.  All lanes of a warp call it together, with ascending t.  A lane holds kEach neighbouring groups.
 template <int ROWS>
 struct TileWalk {
+    static constexpr int kEach = 4;
     const int32_t* offsets;
     int M, n_groups, n_tiles, lane;
-    int first_group;      // of the 32 groups that the lanes hold
+    int first_group;      // of the groups that the lanes hold
     long long first_tile; // tiles of the groups before them
-    int lo, hi, upto;     // this lane's group: rows, tiles of the groups up to and including it
-    int total;            // tiles of the 32 groups
+    int at[kEach + 1];    // this lane's groups: rows [at[j], at[j + 1]), ascending
+    int own, upto;        // tiles of this lane's groups, of the lanes' up to and including this one
+    int total;            // tiles of the groups that the lanes hold
 
     __device__ __forceinline__ TileWalk(const int32_t* off, int m, int groups, int nt, int ln)
         : offsets(off), M(m), n_groups(groups), n_tiles(nt), lane(ln), first_group(0), first_tile(0) {
         load();
     }
+    __device__ __forceinline__ int tiles_of(int j) const { return (at[j + 1] - at[j] + ROWS - 1) / ROWS * n_tiles; }
     __device__ __forceinline__ void load() {
-        const int g = first_group + lane;
-        lo = hi = 0;
-        if (g < n_groups) {
-            // whatever the offsets hold, rows stay inside [0, M)
-            lo = offsets ? min(max(__ldg(offsets + g), 0), M) : 0;
-            hi = offsets ? max(min(__ldg(offsets + g + 1), M), lo) : M;
+        const int g0 = first_group + kEach * lane;
+        // whatever the offsets hold, rows stay inside [0, M), and a group behind the last one has none
+#pragma unroll
+        for (int j = 0; j <= kEach; ++j)
+            at[j] = offsets ? min(max(__ldg(offsets + min(g0 + j, n_groups)), 0), M) : (g0 + j > 0 ? M : 0);
+        own = 0;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            at[j + 1] = max(at[j + 1], at[j]);
+            own += tiles_of(j);
         }
-        upto = (hi - lo + ROWS - 1) / ROWS * n_tiles;
+        upto = own;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, upto, d);
@@ -225,20 +232,27 @@ struct TileWalk {
     }
     __device__ __forceinline__ bool find(long long t, int bn, RowsTile& out) {
         while (t >= first_tile + total) {
-            if (first_group + 32 >= n_groups) return false;
+            if (first_group + 32 * kEach >= n_groups) return false;
             first_tile += total;
-            first_group += 32;
+            first_group += 32 * kEach;
             load();
         }
         const int r = (int)(t - first_tile);
         const int src = __ffs(__ballot_sync(0xffffffffu, upto > r)) - 1;
-        const int before = src ? __shfl_sync(0xffffffffu, upto, src ? src - 1 : 0) : 0;
-        const int glo = __shfl_sync(0xffffffffu, lo, src), ghi = __shfl_sync(0xffffffffu, hi, src);
-        const int mt = (r - before) / n_tiles, nt = (r - before) % n_tiles;
-        out.group = first_group + src;
+        int mine = r - (upto - own), j = 0, glo = at[0], ghi = at[1], skip = 0, before = 0;
+#pragma unroll
+        for (int i = 1; i < kEach; ++i) {
+            before += tiles_of(i - 1);
+            if (mine >= before) { j = i; glo = at[i]; ghi = at[i + 1]; skip = before; }
+        }
+        const int rest = __shfl_sync(0xffffffffu, mine - skip, src);
+        glo = __shfl_sync(0xffffffffu, glo, src);
+        ghi = __shfl_sync(0xffffffffu, ghi, src);
+        out.group = first_group + kEach * src + __shfl_sync(0xffffffffu, j, src);
+        const int mt = rest / n_tiles;
         out.row0 = glo + mt * ROWS;
         out.row1 = min(ghi, out.row0 + ROWS);
-        out.col0 = nt * bn;
+        out.col0 = (rest - mt * n_tiles) * bn;
         return true;
     }
 };

@@ -210,7 +210,8 @@ def grouped_case(ctx, sizes, N, K, *, gather=0, fp8=False, act=0, mode=0, bias=T
     return out[:M, :N].clone()
 
 
-RAGGED = [[1], [128], [129], [0, 5, 0, 0, 130, 1], [3] * 40, [0] * 33 + [7] + [0] * 40, [300, 0, 1, 255, 256, 257], [2, 1, 0, 4, 1, 1, 3, 0]]
+RAGGED = [[1], [128], [129], [0, 5, 0, 0, 130, 1], [3] * 40, [0] * 33 + [7] + [0] * 40, [300, 0, 1, 255, 256, 257], [2, 1, 0, 4, 1, 1, 3, 0],
+          [0] * 130 + [140, 0, 3] + [1] * 127 + [0] * 500 + [60], [1, 0, 2] * 100]
 
 
 @pytest.mark.parametrize("sizes", RAGGED, ids=lambda s: "_".join(map(str, s[:6])))

@@ -21,6 +21,7 @@ constexpr int kRouteRows = 512;     // most rows of a block
 constexpr int kRouteOneBlock = 128; // rows up to which one block does everything
 constexpr int kRouteSums = 256;     // blocks up to which each sums the counts of those before it by itself
 constexpr int kMaxExperts = 1024, kMaxTopK = 16;
+constexpr int kCombineFew = 148 * 8;  // pieces of 32 lanes up to which each gets a warp: eight warps an SM
 
 // Rows per block: as many blocks as there are SMs to fill with a pass of 64 rows or more.
 int route_block_rows(int64_t rows) {
@@ -365,93 +366,151 @@ cudaError_t route_form(int n_experts, Fn fn) {
 }
 size_t route_part_bytes(int n_experts) { return (size_t)kRouteWarps * n_experts * sizeof(uint16_t); }
 
-// out[row] (+)= alpha sum_j weights[row][j] y[slots[row][j]], in 32 bits in the order of j, rounded once.  A thread takes eight
-// columns where rows lie on 16-byte boundaries, else one; four results' pieces are asked for at once.
-template <typename Y, int PER>
-__global__ void __launch_bounds__(256) combine_kernel(const CombineArgs p) {
+// PER neighbouring values, at an address on a boundary of all of them (at most 16 bytes).
+template <typename T, int PER>
+struct Piece {
+    static constexpr int kBytes = PER * (int)sizeof(T), kWords = kBytes >= 4 ? kBytes / 4 : 1;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = 0u;
+    }
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (kBytes >= 16) {
+#pragma unroll
+            for (int i = 0; i < kWords; i += 4) {
+                const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p) + i / 4);
+                w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w;
+            }
+        } else if constexpr (kBytes == 8) {
+            const uint2 v = __ldcs(reinterpret_cast<const uint2*>(p));
+            w[0] = v.x; w[1] = v.y;
+        } else if constexpr (kBytes == 4) {
+            w[0] = __ldcs(reinterpret_cast<const unsigned int*>(p));
+        } else {
+            w[0] = __ldcs(reinterpret_cast<const unsigned short*>(p));
+        }
+    }
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        else return __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    }
+    __device__ __forceinline__ void set(int i, float v) {
+        if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(v);
+        else {
+            const uint32_t h = __bfloat16_as_ushort(__float2bfloat16_rn(v));
+            w[i / 2] = i % 2 ? (w[i / 2] & 0xffffu) | (h << 16) : h;
+        }
+    }
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (kBytes >= 16) {
+#pragma unroll
+            for (int i = 0; i < kWords; i += 4) reinterpret_cast<uint4*>(p)[i / 4] = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+        } else if constexpr (kBytes == 8) {
+            *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+        } else if constexpr (kBytes == 4) {
+            *reinterpret_cast<uint32_t*>(p) = w[0];
+        } else {
+            *reinterpret_cast<unsigned short*>(p) = (unsigned short)w[0];
+        }
+    }
+};
+
+// out[row] (+)= alpha sum_j weights[row][j] y[slots[row][j]], in 32 bits in the order of j, rounded once.  A warp takes U pieces a lane
+// of a row, a piece as many columns as the rows' boundaries allow, so that slots and weights are read once for all of them, and asks
+// for the pieces of four results at once: bound by the bytes in flight.
+// With one or two results a row it asks for no more than those (registers for four leave too few warps: 60 against 44 us at 52360 x
+// 1024, one result); a few rows are spread over as many warps as they give (U = 1).
+template <typename Y, typename O, int PER, int kAhead, int U>
+__global__ void __launch_bounds__(256) combine_kernel(const CombineArgs p, int chunks) {
     pdl_wait();
     pdl_trigger();
-    constexpr int kAhead = 4, kWords = PER * (int)sizeof(Y) / 16 > 0 ? PER * (int)sizeof(Y) / 16 : 1;
-    const int groups = (p.cols + PER - 1) / PER;
-    const int64_t total = (int64_t)p.rows * groups;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-        const int row = (int)(i / groups), col = (int)(i % groups) * PER;
-        float sum[PER];
+    const int lane = threadIdx.x & 31;
+    const int64_t total = (int64_t)p.rows * chunks;
+    for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < total; i += (int64_t)gridDim.x * 8) {
+        // (a 64-bit division only where the work does not fit 32 bits)
+        const int row = total <= 0xffffffffLL ? (int)((uint32_t)i / (uint32_t)chunks) : (int)(i / chunks);
+        const int col0 = ((int)(i - (int64_t)row * chunks) * U * 32 + lane) * PER;
+        const int64_t k0 = (int64_t)row * p.top_k;
+        float sum[U][PER];
 #pragma unroll
-        for (int c = 0; c < PER; ++c) sum[c] = 0.0f;
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int c = 0; c < PER; ++c) sum[u][c] = 0.0f;
         for (int j0 = 0; j0 < p.top_k; j0 += kAhead) {
             int at[kAhead];
             float w[kAhead];
+            Piece<Y, PER> v[kAhead][U];
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) {
-                const int64_t k = (int64_t)row * p.top_k + j0 + j;
-                at[j] = j0 + j < p.top_k ? __ldg(p.slots + k) : -1;
+                at[j] = j0 + j < p.top_k ? __ldg(p.slots + k0 + j0 + j) : -1;
+                w[j] = j0 + j < p.top_k && p.weights ? __ldg(p.weights + k0 + j0 + j) : 1.0f;
                 if ((unsigned)at[j] >= (unsigned long long)p.y_rows) at[j] = -1;
-                w[j] = at[j] >= 0 ? (p.weights ? __ldg(p.weights + k) : 1.0f) : 0.0f;
             }
-            if constexpr (PER == 8) {
-                uint4 v[kAhead][kWords];
 #pragma unroll
-                for (int j = 0; j < kAhead; ++j)
+            for (int j = 0; j < kAhead; ++j) {
+                if (at[j] < 0) continue;
+                const Y* y = static_cast<const Y*>(p.y) + (int64_t)at[j] * p.ldy;
 #pragma unroll
-                    for (int q = 0; q < kWords; ++q) {
-                        v[j][q] = make_uint4(0, 0, 0, 0);
-                        if (at[j] >= 0) v[j][q] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const Y*>(p.y) + (int64_t)at[j] * p.ldy + col) + q);
-                    }
+                for (int u = 0; u < U; ++u)
+                    if (col0 + u * 32 * PER < p.cols) v[j][u].load(y + col0 + u * 32 * PER);
+            }
 #pragma unroll
-                for (int j = 0; j < kAhead; ++j) {
-                    if (at[j] < 0) continue;
-                    if constexpr (sizeof(Y) == 2) {
-                        const uint32_t u[4] = {v[j][0].x, v[j][0].y, v[j][0].z, v[j][0].w};
+            for (int j = 0; j < kAhead; ++j) {
+                if (at[j] < 0) continue;  // (a weight of zero would not do: 0 * inf)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            sum[2 * c] = fmaf(w[j], __uint_as_float(u[c] << 16), sum[2 * c]);
-                            sum[2 * c + 1] = fmaf(w[j], __uint_as_float(u[c] & 0xffff0000u), sum[2 * c + 1]);
-                        }
-                    } else {
+                for (int u = 0; u < U; ++u)
 #pragma unroll
-                        for (int q = 0; q < kWords; ++q) {
-                            const uint32_t u[4] = {v[j][q].x, v[j][q].y, v[j][q].z, v[j][q].w};
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) sum[4 * q + c] = fmaf(w[j], __uint_as_float(u[c]), sum[4 * q + c]);
-                        }
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < kAhead; ++j)
-                    if (at[j] >= 0) sum[0] = fmaf(w[j], (float)static_cast<const Y*>(p.y)[(int64_t)at[j] * p.ldy + col], sum[0]);
+                    for (int c = 0; c < PER; ++c) sum[u][c] = fmaf(w[j], v[j][u].get(c), sum[u][c]);
             }
         }
-        if (p.out_mode == kOutBf16) {
-            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + (int64_t)row * p.ldo + col;
-            if constexpr (PER == 8) {
-                uint32_t u[4];
+        O* out = static_cast<O*>(p.out) + (int64_t)row * p.ldo;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    __nv_bfloat162 b = __floats2bfloat162_rn(p.alpha * sum[2 * c], p.alpha * sum[2 * c + 1]);
-                    u[c] = *reinterpret_cast<uint32_t*>(&b);
-                }
-                *reinterpret_cast<uint4*>(out) = make_uint4(u[0], u[1], u[2], u[3]);
-            } else {
-                *out = __float2bfloat16_rn(p.alpha * sum[0]);
-            }
-        } else {
-            float* out = static_cast<float*>(p.out) + (int64_t)row * p.ldo + col;
+        for (int u = 0; u < U; ++u) {
+            const int col = col0 + u * 32 * PER;
+            if (col >= p.cols) continue;
+            Piece<O, PER> r;
+            r.zero();
+            if (sizeof(O) == 4 && p.out_mode == kOutResidual) r.load(out + col);
 #pragma unroll
-            for (int c = 0; c < PER; c += 4) {
-                if constexpr (PER == 8) {
-                    float4 v = make_float4(p.alpha * sum[c], p.alpha * sum[c + 1], p.alpha * sum[c + 2], p.alpha * sum[c + 3]);
-                    if (p.out_mode == kOutResidual) {
-                        const float4 o = *reinterpret_cast<const float4*>(out + c);
-                        v = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
-                    }
-                    *reinterpret_cast<float4*>(out + c) = v;
-                } else {
-                    *out = (p.out_mode == kOutResidual ? *out : 0.0f) + p.alpha * sum[0];
-                }
+            for (int c = 0; c < PER; ++c) {
+                float v = p.alpha * sum[u][c];
+                if (sizeof(O) == 4 && p.out_mode == kOutResidual) v += r.get(c);
+                r.set(c, v);
             }
+            r.store(out + col);
         }
+    }
+}
+
+template <typename Y, typename O, int PER>
+cudaError_t combine_per(const CombineArgs& g, cudaStream_t stream) {
+    constexpr int kWide = PER == 8 ? 4 : 8;  // pieces a lane: 2 KB of a bf16 row a warp, less of rows on narrower boundaries
+    auto go = [&](auto kernel, int pieces) {
+        const int wide = 32 * PER * pieces, chunks = (g.cols + wide - 1) / wide;
+        const dim3 grid((unsigned)std::min<int64_t>(((int64_t)g.rows * chunks + 7) / 8, 1 << 20));
+        return launch_pdl(kernel, grid, 256, 0, stream, 1, g, chunks);
+    };
+    if ((int64_t)g.rows * ((g.cols + 32 * PER - 1) / (32 * PER)) <= kCombineFew) return go(combine_kernel<Y, O, PER, 4, 1>, 1);
+    if (g.top_k == 1) return go(combine_kernel<Y, O, PER, 1, kWide>, kWide);
+    if (g.top_k == 2) return go(combine_kernel<Y, O, PER, 2, kWide>, kWide);
+    return go(combine_kernel<Y, O, PER, 4, kWide>, kWide);
+}
+
+template <typename Y, typename O>
+cudaError_t combine_t(const CombineArgs& g, cudaStream_t stream) {
+    // boundaries that every row of both sides has, in values: a piece of PER lies on min(PER values, 16 bytes)
+    auto fits = [&](int per) {
+        const int yb = std::min<int>(per * sizeof(Y), 16), ob = std::min<int>(per * sizeof(O), 16);
+        return g.cols % per == 0 && !(reinterpret_cast<uintptr_t>(g.y) % yb) && !(reinterpret_cast<uintptr_t>(g.out) % ob) &&
+               !((g.ldy * (int)sizeof(Y)) % yb) && !((g.ldo * (int)sizeof(O)) % ob);
+    };
+    const int per = fits(8) ? 8 : (fits(4) ? 4 : (fits(2) ? 2 : 1));
+    switch (per) {
+        case 8: return combine_per<Y, O, 8>(g, stream);
+        case 4: return combine_per<Y, O, 4>(g, stream);
+        case 2: return combine_per<Y, O, 2>(g, stream);
+        default: return combine_per<Y, O, 1>(g, stream);
     }
 }
 
@@ -496,15 +555,8 @@ cudaError_t route_launch(const RouteArgs& args, cudaStream_t stream, int64_t* la
 
 cudaError_t combine_launch(const CombineArgs& g, cudaStream_t stream) {
     if (g.rows <= 0) return cudaSuccess;
-    const int ye = g.y_f32 ? 4 : 2, oe = g.out_mode == kOutBf16 ? 2 : 4;
-    const bool vec = g.cols % 8 == 0 && !((reinterpret_cast<uintptr_t>(g.y) | reinterpret_cast<uintptr_t>(g.out)) & 15) &&
-                     !((g.ldy * ye) & 15) && !((g.ldo * oe) & 15);
-    const int64_t threads = (int64_t)g.rows * (vec ? g.cols / 8 : g.cols);
-    const dim3 grid((unsigned)std::min<int64_t>((threads + 255) / 256, 1 << 20));
-    if (vec) return g.y_f32 ? launch_pdl(combine_kernel<float, 8>, grid, 256, 0, stream, 1, g)
-                            : launch_pdl(combine_kernel<__nv_bfloat16, 8>, grid, 256, 0, stream, 1, g);
-    return g.y_f32 ? launch_pdl(combine_kernel<float, 1>, grid, 256, 0, stream, 1, g)
-                   : launch_pdl(combine_kernel<__nv_bfloat16, 1>, grid, 256, 0, stream, 1, g);
+    if (g.out_mode == kOutBf16) return g.y_f32 ? combine_t<float, __nv_bfloat16>(g, stream) : combine_t<__nv_bfloat16, __nv_bfloat16>(g, stream);
+    return g.y_f32 ? combine_t<float, float>(g, stream) : combine_t<__nv_bfloat16, float>(g, stream);
 }
 
 }  // namespace sb

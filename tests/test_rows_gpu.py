@@ -340,9 +340,10 @@ def test_grouped_masked_rows_do_not_spread(ctx):
 
 # ------------------------------------------------------------------------------------------------------------ combine
 @pytest.mark.parametrize("rows,k,cols", [(1, 1, 1), (24, 2, 1024), (77, 3, 640), (130, 4, 1030), (1000, 8, 72), (5, 16, 33), (3000, 2, 1016)])
+@pytest.mark.parametrize("pad", [3, 4, 8])
 @pytest.mark.parametrize("y_f32", [False, True])
 @pytest.mark.parametrize("mode", [0, 1, 2])
-def test_combine(ctx, rows, k, cols, y_f32, mode):
+def test_combine(ctx, rows, k, cols, y_f32, mode, pad):
     import scriptrs_b200 as sb
 
     g = gen(rows + cols)
@@ -356,12 +357,12 @@ def test_combine(ctx, rows, k, cols, y_f32, mode):
         slots[2] = -1  # a row without results
     y[y_rows - 1] = float("nan")
     slots[slots == y_rows - 1] = 0
-    out = torch.full((rows + 1, cols + 3), 3.0, device="cuda", dtype=torch.bfloat16 if mode == 0 else torch.float32)
+    out = torch.full((rows + 1, cols + pad), 3.0, device="cuda", dtype=torch.bfloat16 if mode == 0 else torch.float32)
     for weights in (w, None):
         out.fill_(3.0)
         torch.cuda.synchronize()
         sb.combine_rows(ctx, y.data_ptr(), slots.data_ptr(), weights.data_ptr() if weights is not None else 0, out.data_ptr(), rows, k, cols, y_rows,
-                        ldy=cols + 8, ldo=cols + 3, y_f32=y_f32, out_mode=mode, alpha=0.5)
+                        ldy=cols + 8, ldo=cols + pad, y_f32=y_f32, out_mode=mode, alpha=0.5)
         ctx.synchronize()
         ok = (slots >= 0) & (slots < y_rows)
         f = (w if weights is not None else torch.ones_like(w)).double() * ok.double()

@@ -484,14 +484,13 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
             if constexpr (MODE == kAdapters) {
                 for (int c = 0; c < phases; ++c) {
                     AdapterIds<kTileRows> ids = all;
-                    for (int id = ids.next(); ok && id >= 0;) {
+                    while (ok && ids.any()) {
                         int u_row[C::kUps], n = 0;
 #pragma unroll
                         for (int u = 0; u < C::kUps; ++u) {
-                            if (id < 0) continue;
+                            const int id = ids.next();
                             u_row[u] = id * p.N + w_col;
-                            n = u + 1;
-                            id = ids.next();
+                            n += id >= 0;
                         }
                         ok = __all_sync(0xffffffffu, mbar_wait(empty_bar(stage), ph ^ 1, abort_flag));
                         if (!ok) break;
@@ -520,15 +519,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
         bool ok = true;
         for (long long t = tile0; rank == 0 && ok && walk.find(t, BN, tile); t += tile_step) {
             AdapterIds<kTileRows> all;
-            int mine[4 * CTAS];  // of rows 32 q + lane
-            if (MODE == kAdapters) {
-                all.load(p.row_adapter, p.n_adapters, tile.row0, tile.row1, lane);
-#pragma unroll
-                for (int q = 0; q < 4 * CTAS; ++q) {
-                    const int row = tile.row0 + q * 32 + lane;
-                    mine[q] = row < tile.row1 ? __ldg(p.row_adapter + row) : -1;
-                }
-            }
+            if (MODE == kAdapters) all.load(p.row_adapter, p.n_adapters, tile.row0, tile.row1, lane);
             int kt = 0;
             while (ok && kt < k_tiles) {
                 const int acc = seg & 1;
@@ -560,21 +551,20 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                     if (ok && last) {
                         for (int c = 0; ok && c < phases; ++c) {
                             AdapterIds<kTileRows> ids = all;
-                            int id = ids.next();
-                            if (id < 0) break;
+                            if (!ids.any()) break;
                             ok = __all_sync(0xffffffffu, rows_wait_pair<CTAS>(low_bar, low_ph, abort_flag));
                             low_ph ^= 1;
                             const int groups = min(kGroups, (p.rank - c * kPhaseCols + 15) / 16);
-                            while (ok && id >= 0) {
+                            while (ok && ids.any()) {
                                 ok = __all_sync(0xffffffffu, mbar_wait(full_bar(stage), ph, abort_flag));
                                 if (!ok) break;
                                 tc_fence_after();
 #pragma unroll
                                 for (int u = 0; u < C::kUps; ++u) {
-                                    if (id < 0) continue;
                                     uint32_t off[4 * CTAS];
+                                    if (ids.next(off) < 0) continue;
 #pragma unroll
-                                    for (int q = 0; q < 4 * CTAS; ++q) off[q] = ~__ballot_sync(0xffffffffu, mine[q] == id);
+                                    for (int q = 0; q < 4 * CTAS; ++q) off[q] = ~off[q];
                                     if (elect_one()) {
                                         const uint64_t adesc = make_smem_desc(base + kLowAt);
                                         const uint64_t bdesc = make_smem_desc(a_base + stage * C::kStageBytes + u * C::kBBytes);
@@ -590,11 +580,10 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                                         }
                                     }
                                     __syncwarp();
-                                    id = ids.next();
                                 }
                                 if (elect_one()) {
                                     rows_commit<CTAS>(empty_bar(stage));
-                                    if (id < 0) rows_commit<CTAS>(lowfree_bar);
+                                    if (!ids.any()) rows_commit<CTAS>(lowfree_bar);
                                 }
                                 __syncwarp();
                                 if (++stage == S) { stage = 0; ph ^= 1; }
@@ -882,7 +871,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
         for (long long t = tile0; ok && walk.find(t, BN, tile); t += tile_step) {
             AdapterIds<kTileRows> ids;
             ids.load(p.row_adapter, p.n_adapters, tile.row0, tile.row1, lane);
-            if (ids.next() < 0) continue;
+            if (!ids.any()) continue;
             const int row = tile.row0 + cta_row + r;
             for (int c = 0; c < phases; ++c) {
                 float f[kPhaseCols];

@@ -31,8 +31,7 @@ struct AdapterIds {
 #pragma unroll
         for (int q = kWords - 1; q >= 0; --q)
             if (left[q]) { held = ids[q]; word = left[q]; }
-        if (!word) return -1;
-        const int id = __shfl_sync(0xffffffffu, held, __ffs(word) - 1);
+        const int id = __shfl_sync(0xffffffffu, held, __ffs(word) - 1);  // (held is -1 everywhere where nothing is left)
 #pragma unroll
         for (int q = 0; q < kWords; ++q) {
             rows[q] = __ballot_sync(0xffffffffu, ids[q] == id);

@@ -559,15 +559,19 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                                 ok = __all_sync(0xffffffffu, mbar_wait(full_bar(stage), ph, abort_flag));
                                 if (!ok) break;
                                 tc_fence_after();
+                                uint32_t off[C::kUps][4 * CTAS];  // lanes of other rows
+                                int n = 0;
 #pragma unroll
                                 for (int u = 0; u < C::kUps; ++u) {
-                                    uint32_t off[4 * CTAS];
-                                    if (ids.next(off) < 0) continue;
+                                    n += ids.next(off[u]) >= 0;
 #pragma unroll
-                                    for (int q = 0; q < 4 * CTAS; ++q) off[q] = ~off[q];
-                                    if (elect_one()) {
-                                        const uint64_t adesc = make_smem_desc(base + kLowAt);
-                                        const uint64_t bdesc = make_smem_desc(a_base + stage * C::kStageBytes + u * C::kBBytes);
+                                    for (int q = 0; q < 4 * CTAS; ++q) off[u][q] = ~off[u][q];
+                                }
+                                if (elect_one()) {
+                                    const uint64_t adesc = make_smem_desc(base + kLowAt), bdesc = make_smem_desc(a_base + stage * C::kStageBytes);
+#pragma unroll
+                                    for (int u = 0; u < C::kUps; ++u) {
+                                        if (u >= n) break;
 #pragma unroll
                                         for (int g = 0; g < kGroups; ++g) {
                                             if (g >= groups) break;
@@ -575,13 +579,11 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                                             for (int e = 0; e < kTerms; ++e) {
                                                 constexpr int kTile = kBM * kRowBytes / 16;  // in the descriptor's 16-byte units
                                                 const int at = g * kTerms + e;
-                                                rows_mma_lanes<CTAS>(d_tmem, adesc + at / 4 * kTile + 2 * (at % 4), bdesc + 2 * g, idesc, off);
+                                                rows_mma_lanes<CTAS>(d_tmem, adesc + at / 4 * kTile + 2 * (at % 4), bdesc + u * (C::kBBytes / 16) + 2 * g, idesc,
+                                                                     off[u]);
                                             }
                                         }
                                     }
-                                    __syncwarp();
-                                }
-                                if (elect_one()) {
                                     rows_commit<CTAS>(empty_bar(stage));
                                     if (!ids.any()) rows_commit<CTAS>(lowfree_bar);
                                 }

@@ -7,7 +7,7 @@
 //   - very few rows: a warp per row and eight columns, K over the lanes.
 //   - between them: 16 rows a block on mma.sync m16n8k16 with operands straight from global memory, K over the warps, the columns over
 //     blocks; a row takes its adapter's product (selected, not masked by zeros).
-//     Where more than two adapters meet in the 16 rows, a row is a chain of dot products over the lanes of a warp instead.
+//     Where more than six adapters meet in the 16 rows, a row is a chain of dot products over the lanes of a warp instead.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -25,7 +25,8 @@ namespace {
 
 constexpr int kDownWarps = 8;
 constexpr int kDotsMost = 4096;  // rows x rank up to which every row reads its adapter for itself (8 MB from L2 at K = 1024)
-constexpr int kMaxProducts = 2;  // adapters in 16 rows above which the rows are taken one by one
+constexpr int kMaxProducts = 6;  // adapters in 16 rows above which the rows are taken one by one: at 2048 rows of 1024 a product
+                                 // costs 1.1 us at rank 16 and 4 us at rank 64, the rows one by one 7 and 28
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -178,7 +179,7 @@ __global__ void __launch_bounds__(kDownWarps * 32, 1) adapter_down_kernel(const 
             for (int c = 0; c < kCols; c += 8) {
                 const int cols = min(p.rank - col0 - c, 8);
                 float v = 0.0f;
-                if (mine && cols > 0) v = row_dots<2>(a + (int64_t)(row0 + r) * p.lda, down + ((int64_t)cur * p.rank + col0 + c) * p.K, p.K, cols, lane);
+                if (mine && cols > 0) v = row_dots<4>(a + (int64_t)(row0 + r) * p.lda, down + ((int64_t)cur * p.rank + col0 + c) * p.K, p.K, cols, lane);
                 if (lane < 8) part[warp][r][c + lane] = v;
             }
         }

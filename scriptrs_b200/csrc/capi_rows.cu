@@ -106,7 +106,8 @@ int32_t sb_grouped_gemm(sb_ctx* c, const void* d_a, int64_t lda, int64_t a_rows,
 
 int32_t sb_combine_rows(sb_ctx* c, const void* d_y, int32_t y_f32, int64_t ldy, int64_t y_rows, const int32_t* d_slots, const float* d_weights,
                         void* d_out, int64_t ldo, int64_t rows, int64_t top_k, int64_t cols, int32_t out_mode, float alpha) {
-    if (rows < 0 || rows > kLimit || top_k <= 0 || top_k > kLimit || cols <= 0 || cols > kLimit || y_rows < 0 || y_rows > kLimit || ldy < cols ||
+    // (columns and a row's results are counted in 32 bits, past the last by up to a warp's pieces)
+    if (rows < 0 || rows > kLimit || top_k <= 0 || top_k > kLimit / 2 || cols <= 0 || cols > kLimit / 2 || y_rows < 0 || y_rows > kLimit || ldy < cols ||
         ldo < cols || out_mode < 0 || out_mode > 2)
         return fail(SB_INVALID_ARGUMENT, "bad shape or output mode");
     if (rows > 0 && ((!d_y && y_rows > 0) || !d_slots || !d_out)) return fail(SB_INVALID_ARGUMENT, "null argument");

@@ -62,7 +62,8 @@ def test_route_refusals(change):
 
 
 @pytest.mark.parametrize("change", [dict(rows=-1), dict(k=0), dict(cols=0), dict(ldy=31), dict(ldo=31), dict(mode=3), dict(y=None), dict(slots=None),
-                                    dict(out=None), dict(y=P + 1), dict(y_f32=1, y=P + 2), dict(mode=1, out=P + 2), dict(slots=P + 2), dict(y_rows=-1)], ids=str)
+                                    dict(out=None), dict(y=P + 1), dict(y_f32=1, y=P + 2), dict(mode=1, out=P + 2), dict(slots=P + 2), dict(y_rows=-1),
+                                    dict(k=2 ** 31 - 1, rows=1), dict(cols=2 ** 31 - 1, ldy=2 ** 31, ldo=2 ** 31)], ids=str)
 def test_combine_refusals(change):
     assert call("sb_combine_rows", COMBINE, **change) == 11
     assert "ctx" not in message()

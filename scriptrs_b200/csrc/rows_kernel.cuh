@@ -12,14 +12,15 @@
 //   - Rows leave through a swizzled slab per warp: 32 rows of one group by a TMA store (or reduce-add), which clips at column N;
 //     the last rows of a group, behind which its neighbour's begin, and results off the 16-byte boundaries by ordinary stores.
 //   - The low-rank addition is K = rank more columns of the same product, accumulated in the same tensor memory, `low` against the
-//     rows of U_a.  Where the result is bf16, `low` is rounded to bf16 too, as between any two bf16 products: 2^-9 of the addition,
-//     below the result's own rounding (a second term, 2^-17, took 13 % of the product's time at rank 64 with two adapters a tile).
-//     Where the result is stored in 32 bits it enters as three bf16 terms (2^-26).
+//     rows of U_a.  Where the result is bf16, `low` is rounded to bf16 too, as between any two bf16 products: at most 2^-8 of
+//     |low| |U_a|, as the result's own rounding is 2^-8 of the result (a second term, 2^-16, took 13 % of the product's time at
+//     rank 64 with two adapters a tile).  Where the result is stored in 32 bits it enters as three bf16 terms (2^-24).
 //     A tile may hold rows of several adapters: its MMAs run once for each, with the lanes of the other rows disabled, so that
 //     nothing of one adapter (not even a NaN) reaches rows of another, and the shared weights are read once whatever the adapters.
 //   - Up to 32 rows (live streams, as a rule each with an adapter of its own): an MMA per adapter would take longer than all of
 //     K, so the addition is formed on CUDA cores by the four warps that stage `low` otherwise, in 32 bits, U_a on its way before
-//     `low` is there, and the epilogue adds it (24 rows with as many adapters, rank 16, 1024 -> 4096: 14.8 -> 10.1 us).
+//     `low` is there, and the epilogue adds it (24 rows with as many adapters, rank 16, 1024 -> 4096: 14.8 -> 10.1 us,
+//     and 6.5 us with A stages of 32 rows).
 //   - The tensor core adds into its accumulator by truncation, 1e-6 of the result at K = 1024 and 4.4e-6 at 4096 (measured).
 //     Where the result is stored in 32 bits, it is collected in registers every kSegment stages, rounded to nearest (4.7e-7 at
 //     either K; every four stages: 2.5e-7, but 16384 x 1024 x 1024 then takes 48 us instead of 36, a handshake per segment).

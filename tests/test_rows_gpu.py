@@ -5,8 +5,10 @@ cut off at 24 bits of the largest: at most 17 * 2^-23 (33 * 2^-23) of S, the sum
 is collected every 256 (512) columns of K, that is after 16 MMAs, so its error is below 16 * 33 * 2^-23 S < 2^-13 S whatever K,
 in practice far less: the norm is held to 1e-5 as for the shared product.  bf16 results add one rounding, 2^-8 of the value
 (2^-8 / sqrt(3) in the norm at most, below 4e-3), and sum all of K without a collection: K / 16 * 17 * 2^-23 S < 2^-10 S at
-K = 4096 in the worst case.  The low-rank addition keeps 2^-16 of its first product.  SiLU passes errors on with a factor
-below 1.1 and adds a few 2^-22 of its own."""
+K = 4096 in the worst case.  The first product of a low-rank addition enters a 32-bit result as three bf16 terms, 2^-24 of it; a
+bf16 result as one, 2^-8 |low| |U| = 4 * 2^-10 |low| |U| (in the norm again 2^-8 / sqrt(3) of an addition that is no larger than
+the result: together with the result's own rounding 3.2e-3).  SiLU passes errors on with a factor below 1.1 and adds a few
+2^-22 of its own."""
 import numpy as np
 import pytest
 
@@ -398,7 +400,10 @@ def adapter_case(ctx, who, n_adapters, rank, N, K, *, act=0, mode=0, bias=True, 
             continue
         if bool(here.any()):
             s = float(sc[n]) if scale else 1.0
-            y[here] += s * ((x[here] @ down[n].double().T) @ up[n].double().T)
+            low = x[here] @ down[n].double().T
+            y[here] += s * (low @ up[n].double().T)
+            if mode == 0:
+                size[here] += 4 * s * (low.abs() @ up[n].double().abs().T)  # `low` in bf16
             size[here] += s * ((x[here].abs() @ down[n].double().abs().T) @ up[n].double().abs().T)
     if bias:
         y, size = y + b.double(), size + b.double().abs()

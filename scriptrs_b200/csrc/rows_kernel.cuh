@@ -10,7 +10,8 @@
 //   - Rows picked by an index arrive by TMA gathers of four rows each, issued by four warps (32 rows each) from one elected
 //     lane (from every lane by turns a gather takes ten times as long); a tile with few rows fetches only those.
 //   - Rows leave through a swizzled slab per warp: 32 rows of one group by a TMA store (or reduce-add), which clips at column N;
-//     the last rows of a group, behind which its neighbour's begin, and results off the 16-byte boundaries by ordinary stores.
+//     the last rows of a group, behind which its neighbour's begin, results off the 16-byte boundaries, and the last columns where N
+//     ends inside 16 bytes (the store clips at whole ones) by ordinary stores.
 //   - The low-rank addition is K = rank more columns of the same product, accumulated in the same tensor memory, `low` against the
 //     rows of U_a.  Where the result is bf16, `low` is rounded to bf16 too, as between any two bf16 products: at most 2^-8 of
 //     |low| |U_a|, as the result's own rounding is 2^-8 of the result (a second term, 2^-16, took 13 % of the product's time at
@@ -182,6 +183,7 @@ struct RowsParams {
     int M, N, K, n_groups, act, out_mode;
     float alpha;
     bool out_vec;    // output rows on 16-byte boundaries
+    bool n_vec;      // and N columns end on one (a TMA store clips at column N in whole 16 bytes)
     // adapters
     const int32_t* row_adapter;
     const float* low;
@@ -672,8 +674,8 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                 if (elect_one()) bulk_wait_read0();
                 __syncwarp();
             };
-            auto leave = [&](int col0, auto&& store) {
-                if (whole) {
+            auto leave = [&](int col0, int cols, auto&& store) {
+                if (whole && (p.n_vec || col0 + cols <= p.N)) {
                     fence_proxy_async();
                     __syncwarp();
                     if (elect_one()) {
@@ -727,7 +729,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                     for (int q = 0; q < 8; ++q)
                         *reinterpret_cast<float4*>(slab + lane * 128 + ((q ^ (lane & 7)) << 4)) =
                             make_float4(p.alpha * x[4 * q], p.alpha * x[4 * q + 1], p.alpha * x[4 * q + 2], p.alpha * x[4 * q + 3]);
-                    leave(col0, [&]() { rows_store<float, 32>(slab, p, row0, tile.row1, col0, lane); });
+                    leave(col0, 32, [&]() { rows_store<float, 32>(slab, p, row0, tile.row1, col0, lane); });
                 }
             } else {
                 constexpr int kCols = C::kHalfCols < 64 ? C::kHalfCols : 64;
@@ -768,7 +770,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                         for (int q = 0; q < kCols / 8; ++q)
                             *reinterpret_cast<uint4*>(slab + lane * (kCols * 2) + ((q ^ ((lane >> kShift) & kMask)) << 4)) =
                                 make_uint4(packed[4 * q], packed[4 * q + 1], packed[4 * q + 2], packed[4 * q + 3]);
-                        leave(col0, [&]() { rows_store<__nv_bfloat16, kCols>(slab, p, row0, tile.row1, col0, lane); });
+                        leave(col0, kCols, [&]() { rows_store<__nv_bfloat16, kCols>(slab, p, row0, tile.row1, col0, lane); });
                     }
                 }
                 if (held) release();
@@ -943,6 +945,7 @@ cudaError_t rows_launch_t(const RowsArgs& g, int sm_count, int* d_error, cudaStr
     p.a_rows = g.a_rows; p.ldo = g.ldo; p.M = g.M; p.N = g.N; p.K = g.K; p.n_groups = g.n_groups; p.act = g.act; p.out_mode = g.out_mode;
     p.alpha = g.alpha;
     p.out_vec = !(reinterpret_cast<uintptr_t>(g.out) & 15) && !((g.ldo * eb) & 15);
+    p.n_vec = (int64_t)g.N * eb % 16 == 0;
     mo = mw;  // stores by TMA want 32 rows of a group
     if (p.out_vec && g.M >= 32 && !rows_out_map(&mo, g.out, g.M, g.N, g.ldo, F32, F32 || RCfg<BN, CTAS, MODE, F32>::kHalfCols >= 64 ? 128 : 64)) return cudaErrorInvalidValue;
     p.row_adapter = g.row_adapter; p.low = g.low; p.up = g.up; p.rank = g.rank; p.n_adapters = g.n_adapters;

@@ -245,6 +245,17 @@ def test_grouped_strides_and_boundaries(ctx, gather, mode):
     grouped_case(ctx, [70, 60], 201, 64, gather=gather, mode=mode, pad_o=1, shift=3)
 
 
+@pytest.mark.parametrize("N,pad", [(203, 5), (201, 7), (1030, 10), (2, 6)])
+@pytest.mark.parametrize("mode", [0, 1, 2])
+def test_columns_behind_the_last_are_left(ctx, N, pad, mode):
+    """Rows on 16-byte boundaries whose last column lies inside 16 bytes: what stands behind it stays."""
+    grouped_case(ctx, [70, 300, 60], N, 64, mode=mode, pad_o=pad)
+    grouped_case(ctx, [70, 300, 60], N, 64, mode=mode, gather=90, pad_o=pad)
+    grouped_case(ctx, [20, 0, 12], N, 64, mode=mode, gather=90, pad_o=pad)
+    adapter_case(ctx, [i // 90 % 3 - 1 for i in range(400)], 2, 16, N, 64, mode=mode, pad_o=pad)
+    adapter_case(ctx, [i % 3 - 1 for i in range(32)], 2, 16, N, 64, mode=mode, pad_o=pad)
+
+
 @pytest.mark.parametrize("M,N,K,G", [(9000, 1024, 512, 3), (20011, 512, 256, 9), (4000, 2048, 1024, 1)])
 @pytest.mark.parametrize("gather", [0, 777])
 def test_grouped_large(ctx, M, N, K, G, gather):

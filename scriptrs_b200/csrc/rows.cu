@@ -63,11 +63,12 @@ cudaError_t rows_configure(const char** why) {
 cudaError_t rows_launch(const RowsArgs& g, int sm_count, int* d_error, cudaStream_t stream) {
     if (!g_rows_encode) return cudaErrorNotReady;
     if (g.M <= 0) return cudaSuccess;
-    const RowsTileShape t = rows_tile(g.M, g.N, g.n_groups, g.out_mode != kOutBf16, sm_count);
+    // few rows a group: gathers fetch only those, a box always 128
+    const bool picked = g.rows || (int64_t)g.M < (int64_t)g.n_groups * 64;
+    const RowsTileShape t = rows_tile(g.M, g.N, g.n_groups, g.out_mode != kOutBf16, picked, sm_count);
     if (rows_few(g)) return rows_few_launch(g, t, sm_count, d_error, stream);
     if (g.row_adapter) return rows_adapters_launch(g, t, sm_count, d_error, stream);
-    // few rows a group: gathers fetch only those, a box always 128
-    if (g.rows || (int64_t)g.M < (int64_t)g.n_groups * 64) return rows_gathered_launch(g, t, sm_count, d_error, stream);
+    if (picked) return rows_gathered_launch(g, t, sm_count, d_error, stream);
     return rows_grouped_launch(g, t, sm_count, d_error, stream);
 }
 

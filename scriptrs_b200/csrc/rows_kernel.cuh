@@ -84,9 +84,10 @@ struct RCfg {
     static constexpr uint32_t kTmemCols = 2 * BN;
 };
 
-// Four warps more where rows are picked (gathers) or have adapters (`low`), 32 rows each.
-constexpr int kAuxWarps = 4;
-constexpr int rows_threads(int mode) { return 32 * (2 + kEpiWarps + (mode == kGrouped ? 0 : kAuxWarps)); }
+// Warps more where rows are picked (gathers) or have adapters (`low`): four, 32 rows each; two beside an epilogue that keeps 128 sums
+// a thread in registers (168 registers for 12 warps, 144 for 14).
+constexpr int rows_aux_warps(int mode, int bn, bool f32) { return mode == kGrouped ? 0 : (f32 && bn == 256 ? 2 : 4); }
+constexpr int rows_threads(int mode, int bn, bool f32) { return 32 * (2 + kEpiWarps + rows_aux_warps(mode, bn, f32)); }
 
 template <int BN, int CTAS, bool FP8>
 __device__ __forceinline__ uint32_t rows_idesc() {
@@ -368,7 +369,7 @@ __device__ __forceinline__ float bf16_rest(float v) {
 }
 
 template <int BN, int CTAS, bool FP8, int MODE, bool F32>
-__global__ void __launch_bounds__(rows_threads(MODE), 1)
+__global__ void __launch_bounds__(rows_threads(MODE, BN, F32), 1)
 rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_w,
             const __grid_constant__ CUtensorMap tma_up, const __grid_constant__ CUtensorMap tma_out, const RowsParams p,
             int* __restrict__ error) {
@@ -376,6 +377,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
     constexpr int S = C::kStages;
     constexpr int kStepCols = FP8 ? 128 : 64;
     constexpr int kTerms = C::kTerms, kGroups = C::kGroups, kPhaseCols = 16 * kGroups;
+    constexpr int kAuxWarps = rows_aux_warps(MODE, BN, F32);
     // rank of this CTA in its pair (the leader, rank 0, owns the barriers that the MMAs wait on)
     const uint32_t rank = CTAS == 2 ? __shfl_sync(0xffffffffu, cluster_ctarank(), 0) : 0u;
     extern __shared__ __align__(1024) unsigned char smem_dyn[];  // the operands' swizzle wants 1024-byte boundaries
@@ -418,7 +420,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
             mbar_init(tfull_bar(a), 1);
             mbar_init(tempty_bar(a), 4 * C::kHalves * CTAS);
         }
-        mbar_init(low_bar, kAuxWarps * CTAS);
+        mbar_init(low_bar, std::max(kAuxWarps, 1) * CTAS);
         mbar_init(lowfree_bar, MODE == kFewAdapters ? C::kHalves : 1);
         *abort_flag = 0;
         rows_set_turn(turn_at, 0);
@@ -867,9 +869,8 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
             if (ok && lane == 0) mbar_arrive(low_bar);
         }
     } else if constexpr (MODE == kAdapters) {
-        // ------------------------------------------------------------ `low` of the tile's rows as an operand, a row per thread
-        const int r = (warp - 2 - kEpiWarps) * 32 + lane;
-        unsigned char* dst = base_ptr + kLowAt + r * kRowBytes;
+        // ------------------------------------------------------------ `low` of the tile's rows as an operand, a row per thread at a time
+        const int r0 = (warp - 2 - kEpiWarps) * 32 + lane;
         uint32_t ph = 0;
         bool ok = true;
         pdl_wait();
@@ -877,38 +878,43 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
             AdapterIds<kTileRows> ids;
             ids.load(p.row_adapter, p.n_adapters, tile.row0, tile.row1, lane);
             if (!ids.any()) continue;
-            const int row = tile.row0 + cta_row + r;
-            for (int c = 0; c < phases; ++c) {
-                float f[kPhaseCols];
+            for (int c = 0; ok && c < phases; ++c) {
+#pragma unroll 1
+                for (int r = r0; r < kBM; r += 32 * kAuxWarps) {
+                    const int row = tile.row0 + cta_row + r;
+                    unsigned char* dst = base_ptr + kLowAt + r * kRowBytes;
+                    float f[kPhaseCols];
 #pragma unroll
-                for (int i = 0; i < kPhaseCols; i += 4) {
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (row < tile.row1 && c * kPhaseCols + i < p.rank)
-                        v = *reinterpret_cast<const float4*>(p.low + (int64_t)row * p.rank + c * kPhaseCols + i);
-                    f[i] = v.x; f[i + 1] = v.y; f[i + 2] = v.z; f[i + 3] = v.w;
-                }
-                ok = __all_sync(0xffffffffu, mbar_wait(lowfree_bar, ph ^ 1, abort_flag));
-                if (!ok) break;
-#pragma unroll
-                for (int g = 0; g < kGroups; ++g)
-#pragma unroll
-                    for (int e = 0; e < kTerms; ++e) {
-                        uint32_t w[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            float& x = f[16 * g + 2 * i];
-                            float& y = f[16 * g + 2 * i + 1];
-                            w[i] = pack_bf16(x, y);
-                            if (kTerms > 1) {
-                                x = bf16_rest(x);
-                                y = bf16_rest(y);
-                            }
-                        }
-                        const int at = g * kTerms + e, chunk = 2 * (at % 4);
-                        unsigned char* d = dst + at / 4 * kBM * kRowBytes;
-                        *reinterpret_cast<uint4*>(d + ((chunk ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                        *reinterpret_cast<uint4*>(d + (((chunk + 1) ^ (r & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
+                    for (int i = 0; i < kPhaseCols; i += 4) {
+                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (row < tile.row1 && c * kPhaseCols + i < p.rank)
+                            v = *reinterpret_cast<const float4*>(p.low + (int64_t)row * p.rank + c * kPhaseCols + i);
+                        f[i] = v.x; f[i + 1] = v.y; f[i + 2] = v.z; f[i + 3] = v.w;
                     }
+                    if (r == r0) ok = __all_sync(0xffffffffu, mbar_wait(lowfree_bar, ph ^ 1, abort_flag));
+                    if (!ok) break;
+#pragma unroll
+                    for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+                        for (int e = 0; e < kTerms; ++e) {
+                            uint32_t w[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                float& x = f[16 * g + 2 * i];
+                                float& y = f[16 * g + 2 * i + 1];
+                                w[i] = pack_bf16(x, y);
+                                if (kTerms > 1) {
+                                    x = bf16_rest(x);
+                                    y = bf16_rest(y);
+                                }
+                            }
+                            const int at = g * kTerms + e, chunk = 2 * (at % 4);
+                            unsigned char* d = dst + at / 4 * kBM * kRowBytes;
+                            *reinterpret_cast<uint4*>(d + ((chunk ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                            *reinterpret_cast<uint4*>(d + (((chunk + 1) ^ (r & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
+                        }
+                }
+                if (!ok) break;
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) {
@@ -953,7 +959,7 @@ cudaError_t rows_launch_t(const RowsArgs& g, int sm_count, int* d_error, cudaStr
     const int64_t n_tiles = (g.N + BN - 1) / BN;
     const int64_t tiles = ((int64_t)(g.M + kBM * CTAS - 1) / (kBM * CTAS) + std::min(g.n_groups - 1, g.M)) * n_tiles;
     const int grid = CTAS * (int)std::min<int64_t>(tiles, sm_count / CTAS);
-    return launch_pdl(rows_kernel<BN, CTAS, FP8, MODE, F32>, dim3(grid), rows_threads(MODE), RCfg<BN, CTAS, MODE, F32>::kSmemBytes, stream, CTAS, ma, mw, mu, mo, p,
+    return launch_pdl(rows_kernel<BN, CTAS, FP8, MODE, F32>, dim3(grid), rows_threads(MODE, BN, F32), RCfg<BN, CTAS, MODE, F32>::kSmemBytes, stream, CTAS, ma, mw, mu, mo, p,
                       d_error);
 }
 
@@ -962,12 +968,14 @@ cudaError_t rows_set() {
     return cudaFuncSetAttribute(rows_kernel<BN, CTAS, FP8, MODE, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, RCfg<BN, CTAS, MODE, F32>::kSmemBytes);
 }
 
-// The tiles of one form of the product: columns per tile, CTAs per tile.  A 32-bit result keeps its sums in registers, 64 a
-// thread at most, so its widest tile has 128 columns.
+// The tiles of one form of the product: columns per tile, CTAs per tile.  A 32-bit result keeps its sums in registers; 128 a thread
+// leave no room for the gathering warps, so the widest tile of such rows has 128 columns.
 template <bool FP8, int MODE>
 cudaError_t rows_pick(const RowsArgs& g, RowsTileShape t, int sm_count, int* err, cudaStream_t st) {
     if constexpr (rows_few(MODE)) t.ctas = 1;
     if (g.out_mode != kOutBf16) {
+        if constexpr (!rows_few(MODE) && !rows_gathers(MODE))
+            if (t.ctas == 2) return rows_launch_t<256, 2, FP8, MODE, true>(g, sm_count, err, st);
         switch (t.bn) {
             case 32: return rows_launch_t<32, 1, FP8, MODE, true>(g, sm_count, err, st);
             case 64: return rows_launch_t<64, 1, FP8, MODE, true>(g, sm_count, err, st);
@@ -990,7 +998,9 @@ cudaError_t rows_set_all() {
                               rows_set<32, 1, FP8, MODE, false>(), rows_set<64, 1, FP8, MODE, false>(), rows_set<128, 1, FP8, MODE, false>(),
                               rows_set<256, 1, FP8, MODE, false>()};
     if constexpr (!rows_few(MODE)) {
-        const cudaError_t pair = rows_set<256, 2, FP8, MODE, false>();
+        cudaError_t pair = rows_set<256, 2, FP8, MODE, false>();
+        if constexpr (!rows_gathers(MODE))
+            if (pair == cudaSuccess) pair = rows_set<256, 2, FP8, MODE, true>();
         if (pair != cudaSuccess) return pair;
     }
     for (cudaError_t x : e)

@@ -117,10 +117,10 @@ int main() {
     for (long M : {1L, 2L, 24L, 127L, 128L, 129L, 1000L, 13160L, 52360L, 2000000L})
         for (int N = 1; N < 5000; N = N * 5 / 4 + 1)
             for (int G : {1, 2, 31, 32, 33, 1000, 60000})
-                for (int f32 = 0; f32 < 2; ++f32)
+                for (int f32 = 0; f32 < 4; ++f32)
                     for (int sms : {20, 132, 148}) {
-                        const sb::RowsTileShape t = sb::rows_tile(M, N, G, f32 != 0, sms); const int bn = t.bn;
-                        if (t.ctas == 2 ? (f32 || bn != 256) : !(bn == 32 || bn == 64 || bn == 128 || (bn == 256 && !f32))) { std::printf("bad %ld %d %d %d\n", M, N, G, bn); return 1; }
+                        const sb::RowsTileShape t = sb::rows_tile(M, N, G, (f32 & 1) != 0, f32 > 1, sms); const int bn = t.bn;
+                        if (t.ctas == 2 ? (f32 == 3 || bn != 256) : !(bn == 32 || bn == 64 || bn == 128 || (bn == 256 && !(f32 & 1)))) { std::printf("bad %ld %d %d %d\n", M, N, G, bn); return 1; }
                         ++n;
                     }
     std::printf("%ld\n", n);

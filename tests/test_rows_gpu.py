@@ -266,6 +266,14 @@ def test_grouped_large(ctx, M, N, K, G, gather):
 
 
 @pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("mode", [1, 2])
+@pytest.mark.parametrize("sizes,N,K", [([13160], 1024, 1024), ([6000, 0, 1, 255, 7000], 1000, 640), ([1, 13000, 300], 1030, 528), ([20000], 1024, 64)])
+def test_grouped_large_in_32_bits(ctx, sizes, N, K, mode, fp8):
+    """Enough rows for tiles of 256 x 256, which keep 128 sums a thread: one and several collections, groups that end inside a tile."""
+    grouped_case(ctx, sizes, N, K, mode=mode, fp8=fp8, act=SILU, alpha=0.5, start=2, tail=9, pad_o=N % 4)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
 def test_gathered_short_tiles_over_many_turns_of_the_ring(ctx, fp8):
     """Tiles with rows for some of the gathering warps only, K of many turns of the operand ring, several tiles per CTA."""
     r = np.random.RandomState(4)
@@ -506,6 +514,16 @@ def test_a_broken_adapter_among_many_rows(ctx, mode):
     who = np.repeat(r.randint(-1, 90, 700), r.randint(1, 35, 700))
     who[5000:5600] = r.randint(-1, 90, 600)
     adapter_case(ctx, who.tolist(), 90, 16, 1024, 64, mode=mode, poison=7)
+
+
+@pytest.mark.parametrize("rank,mode", [(8, 1), (40, 2), (128, 1)])
+def test_adapters_large_in_32_bits(ctx, rank, mode):
+    """Tiles of 256 x 256 with several adapters each, one of them broken, and rows without any; off the 16-byte boundaries too."""
+    r = np.random.RandomState(rank)
+    who = np.repeat(r.randint(-1, 60, 500), r.randint(1, 60, 500))[:13100]
+    who[4000:4300] = r.randint(-1, 60, 300)
+    adapter_case(ctx, who.tolist(), 60, rank, 1024, 576, mode=mode, act=SILU, alpha=0.5, poison=7)
+    adapter_case(ctx, who.tolist(), 60, rank, 1000, 520, mode=mode, pad_a=8, pad_o=3, shift=1)
 
 
 def test_rows_without_an_adapter_equal_the_shared_product(ctx):

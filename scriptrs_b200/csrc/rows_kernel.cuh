@@ -48,8 +48,6 @@ using namespace ptx;
 
 constexpr int kBM = 128;
 constexpr int kRowBytes = 128;  // of an operand row in a stage: one swizzle row
-constexpr int kEpiWarps = 8;
-constexpr int kSlabBytes = 32 * 128;
 constexpr int kFewRows = 32, kFewPitch = kFewRows + 1;  // rows of the few-row forms; an odd pitch spreads both sides over the banks
 constexpr int kSegment = 8;     // stages (64 bf16 or 128 e4m3 columns of K each) between two collections of a 32-bit result
 
@@ -57,10 +55,23 @@ enum RowsMode : int { kGrouped = 0, kGathered = 1, kAdapters = 2, kFewAdapters =
 constexpr bool rows_few(int mode) { return mode == kFewAdapters || mode == kFewGathered; }
 constexpr bool rows_gathers(int mode) { return mode == kGathered || mode == kFewGathered; }
 
+// Parts of a tile's columns, four epilogue warps (128 rows) each.  A pair's e4m3 tile is over in half the time, so its epilogue sets the
+// pace: sixteen warps instead of eight (16384 x 4096 x 1024: 71 -> 67 us, gathered 88 -> 76, 16 groups 97 -> 87; their slabs take a
+// stage, which costs 26000 x 1024 x 4096 3 %).  bf16 gains nothing by them.
+constexpr int rows_parts(int bn, int ctas, bool fp8, bool f32) { return bn == 256 && ctas == 2 && fp8 && !f32 ? 4 : gemm_halves(bn); }
+
 // CTAS = 2: a cluster of two CTAs on 256 rows x BN columns (tcgen05 cta_group::2); each stages its own 128 rows of A and its own
 // half of the W rows.
-template <int BN, int CTAS, int MODE, bool F32>
+template <int BN, int CTAS, bool FP8, int MODE, bool F32>
 struct RCfg {
+    static constexpr int kParts = rows_parts(BN, CTAS, FP8, F32), kEpiWarps = kParts == 4 ? 16 : 8;
+    static constexpr int kPartCols = BN / kParts;
+    static constexpr int kOutCols = F32 || kPartCols < 64 ? 32 : 64;  // that a warp sends off at a time
+    static constexpr int kSlabBytes = 32 * 128;
+    // Warps more where rows are picked (gathers) or have adapters (`low`): four, 32 rows each; two beside an epilogue that keeps 128
+    // sums a thread in registers (168 registers for 12 warps, 144 for 14).
+    static constexpr int kAuxWarps = MODE == kGrouped ? 0 : (F32 && BN == 256 ? 2 : 4);
+    static constexpr int kThreads = 32 * (2 + kEpiWarps + kAuxWarps);
     // The few-row forms stage 32 rows of A.  The MMA reads 128: the others are whatever lies behind, and so are their lanes of the
     // accumulator, which nobody reads.  What that saves goes into stages: narrow tiles are paced by the weights in flight
     // (24 rows, 1024 -> 4096, no adapters, the adapters' kernel included: 9.6 -> 6.5 us).
@@ -71,7 +82,8 @@ struct RCfg {
     static constexpr int kTerms = F32 ? 3 : 1, kGroups = F32 ? 2 : 4;  // bf16 terms, blocks of columns that are held at once
     static constexpr int kLowBytes = MODE == kAdapters ? (kTerms * kGroups + 3) / 4 * kBM * kRowBytes
                                                        : (MODE == kFewAdapters ? (BN * kFewPitch * 4 + 1023) / 1024 * 1024 : 0);  // the addition, by column
-    static constexpr int kColumnBytes = 2 * BN * 4;                                // bias and column scales of the tile
+    static constexpr int kColumnSets = kParts == 4 ? 1 : 2;  // by turns, where a stage does not go for it
+    static constexpr int kColumnBytes = kColumnSets * (FP8 ? 2 : 1) * BN * 4;  // bias and column scales of a tile
     static constexpr int kIndexBytes = rows_gathers(MODE) ? kBM * 4 : 0;
     static constexpr int kBarBytes = 384;
     static constexpr int kFixedBytes = kLowBytes + kEpiWarps * kSlabBytes + kColumnBytes + kIndexBytes + kBarBytes;
@@ -79,15 +91,8 @@ struct RCfg {
     static constexpr int kSmemBytes = kStages * kStageBytes + kFixedBytes;
     static_assert(kLowBytes % 1024 == 0 && kStages >= 3 && 8 * (2 * kStages + 6) + 16 <= kBarBytes, "shared memory");
     static constexpr int kUps = kStageBytes / kBBytes;  // adapters' tiles of `up` in a stage
-    static constexpr int kHalves = gemm_halves(BN);
-    static constexpr int kHalfCols = BN / kHalves;
     static constexpr uint32_t kTmemCols = 2 * BN;
 };
-
-// Warps more where rows are picked (gathers) or have adapters (`low`): four, 32 rows each; two beside an epilogue that keeps 128 sums
-// a thread in registers (168 registers for 12 warps, 144 for 14).
-constexpr int rows_aux_warps(int mode, int bn, bool f32) { return mode == kGrouped ? 0 : (f32 && bn == 256 ? 2 : 4); }
-constexpr int rows_threads(int mode, int bn, bool f32) { return 32 * (2 + kEpiWarps + rows_aux_warps(mode, bn, f32)); }
 
 template <int BN, int CTAS, bool FP8>
 __device__ __forceinline__ uint32_t rows_idesc() {
@@ -369,22 +374,22 @@ __device__ __forceinline__ float bf16_rest(float v) {
 }
 
 template <int BN, int CTAS, bool FP8, int MODE, bool F32>
-__global__ void __launch_bounds__(rows_threads(MODE, BN, F32), 1)
+__global__ void __launch_bounds__(RCfg<BN, CTAS, FP8, MODE, F32>::kThreads, 1)
 rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_w,
             const __grid_constant__ CUtensorMap tma_up, const __grid_constant__ CUtensorMap tma_out, const RowsParams p,
             int* __restrict__ error) {
-    using C = RCfg<BN, CTAS, MODE, F32>;
+    using C = RCfg<BN, CTAS, FP8, MODE, F32>;
     constexpr int S = C::kStages;
     constexpr int kStepCols = FP8 ? 128 : 64;
     constexpr int kTerms = C::kTerms, kGroups = C::kGroups, kPhaseCols = 16 * kGroups;
-    constexpr int kAuxWarps = rows_aux_warps(MODE, BN, F32);
+    constexpr int kEpiWarps = C::kEpiWarps, kAuxWarps = C::kAuxWarps;
     // rank of this CTA in its pair (the leader, rank 0, owns the barriers that the MMAs wait on)
     const uint32_t rank = CTAS == 2 ? __shfl_sync(0xffffffffu, cluster_ctarank(), 0) : 0u;
     extern __shared__ __align__(1024) unsigned char smem_dyn[];  // the operands' swizzle wants 1024-byte boundaries
     const uint32_t base = smem_u32(smem_dyn);
     unsigned char* base_ptr = smem_dyn;
     const uint32_t a_base = base, b_base = base + C::kABytes;  // of stage 0; a stage holds its A and its W side by side
-    constexpr int kLowAt = S * C::kStageBytes, kSlabAt = kLowAt + C::kLowBytes, kColumnAt = kSlabAt + kEpiWarps * kSlabBytes;
+    constexpr int kLowAt = S * C::kStageBytes, kSlabAt = kLowAt + C::kLowBytes, kColumnAt = kSlabAt + kEpiWarps * C::kSlabBytes;
     constexpr int kIndexAt = kColumnAt + C::kColumnBytes;
     constexpr int kBarAt = kIndexAt + C::kIndexBytes;
     const uint32_t bar_base = base + kBarAt;
@@ -418,10 +423,10 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(tfull_bar(a), 1);
-            mbar_init(tempty_bar(a), 4 * C::kHalves * CTAS);
+            mbar_init(tempty_bar(a), 4 * C::kParts * CTAS);
         }
         mbar_init(low_bar, std::max(kAuxWarps, 1) * CTAS);
-        mbar_init(lowfree_bar, MODE == kFewAdapters ? C::kHalves : 1);
+        mbar_init(lowfree_bar, MODE == kFewAdapters ? C::kParts : 1);
         *abort_flag = 0;
         rows_set_turn(turn_at, 0);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -606,41 +611,45 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
         }
     } else if (warp < 2 + kEpiWarps) {
         // ------------------------------------------------------------ epilogue
-        const int ew = warp - 2, quad = warp & 3, half = ew >> 2;
-        unsigned char* slab = base_ptr + kSlabAt + ew * kSlabBytes;
-        uint32_t seg = 0, tiles = 0;
+        const int ew = warp - 2, quad = warp & 3, part = ew >> 2;
+        unsigned char* slab = base_ptr + kSlabAt + ew * C::kSlabBytes;
+        uint32_t seg = 0;
         bool ok = true;
-        const int cbeg = half * C::kHalfCols;
-        float* columns = reinterpret_cast<float*>(base_ptr + kColumnAt) + cbeg;  // bias; the scales BN further on
-        // the four warps of a half bring in its columns' bias and scales, fetched a tile ahead
+        const int cbeg = part * C::kPartCols;
+        float* columns = reinterpret_cast<float*>(base_ptr + kColumnAt) + cbeg;  // bias of this tile; the scales 2 BN further on
+        // the four warps of a part bring in its columns' bias and scales, fetched a tile ahead
         float next_bias = 0.0f, next_scale = 1.0f;
         auto fetch_columns = [&](const RowsTile& at) {
             const int c = quad * 32 + lane, col = at.col0 + cbeg + c;
-            const bool in = c < C::kHalfCols && col < p.N;
+            const bool in = c < C::kPartCols && col < p.N;
             next_bias = p.bias && in ? __ldg(p.bias + (int64_t)at.group * p.N + col) : 0.0f;
             if (FP8) next_scale = p.col_scale && in ? __ldg(p.col_scale + (int64_t)at.group * p.N + col) : 1.0f;
         };
-        static_assert(C::kHalfCols <= 128, "a thread brings in one column");
-        auto half_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory"); };
-        bool more = half < C::kHalves && walk.find(tile0, BN, tile);
+        static_assert(C::kPartCols <= 128, "a thread brings in one column");
+        uint32_t tiles = 0;
+        auto next_columns = [&]() { return reinterpret_cast<float*>(base_ptr + kColumnAt) + cbeg + (C::kColumnSets == 2 ? (tiles & 1) * BN : 0); };
+        bool more = part < C::kParts && walk.find(tile0, BN, tile);
         RowsTile ahead;
         if (more) fetch_columns(tile);
-        for (long long t = tile0; more; t += tile_step, tile = ahead) {
-            // the tile before has been read; where a wait ran out in one of the four warps, all of them leave here
-            uint32_t all_ok;
-            asm volatile(
-                "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %2, 0;\n\t"
-                "barrier.cta.red.and.pred p, %1, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                : "=r"(all_ok)
-                : "r"(1 + half), "r"(ok ? 1u : 0u)
-                : "memory");
-            ok = all_ok != 0;
-            if (!ok) break;
-            if (quad * 32 + lane < C::kHalfCols) {
+        for (long long t = tile0; more; t += tile_step, tile = ahead, columns = next_columns()) {
+            // Where a wait ran out in one of the four warps, all of them leave here.
+            auto meet = [&]() {
+                uint32_t all_ok;
+                asm volatile(
+                    "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %2, 0;\n\t"
+                    "barrier.cta.red.and.pred p, %1, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                    : "=r"(all_ok)
+                    : "r"(1 + part), "r"(ok ? 1u : 0u)
+                    : "memory");
+                ok = all_ok != 0;
+            };
+            if (C::kColumnSets == 1) meet();  // the tile before has been read (of two sets: the tile before the last, its readers met since)
+            if (quad * 32 + lane < C::kPartCols) {
                 columns[quad * 32 + lane] = next_bias;
-                if (FP8) columns[BN + quad * 32 + lane] = next_scale;
+                if (FP8) columns[C::kColumnSets * BN + quad * 32 + lane] = next_scale;
             }
-            half_sync();
+            meet();
+            if (!ok) break;
             more = walk.find(t + tile_step, BN, ahead);
             if (more) fetch_columns(ahead);
             const int row0 = tile.row0 + cta_row + quad * 32;  // of this warp
@@ -692,7 +701,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                 __syncwarp();
             };
             if constexpr (F32) {
-                constexpr int kCols = C::kHalfCols;
+                constexpr int kCols = C::kPartCols;
                 float sum[kCols];
 #pragma unroll
                 for (int j = 0; j < kCols; ++j) sum[j] = 0.0f;
@@ -725,7 +734,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                     float x[32];
 #pragma unroll
                     for (int j = 0; j < 32; ++j) x[j] = sum[c + j];
-                    rows_finish<FP8, F32>(x, p, reinterpret_cast<const float4*>(columns + c), reinterpret_cast<const float4*>(columns + BN + c), rs, known);
+                    rows_finish<FP8, F32>(x, p, reinterpret_cast<const float4*>(columns + c), reinterpret_cast<const float4*>(columns + C::kColumnSets * BN + c), rs, known);
                     ready();
 #pragma unroll
                     for (int q = 0; q < 8; ++q)
@@ -734,7 +743,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                     leave(col0, 32, [&]() { rows_store<float, 32>(slab, p, row0, tile.row1, col0, lane); });
                 }
             } else {
-                constexpr int kCols = C::kHalfCols < 64 ? C::kHalfCols : 64;
+                constexpr int kCols = C::kOutCols;
                 constexpr int kShift = kCols == 32 ? 1 : 0, kMask = kCols / 8 - 1;
                 ok = __all_sync(0xffffffffu, mbar_wait(tfull_bar(seg & 1), (seg >> 1) & 1, abort_flag));
                 if (!ok) continue;
@@ -742,16 +751,15 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                 bool held = true;
                 if (any) {
 #pragma unroll 1
-                    for (int c = 0; c < C::kHalfCols; c += kCols) {
+                    for (int c = 0; c < C::kPartCols; c += kCols) {
                         const int col0 = tile.col0 + cbeg + c;
                         if (col0 >= p.N) break;
-                        uint32_t packed[kCols / 2];
 #pragma unroll
                         for (int sub = 0; sub < kCols / 32; ++sub) {
                             uint32_t v[32];
                             tmem_ld32(taddr() + c + 32 * sub, v);
                             tmem_wait_ld();
-                            if (c + 32 * (sub + 1) >= C::kHalfCols) {  // the accumulator is free for the tile after the next
+                            if (c + 32 * (sub + 1) >= C::kPartCols) {  // the accumulator is free for the tile after the next
                                 release();
                                 held = false;
                             }
@@ -763,15 +771,14 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                                 for (int j = 0; j < 32; ++j) x[j] += addition[(cbeg + c + 32 * sub + j) * kFewPitch];
                             }
                             rows_finish<FP8, F32>(x, p, reinterpret_cast<const float4*>(columns + c + 32 * sub),
-                                                  reinterpret_cast<const float4*>(columns + BN + c + 32 * sub), rs, known);
+                                                  reinterpret_cast<const float4*>(columns + C::kColumnSets * BN + c + 32 * sub), rs, known);
+                            if (sub == 0) ready();
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) packed[16 * sub + j] = pack_bf16(x[2 * j], x[2 * j + 1]);
+                            for (int q = 0; q < 4; ++q)
+                                *reinterpret_cast<uint4*>(slab + lane * (kCols * 2) + (((4 * sub + q) ^ ((lane >> kShift) & kMask)) << 4)) =
+                                    make_uint4(pack_bf16(x[8 * q], x[8 * q + 1]), pack_bf16(x[8 * q + 2], x[8 * q + 3]),
+                                               pack_bf16(x[8 * q + 4], x[8 * q + 5]), pack_bf16(x[8 * q + 6], x[8 * q + 7]));
                         }
-                        ready();
-#pragma unroll
-                        for (int q = 0; q < kCols / 8; ++q)
-                            *reinterpret_cast<uint4*>(slab + lane * (kCols * 2) + ((q ^ ((lane >> kShift) & kMask)) << 4)) =
-                                make_uint4(packed[4 * q], packed[4 * q + 1], packed[4 * q + 2], packed[4 * q + 3]);
                         leave(col0, kCols, [&]() { rows_store<__nv_bfloat16, kCols>(slab, p, row0, tile.row1, col0, lane); });
                     }
                 }
@@ -940,7 +947,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
 template <int BN, int CTAS, bool FP8, int MODE, bool F32>
 cudaError_t rows_launch_t(const RowsArgs& g, int sm_count, int* d_error, cudaStream_t stream) {
     alignas(64) CUtensorMap ma, mw, mu, mo;
-    if (!rows_map(&ma, g.a, g.a_rows, g.K, g.lda, FP8, rows_gathers(MODE) ? 1 : RCfg<BN, CTAS, MODE, F32>::kABytes / kRowBytes) ||
+    if (!rows_map(&ma, g.a, g.a_rows, g.K, g.lda, FP8, rows_gathers(MODE) ? 1 : RCfg<BN, CTAS, FP8, MODE, F32>::kABytes / kRowBytes) ||
         !rows_map(&mw, g.w, (int64_t)g.n_groups * g.N, g.K, g.K, FP8, BN / CTAS))
         return cudaErrorInvalidValue;
     mu = mw;
@@ -953,19 +960,19 @@ cudaError_t rows_launch_t(const RowsArgs& g, int sm_count, int* d_error, cudaStr
     p.out_vec = !(reinterpret_cast<uintptr_t>(g.out) & 15) && !((g.ldo * eb) & 15);
     p.n_vec = (int64_t)g.N * eb % 16 == 0;
     mo = mw;  // stores by TMA want 32 rows of a group
-    if (p.out_vec && g.M >= 32 && !rows_out_map(&mo, g.out, g.M, g.N, g.ldo, F32, F32 || RCfg<BN, CTAS, MODE, F32>::kHalfCols >= 64 ? 128 : 64)) return cudaErrorInvalidValue;
+    if (p.out_vec && g.M >= 32 && !rows_out_map(&mo, g.out, g.M, g.N, g.ldo, F32, F32 || RCfg<BN, CTAS, FP8, MODE, F32>::kOutCols == 64 ? 128 : 64)) return cudaErrorInvalidValue;
     p.row_adapter = g.row_adapter; p.low = g.low; p.up = g.up; p.rank = g.rank; p.n_adapters = g.n_adapters;
     // at most this many tiles: a group's last one may be short
     const int64_t n_tiles = (g.N + BN - 1) / BN;
     const int64_t tiles = ((int64_t)(g.M + kBM * CTAS - 1) / (kBM * CTAS) + std::min(g.n_groups - 1, g.M)) * n_tiles;
     const int grid = CTAS * (int)std::min<int64_t>(tiles, sm_count / CTAS);
-    return launch_pdl(rows_kernel<BN, CTAS, FP8, MODE, F32>, dim3(grid), rows_threads(MODE, BN, F32), RCfg<BN, CTAS, MODE, F32>::kSmemBytes, stream, CTAS, ma, mw, mu, mo, p,
+    return launch_pdl(rows_kernel<BN, CTAS, FP8, MODE, F32>, dim3(grid), RCfg<BN, CTAS, FP8, MODE, F32>::kThreads, RCfg<BN, CTAS, FP8, MODE, F32>::kSmemBytes, stream, CTAS, ma, mw, mu, mo, p,
                       d_error);
 }
 
 template <int BN, int CTAS, bool FP8, int MODE, bool F32>
 cudaError_t rows_set() {
-    return cudaFuncSetAttribute(rows_kernel<BN, CTAS, FP8, MODE, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, RCfg<BN, CTAS, MODE, F32>::kSmemBytes);
+    return cudaFuncSetAttribute(rows_kernel<BN, CTAS, FP8, MODE, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, RCfg<BN, CTAS, FP8, MODE, F32>::kSmemBytes);
 }
 
 // The tiles of one form of the product: columns per tile, CTAs per tile.  A 32-bit result keeps its sums in registers; 128 a thread

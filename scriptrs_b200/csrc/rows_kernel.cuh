@@ -7,7 +7,7 @@
 //   - The tiles are found on the device.  A tile belongs to one group: 128 consecutive rows of it per CTA (the last ones of a
 //     group may be missing) times BN columns.  Every warp walks the offsets 128 groups at a time with a prefix sum over its
 //     lanes, so no table of groups is kept and the host never learns the sizes.
-//   - Rows picked by an index arrive by TMA gathers of four rows each, issued by four warps (32 rows each) from one elected
+//   - Rows picked by an index arrive by TMA gathers of four rows each, issued by four or eight warps from one elected
 //     lane (from every lane by turns a gather takes ten times as long); a tile with few rows fetches only those.
 //   - Rows leave through a swizzled slab per warp: 32 rows of one group by a TMA store (or reduce-add), which clips at column N;
 //     the last rows of a group, behind which its neighbour's begin, results off the 16-byte boundaries, and the last columns where N
@@ -69,8 +69,9 @@ struct RCfg {
     static constexpr int kOutCols = F32 || kPartCols < 64 ? 32 : 64;  // that a warp sends off at a time
     static constexpr int kSlabBytes = 32 * 128;
     // Warps more where rows are picked (gathers) or have adapters (`low`): four, 32 rows each; two beside an epilogue that keeps 128
-    // sums a thread in registers (168 registers for 12 warps, 144 for 14).
-    static constexpr int kAuxWarps = MODE == kGrouped ? 0 : (F32 && BN == 256 ? 2 : 4);
+    // sums a thread in registers (168 registers for 12 warps, 144 for 14); eight for the gathers of bf16 results, which four warps only
+    // just issue in a stage's time (16384 x 4096 x 1024: 110 -> 106 us, 8064 rows of 16 groups 77 -> 71), where registers allow.
+    static constexpr int kAuxWarps = MODE == kGrouped ? 0 : (F32 && BN == 256 ? 2 : (MODE == kGathered && kEpiWarps == 8 && !F32 ? 8 : 4));
     static constexpr int kThreads = 32 * (2 + kEpiWarps + kAuxWarps);
     // The few-row forms stage 32 rows of A.  The MMA reads 128: the others are whatever lies behind, and so are their lanes of the
     // accumulator, which nobody reads.  What that saves goes into stages: narrow tiles are paced by the weights in flight
@@ -789,29 +790,38 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
         if (elect_one()) bulk_wait_all();
         __syncwarp();
     } else if constexpr (rows_gathers(MODE)) {
-        // ------------------------------------------------------------ gathers, 32 rows a warp
+        // ------------------------------------------------------------ gathers, kGatherRows rows a warp
+        constexpr int kGatherRows = kBM / kAuxWarps;
         const int gw = warp - 2 - kEpiWarps;
-        int32_t* index = reinterpret_cast<int32_t*>(base_ptr + kIndexAt) + gw * 32;
+        int32_t* index = reinterpret_cast<int32_t*>(base_ptr + kIndexAt) + gw * kGatherRows;
         uint32_t begun = 0;
         bool ok = true;
-        for (long long t = tile0; ok && walk.find(t, BN, tile); t += tile_step, begun += k_tiles) {
-            const int first = tile.row0 + cta_row + gw * 32, count = tile.row1 - first;
+        int next = 0;  // the index of this lane's row, fetched a tile ahead
+        auto fetch_index = [&](const RowsTile& at) {
+            const int i = min(at.row0 + cta_row + gw * kGatherRows + (lane % kGatherRows), at.row1 - 1);
+            next = p.rows ? __ldg(p.rows + i) : i;
+        };
+        bool more = walk.find(tile0, BN, tile);
+        RowsTile ahead;
+        if (more) fetch_index(tile);
+        for (long long t = tile0; ok && more; t += tile_step, tile = ahead, begun += k_tiles) {
+            const int count = tile.row1 - (tile.row0 + cta_row + gw * kGatherRows), v = next;
+            more = walk.find(t + tile_step, BN, ahead);
+            if (more) fetch_index(ahead);
             if (count <= 0) continue;
-            const int i = min(first + lane, tile.row1 - 1);
-            const int v = p.rows ? __ldg(p.rows + i) : i;
-            index[lane] = (unsigned)v < (unsigned long long)p.a_rows ? v : 0;
+            if (lane < kGatherRows) index[lane] = (unsigned)v < (unsigned long long)p.a_rows ? v : 0;
             __syncwarp();
             bool failed = false;
             if (elect_one()) {
-                int4 r[8];
+                int4 r[kGatherRows / 4];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) r[j] = reinterpret_cast<const int4*>(index)[j];
+                for (int j = 0; j < kGatherRows / 4; ++j) r[j] = reinterpret_cast<const int4*>(index)[j];
                 int s = (int)(begun % S);
                 for (int kt = 0; kt < k_tiles; ++kt) {
                     if (!rows_wait_turn(turn_at, begun + (uint32_t)kt + 1, abort_flag)) { failed = true; break; }
-                    const uint32_t dst = a_base + s * C::kStageBytes + gw * 32 * kRowBytes, bar = lead(full_bar(s));
+                    const uint32_t dst = a_base + s * C::kStageBytes + gw * kGatherRows * kRowBytes, bar = lead(full_bar(s));
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
+                    for (int j = 0; j < kGatherRows / 4; ++j)
                         if (4 * j < count) tma_gather4<CTAS>(dst + j * 4 * kRowBytes, &tma_a, bar, kt * kStepCols, r[j].x, r[j].y, r[j].z, r[j].w);
                     if (++s == S) s = 0;
                 }

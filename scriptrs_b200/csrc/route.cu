@@ -31,10 +31,7 @@ int route_block_rows(int64_t rows) {
 int64_t route_blocks(int64_t rows) { return (rows + route_block_rows(rows) - 1) / route_block_rows(rows); }
 
 // What a logit counts as: NaN as -inf, which is never chosen, +inf as the largest finite value of its type.
-template <typename T>
-__device__ __forceinline__ float route_logit(float x) {
-    return fminf(fmaxf(x, -INFINITY), sizeof(T) == 2 ? __uint_as_float(0x7f7f0000u) : FLT_MAX);
-}
+__device__ __forceinline__ float route_logit(float x) { return fminf(fmaxf(x, -INFINITY), FLT_MAX); }
 // Order-preserving image of a float (-0 as 0); below kRouteNone: -inf.
 constexpr uint32_t kRouteNone = 0x00800000u;
 __device__ __forceinline__ uint32_t route_key(float x) {
@@ -47,68 +44,148 @@ __device__ __forceinline__ float route_value(uint32_t k) {
 // exp(x) for x <= 0: the argument's rounding is 2^-24 of it, the function's error 2^-22, and what counts lies near 0.
 __device__ __forceinline__ float route_exp(float x) { return ptx::ex2_approx(x * 1.44269504f); }
 
+// the largest of key - below (mod 2^32) over the row
+template <int LANES, int PER>
+__device__ __forceinline__ uint32_t route_most(const uint32_t (&key)[PER], uint32_t below) {
+    uint32_t m = key[0] - below;
+#pragma unroll
+    for (int i = 1; i < PER; ++i) m = __viaddmax_u32(key[i], 0u - below, m);
+#pragma unroll
+    for (int d = LANES / 2; d; d >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+    return m;
+}
+template <int LANES>
+__device__ __forceinline__ float route_sum(float v) {
+#pragma unroll
+    for (int d = LANES / 2; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    return v;
+}
+
 // LANES lanes take a row, PER neighbouring experts each, in registers.  A round finds the largest key below the one before as the
 // maximum of key - previous in unsigned arithmetic: what lies below wraps round to the top, nearest first.
 //   bf16: a key is 16 bits, the expert (counted down) takes the other 16: keys differ and a round yields one choice.
 //   f32:  a round yields a value; the experts that have it follow in ascending order.
 // `live`: the row exists (its lanes take part in the shuffles either way).
-template <int LANES, int PER, typename T>
-__device__ __forceinline__ void route_row(const RouteArgs& p, int row, bool live, int lane, int16_t* chosen) {
-    constexpr bool kPacked = sizeof(T) == 2;
+// Bound by issue slots, so for bf16 the keys are made two at a time, NaN and +inf are looked at only where a row's largest key says that
+// there are some, and a choice is turned back into its value once, by the lane that keeps it (52360 rows of 128, 4 each: 15 -> 11 us).
+template <int LANES, int PER>
+__device__ __forceinline__ void route_row(const RouteArgs& p, int row, bool live, int lane, int16_t* chosen, const __nv_bfloat16* logits) {
+    const int l = lane % LANES;
+    uint32_t w[PER / 2], key[PER];
+#pragma unroll
+    for (int i = 0; i < PER / 2; ++i) w[i] = 0xff80ff80u;  // -inf
+    const unsigned short* x = reinterpret_cast<const unsigned short*>(logits) + (int64_t)row * p.ld + l * PER;
+    const int mine = p.n_experts - l * PER;  // experts from this lane's first on
+    if (p.vec) {
+#pragma unroll
+        for (int i = 0; i < PER; i += 8) {
+            if (!live || i >= mine) continue;
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(x + i));
+            w[i / 2] = v.x; w[i / 2 + 1] = v.y; w[i / 2 + 2] = v.z; w[i / 2 + 3] = v.w;
+        }
+    } else if (live) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (i < mine) w[i / 2] = i % 2 ? (w[i / 2] & 0xffffu) | ((uint32_t)__ldg(x + i) << 16) : (w[i / 2] & 0xffff0000u) | __ldg(x + i);
+    }
+#pragma unroll
+    for (int i = 0; i < PER / 2; ++i) {
+        // -0 as 0; then a negative value's bits are inverted, the others' sign set
+        asm("{\n\t.reg .b32 z, n;\n\tmov.b32 z, 0;\n\tadd.rn.bf16x2 %0, %0, z;\n\tprmt.b32 n, %0, z, 0xBB99;\n\tor.b32 n, n, 0x80008000;\n\txor.b32 %1, %0, n;\n\t}"
+            : "+r"(w[i]), "=r"(key[2 * i]));
+        key[2 * i + 1] = (key[2 * i] & 0xffff0000u) | (0xffffu - (uint32_t)(l * PER + 2 * i + 1));
+        key[2 * i] = (key[2 * i] << 16) | (0xffffu - (uint32_t)(l * PER + 2 * i));
+    }
+    uint32_t first = route_most<LANES>(key, 0u);
+    if (__any_sync(0xffffffffu, first >= 0xff800000u)) {  // +inf (counts as the largest finite value) or, above it, NaN (as -inf)
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            if (key[i] < 0xff800000u) continue;
+            const bool nan = key[i] >= 0xff810000u;
+            key[i] = (key[i] & 0xffffu) | (nan ? 0u : 0xff7f0000u);
+            const uint32_t as = nan ? 0xff80u : 0x7f7fu;
+            w[i / 2] = i % 2 ? (w[i / 2] & 0xffffu) | (as << 16) : (w[i / 2] & 0xffff0000u) | as;
+        }
+        first = route_most<LANES>(key, 0u);
+    }
+    // a key's lower half stands for the zeros of a bf16 value, inverted where it is negative
+    auto value = [](uint32_t k) { return route_value((k & 0xffff0000u) | ((k & 0x80000000u) ? 0u : 0xffffu)); };
+    const float top = first >= kRouteNone ? value(first) : 0.0f;
+    float total = 0.0f;
+    if (!p.normalize) {
+#pragma unroll
+        for (int i = 0; i < PER / 2; ++i)
+            total += route_exp(__uint_as_float(w[i] << 16) - top) + route_exp(__uint_as_float(w[i] & 0xffff0000u) - top);
+        total = route_sum<LANES>(total);
+    }
+    constexpr int kKeep = (kMaxTopK + LANES - 1) / LANES;  // lane l keeps the choices l, l + LANES, ...
+    uint32_t kept[kKeep];
+#pragma unroll
+    for (int i = 0; i < kKeep; ++i) kept[i] = 0u;
+    uint32_t best = first;
+    for (int j = 0;; ++j) {
+#pragma unroll
+        for (int i = 0; i < kKeep; ++i)
+            if (l + i * LANES == j) kept[i] = best;
+        if (j + 1 == p.top_k) break;
+        const uint32_t next = route_most<LANES>(key, best) + best;  // shuffles: by every lane, its row over or not
+        best = best >= kRouteNone ? next : 0u;
+    }
+    float weight[kKeep];
+#pragma unroll
+    for (int i = 0; i < kKeep; ++i) weight[i] = kept[i] >= kRouteNone ? route_exp(value(kept[i]) - top) : 0.0f;
+    if (p.normalize) {
+#pragma unroll
+        for (int i = 0; i < kKeep; ++i) total += weight[i];
+        total = route_sum<LANES>(total);
+    }
+    if (!live) return;
+    const int64_t out = (int64_t)row * p.top_k;
+#pragma unroll
+    for (int i = 0; i < kKeep; ++i) {
+        const int j = l + i * LANES;
+        if (j >= p.top_k) break;
+        const int who = kept[i] >= kRouteNone ? (int)(0xffffu - (kept[i] & 0xffffu)) : -1;
+        p.experts[out + j] = who;
+        p.weights[out + j] = who >= 0 ? __fdividef(weight[i], total) : 0.0f;  // 1 <= total <= 1024
+        chosen[j] = (int16_t)who;
+    }
+}
+
+template <int LANES, int PER>
+__device__ __forceinline__ void route_row(const RouteArgs& p, int row, bool live, int lane, int16_t* chosen, const float* logits) {
     const int l = lane % LANES;
     uint32_t key[PER];
     float total = 0.0f, top;
     uint32_t first;
-    // the largest of key - below (mod 2^32) over the row
-    auto most = [&](uint32_t below) {
-        uint32_t m = key[0] - below;
-#pragma unroll
-        for (int i = 1; i < PER; ++i) m = __viaddmax_u32(key[i], 0u - below, m);
-#pragma unroll
-        for (int d = LANES / 2; d; d >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
-        return m;
-    };
-    // a packed key's lower half stands for the zeros of a bf16 value, inverted where it is negative
-    auto value = [](uint32_t k) {
-        if (kPacked) k = (k & 0xffff0000u) | ((k & 0x80000000u) ? 0u : 0xffffu);
-        return route_value(k);
-    };
     {
         float f[PER];
 #pragma unroll
         for (int i = 0; i < PER; ++i) f[i] = -INFINITY;
-        const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.ld;
-        constexpr int kVec = 16 / (int)sizeof(T);
-        if (PER % kVec == 0 && p.vec) {
+        const float* x = logits + (int64_t)row * p.ld;
+        if (PER % 4 == 0 && p.vec) {
 #pragma unroll
-            for (int i = 0; i < PER; i += kVec) {
+            for (int i = 0; i < PER; i += 4) {
                 if (!live || l * PER + i >= p.n_experts) continue;
-                const uint4 v = __ldg(reinterpret_cast<const uint4*>(x + l * PER + i));
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int j = 0; j < kVec; ++j) {
-                    if constexpr (kPacked) f[(i + j) % PER] = __uint_as_float(j % 2 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
-                    else f[(i + j) % PER] = __uint_as_float(w[j]);
-                }
+                const float4 v = __ldg(reinterpret_cast<const float4*>(x + l * PER + i));
+                f[i] = v.x; f[i + 1] = v.y; f[i + 2] = v.z; f[i + 3] = v.w;
             }
         } else if (live) {
 #pragma unroll
             for (int i = 0; i < PER; ++i)
-                if (l * PER + i < p.n_experts) f[i] = (float)x[l * PER + i];
+                if (l * PER + i < p.n_experts) f[i] = x[l * PER + i];
         }
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            f[i] = route_logit<T>(f[i]);
+            f[i] = route_logit(f[i]);
             key[i] = route_key(f[i]);
-            if (kPacked) key[i] = (key[i] & 0xffff0000u) | (0xffffu - (uint32_t)(l * PER + i));
         }
-        first = most(0u);
-        top = first >= kRouteNone ? value(first) : 0.0f;
+        first = route_most<LANES>(key, 0u);
+        top = first >= kRouteNone ? route_value(first) : 0.0f;
         if (!p.normalize) {
 #pragma unroll
             for (int i = 0; i < PER; ++i) total += route_exp(f[i] - top);
-#pragma unroll
-            for (int d = LANES / 2; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+            total = route_sum<LANES>(total);
         }
     }
     constexpr int kKeep = (kMaxTopK + LANES - 1) / LANES;  // lane l keeps the choices l, l + LANES, ...
@@ -123,36 +200,28 @@ __device__ __forceinline__ void route_row(const RouteArgs& p, int row, bool live
             if (l + i * LANES == j) { mine[i] = w; who[i] = e; }
     };
     uint32_t best = first;
-    if constexpr (kPacked) {
-        for (int j = 0; j < p.top_k; ++j) {
-            if (best >= kRouteNone) keep(j, route_exp(value(best) - top), (int)(0xffffu - (best & 0xffffu)));
-            const uint32_t next = most(best) + best;  // shuffles: by every lane, its row over or not
-            best = best >= kRouteNone ? next : 0u;
-        }
-    } else {
-        const int group0 = lane / LANES * LANES;
-        int j = 0;
-        while (__any_sync(0xffffffffu, best >= kRouteNone && j < p.top_k)) {
-            uint32_t has = 0;  // this lane's experts with that value
+    const int group0 = lane / LANES * LANES;
+    int j = 0;
+    while (__any_sync(0xffffffffu, best >= kRouteNone && j < p.top_k)) {
+        uint32_t has = 0;  // this lane's experts with that value
 #pragma unroll
-            for (int i = 0; i < PER; ++i) has |= key[i] == best ? 1u << i : 0u;
-            if (best < kRouteNone) has = 0;
-            const float w = best >= kRouteNone ? route_exp(value(best) - top) : 0.0f;
-            while (true) {
-                const uint32_t lanes = (__ballot_sync(0xffffffffu, has != 0) >> group0) & (LANES == 32 ? 0xffffffffu : (1u << LANES) - 1u);
-                const bool go = lanes && j < p.top_k;
-                if (!__any_sync(0xffffffffu, go)) break;
-                const int from = group0 + (lanes ? __ffs(lanes) - 1 : 0);
-                const int at = __shfl_sync(0xffffffffu, l * PER + __ffs(has) - 1, from);
-                if (go) {
-                    keep(j, w, at);
-                    ++j;
-                    if (lane == from) has &= has - 1;
-                }
+        for (int i = 0; i < PER; ++i) has |= key[i] == best ? 1u << i : 0u;
+        if (best < kRouteNone) has = 0;
+        const float w = best >= kRouteNone ? route_exp(route_value(best) - top) : 0.0f;
+        while (true) {
+            const uint32_t lanes = (__ballot_sync(0xffffffffu, has != 0) >> group0) & (LANES == 32 ? 0xffffffffu : (1u << LANES) - 1u);
+            const bool go = lanes && j < p.top_k;
+            if (!__any_sync(0xffffffffu, go)) break;
+            const int from = group0 + (lanes ? __ffs(lanes) - 1 : 0);
+            const int at = __shfl_sync(0xffffffffu, l * PER + __ffs(has) - 1, from);
+            if (go) {
+                keep(j, w, at);
+                ++j;
+                if (lane == from) has &= has - 1;
             }
-            const uint32_t next = most(best) + best;
-            best = best >= kRouteNone ? next : 0u;
         }
+        const uint32_t next = route_most<LANES>(key, best) + best;
+        best = best >= kRouteNone ? next : 0u;
     }
     if (!live) return;
     const int64_t out = (int64_t)row * p.top_k;
@@ -248,7 +317,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_choose_kernel(const Route
     constexpr int kPer = 32 / LANES;  // rows of a warp at once
     for (int r0 = warp * kPer; r0 < rows; r0 += kRouteWarps * kPer) {
         const int r = r0 + lane / LANES;
-        route_row<LANES, PER, T>(p, row0 + r, r < rows, lane, chosen + min(r, rows - 1) * p.top_k);
+        route_row<LANES, PER>(p, row0 + r, r < rows, lane, chosen + min(r, rows - 1) * p.top_k, static_cast<const T*>(p.logits));
     }
     __syncthreads();
     const int n = rows * p.top_k;

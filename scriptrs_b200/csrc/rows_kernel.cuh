@@ -267,6 +267,15 @@ struct TileWalk {
     }
 };
 
+// x sigmoid(x), its relative error a few 2^-22 on either side of 0 and 2^-23 |x| by the exponential's argument; 0 below -87, where the
+// result is under 2^-118.  The exponential of -|x| does not overflow and the divisor lies in [1, 2].  (Through one tanh, x / 2 (1 + tanh),
+// the sum cancels where x is negative: 1 % of the result at -4, 70 % at -8.  13160 rows x 4096 x 1024 took 80 us then and take 84, in
+// e4m3 58 and 63.)
+__device__ __forceinline__ float rows_silu(float x) {
+    const float e = ex2_approx(-1.44269504f * fabsf(x));
+    return (x < 0.0f ? x * e : x) * rcp_approx(1.0f + e);
+}
+
 // 32 accumulator columns -> scales, bias, activation.  bias, scale: of these columns, in shared memory.  (From global memory the
 // same loads cost a trip to L2 every 32 columns even where they had been touched before: 28 us of 75 in a product of 16384 x 4096
 // with K = 64; handed round by shuffles 7 us, but as many again for the scales.)
@@ -292,7 +301,7 @@ __device__ __forceinline__ void rows_finish(float (&x)[32], const RowsParams& p,
     }
     if (p.act == kActSilu) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) x[j] = F32 ? __fdividef(x[j], 1.0f + __expf(-x[j])) : silu_fast(x[j]);
+        for (int j = 0; j < 32; ++j) x[j] = rows_silu(x[j]);
     } else if (p.act == kActRelu) {
 #pragma unroll
         for (int j = 0; j < 32; ++j) x[j] = x[j] < 0.0f ? 0.0f : x[j];  // NaN stays

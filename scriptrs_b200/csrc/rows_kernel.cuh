@@ -13,9 +13,9 @@
 //     the last rows of a group, behind which its neighbour's begin, results off the 16-byte boundaries, and the last columns where N
 //     ends inside 16 bytes (the store clips at whole ones) by ordinary stores.
 //   - The low-rank addition is K = rank more columns of the same product, accumulated in the same tensor memory, `low` against the
-//     rows of U_a.  Where the result is bf16, `low` is rounded to bf16 too, as between any two bf16 products: at most 2^-8 of
-//     |low| |U_a|, as the result's own rounding is 2^-8 of the result (a second term, 2^-16, took 13 % of the product's time at
-//     rank 64 with two adapters a tile).  Where the result is stored in 32 bits it enters as three bf16 terms (2^-24).
+//     rows of U_a, as bf16 terms: two where the result is bf16 (an error of at most 2^-16 of |low| |U_a|, below the result's own rounding
+//     even where the addition cancels in part; one term, 2^-8, takes 5 % less, 448 against 472 us for 52360 rows x 4096 x 1024 at rank
+//     64 with two adapters a tile, but a row's numbers then depend on whether its call has more than 32 rows), three where it is stored in 32 bits (2^-24).
 //     A tile may hold rows of several adapters: its MMAs run once for each, with the lanes of the other rows disabled, so that
 //     nothing of one adapter (not even a NaN) reaches rows of another, and the shared weights are read once whatever the adapters.
 //   - Up to 32 rows (live streams, as a rule each with an adapter of its own): an MMA per adapter would take longer than all of
@@ -80,7 +80,7 @@ struct RCfg {
     static constexpr int kBBytes = BN / CTAS * kRowBytes;
     static constexpr int kStageBytes = kABytes + kBBytes;
     // `low` of the tile's rows as an operand: blocks of 16 of its columns (32 bytes a row), four to an operand tile
-    static constexpr int kTerms = F32 ? 3 : 1, kGroups = F32 ? 2 : 4;  // bf16 terms, blocks of columns that are held at once
+    static constexpr int kTerms = F32 ? 3 : 2, kGroups = F32 ? 2 : 4;  // bf16 terms, blocks of columns that are held at once
     static constexpr int kLowBytes = MODE == kAdapters ? (kTerms * kGroups + 3) / 4 * kBM * kRowBytes
                                                        : (MODE == kFewAdapters ? (BN * kFewPitch * 4 + 1023) / 1024 * 1024 : 0);  // the addition, by column
     static constexpr int kColumnSets = kParts == 4 ? 1 : 2;  // by turns, where a stage does not go for it
@@ -937,10 +937,8 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
                                 float& x = f[16 * g + 2 * i];
                                 float& y = f[16 * g + 2 * i + 1];
                                 w[i] = pack_bf16(x, y);
-                                if (kTerms > 1) {
-                                    x = bf16_rest(x);
-                                    y = bf16_rest(y);
-                                }
+                                x = bf16_rest(x);
+                                y = bf16_rest(y);
                             }
                             const int at = g * kTerms + e, chunk = 2 * (at % 4);
                             unsigned char* d = dst + at / 4 * kBM * kRowBytes;

@@ -76,3 +76,69 @@ def test_silu_beside_adapters(ctx, M, mode):
                     d_bias=x.data_ptr(), act=SILU, out_mode=mode)
     ctx.synchronize()
     silu_check(out, x, mode)
+
+
+# ------------------------------------------------------------------------------------------------------------ adapters
+def adapters_alone(ctx, a, down, up, who, mode):
+    """The addition by itself, beside shared weights of zero."""
+    import scriptrs_b200 as sb
+
+    (M, K), (n, N, r) = a.shape, up.shape
+    w = torch.zeros(N, K, device="cuda").bfloat16()
+    out = torch.full((M, N), 3.0, device="cuda", dtype=torch.float32 if mode else torch.bfloat16)
+    size = sb.adapter_gemm_workspace(M, r)
+    work = torch.full((size,), 0xff, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    sb.adapter_gemm(ctx, a.data_ptr(), w.data_ptr(), down.data_ptr(), up.data_ptr(), who.data_ptr(), out.data_ptr(), n, r, M, N, K, work.data_ptr(), size,
+                    out_mode=mode)
+    ctx.synchronize()
+    return out
+
+
+FORMS = [1, 32, 33, 200, 2500, 9000]  # rows: CUDA cores, then tiles of 128 rows and of 256
+
+
+@pytest.mark.parametrize("mode", [0, 1])
+@pytest.mark.parametrize("M", FORMS)
+@pytest.mark.parametrize("rank", [8, 24])
+def test_an_addition_that_cancels(ctx, M, rank, mode):
+    """low = (257, 256, 0, ...) against up = (c, -c, 0, ...): c, where 257 in bf16 would give 0 or 2 c.  The values are exact in bf16."""
+    K, N = 16, 1024
+    a = torch.ones(M, K, device="cuda").bfloat16()
+    down, up = torch.zeros(2, rank, K, device="cuda").bfloat16(), torch.zeros(2, N, rank, device="cuda").bfloat16()
+    down[:, 0, 0], down[:, 0, 1], down[:, 1, 0] = 256.0, 1.0, 256.0
+    c = (torch.arange(N, device="cuda") % 19 - 9).float()
+    up[:, :, 0], up[:, :, 1] = c.bfloat16(), -c.bfloat16()
+    who = (torch.arange(M, device="cuda") // 3 % 2).int()
+    out = adapters_alone(ctx, a, down, up, who, mode)
+    assert torch.equal(out.float(), c.expand(M, N))
+
+
+@pytest.mark.parametrize("rank", [8, 64, 128])
+def test_a_row_keeps_its_numbers_whatever_the_batch(ctx, rank):
+    """`low` enters with an error of 2^-16 of |low| |up| at most (two bf16 terms), is itself summed in 32 bits (K / 16 MMAs, 17 addends cut
+    off at 2^-23 each: below 2^-16 of |x| |down| |up|), and the result is rounded once: 2^-8.  So the same row differs by a rounding to
+    bf16 at most between a call of 32 rows and one of 33 or more."""
+    K, N, n = 64, 512, 4
+    g = torch.Generator(device="cuda").manual_seed(rank)
+    a = torch.randn(max(FORMS), K, device="cuda", generator=g).bfloat16()
+    down = (torch.randn(n, rank, K, device="cuda", generator=g) * K ** -0.5).bfloat16()
+    up = (torch.randn(n, N, rank, device="cuda", generator=g) * rank ** -0.5).bfloat16()
+    who = torch.randint(-1, n, (max(FORMS),), device="cuda", generator=g).int()
+    ref = torch.zeros(max(FORMS), N, device="cuda", dtype=torch.float64)
+    size = torch.zeros_like(ref)
+    for e in range(n):
+        here = who == e
+        low = a[here].double() @ down[e].double().T
+        ref[here] = low @ up[e].double().T
+        size[here] = (low.abs() + a[here].double().abs() @ down[e].double().abs().T) @ up[e].double().abs().T
+    bound = 2.0 ** -16 * size + (1.0 + 2.0 ** -7) * 2.0 ** -8 * ref.abs()
+    few = None
+    for M in FORMS:
+        out = adapters_alone(ctx, a[:M], down, up, who[:M].contiguous(), 0).double()
+        far = (out - ref[:M]).abs()
+        assert bool((far <= bound[:M]).all()), (M, float((far - bound[:M]).max()))
+        if M == 32:
+            few = out
+        elif few is not None:
+            assert bool(((out[:32] - few).abs() <= 2.0 ** -15 * size[:32] + (1.0 + 2.0 ** -7) * 2.0 ** -7 * few.abs()).all()), M

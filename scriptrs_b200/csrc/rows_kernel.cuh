@@ -23,8 +23,10 @@
 //     `low` is there, and the epilogue adds it (24 rows with as many adapters, rank 16, 1024 -> 4096: 14.8 -> 10.1 us,
 //     and 6.5 us with A stages of 32 rows).
 //   - The tensor core adds into its accumulator by truncation, 1e-6 of the result at K = 1024 and 4.4e-6 at 4096 (measured).
-//     Where the result is stored in 32 bits, it is collected in registers every kSegment stages, rounded to nearest (4.7e-7 at
-//     either K; every four stages: 2.5e-7, but 16384 x 1024 x 1024 then takes 48 us instead of 36, a handshake per segment).
+//     Where the result is stored in 32 bits, it is collected in registers every 512 columns of K, rounded to nearest (4.7e-7 at
+//     either K in bf16; every 256 columns: 2.5e-7, but 16384 x 1024 x 1024 then takes 48 us instead of 36, a handshake per segment.  e4m3:
+//     13160 x 4096 x 1024 takes 95 us, 84 if collected every 1024 columns, where a product of a large value and small ones loses 2.7e-5
+//     instead of 1.3e-5).
 // Every wait on an mbarrier is bounded; when one runs out the kernel sets *error, drains, frees its tensor memory and returns.
 #pragma once
 #include <cuda.h>
@@ -49,7 +51,7 @@ using namespace ptx;
 constexpr int kBM = 128;
 constexpr int kRowBytes = 128;  // of an operand row in a stage: one swizzle row
 constexpr int kFewRows = 32, kFewPitch = kFewRows + 1;  // rows of the few-row forms; an odd pitch spreads both sides over the banks
-constexpr int kSegment = 8;     // stages (64 bf16 or 128 e4m3 columns of K each) between two collections of a 32-bit result
+constexpr int kSegmentCols = 512;  // columns of K between two collections of a 32-bit result
 
 enum RowsMode : int { kGrouped = 0, kGathered = 1, kAdapters = 2, kFewAdapters = 3, kFewGathered = 4 };
 constexpr bool rows_few(int mode) { return mode == kFewAdapters || mode == kFewGathered; }
@@ -398,7 +400,7 @@ rows_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ C
             int* __restrict__ error) {
     using C = RCfg<BN, CTAS, FP8, MODE, F32>;
     constexpr int S = C::kStages;
-    constexpr int kStepCols = FP8 ? 128 : 64;
+    constexpr int kStepCols = FP8 ? 128 : 64, kSegment = kSegmentCols / kStepCols;
     constexpr int kTerms = C::kTerms, kGroups = C::kGroups, kPhaseCols = 16 * kGroups;
     constexpr int kEpiWarps = C::kEpiWarps, kAuxWarps = C::kAuxWarps;
     // rank of this CTA in its pair (the leader, rank 0, owns the barriers that the MMAs wait on)

@@ -550,7 +550,7 @@ int32_t sb_gemm(sb_ctx* ctx, const void* d_a, const void* d_w, const float* d_bi
  * device memory are not read by the host.  Pointers are device pointers of the context's GPU.  Zero rows are a call
  * without effect (sb_route_topk still writes its offsets). */
 
-/* Scratch bytes of sb_route_topk and sb_adapter_gemm; 0 for sizes that those refuse. */
+/* Scratch bytes of sb_route_topk and sb_adapter_gemm; 0 for no rows and for sizes (of those given) that they refuse. */
 int64_t sb_route_topk_workspace(int64_t rows, int64_t n_experts, int64_t top_k);
 int64_t sb_adapter_gemm_workspace(int64_t M, int64_t rank);
 

@@ -17,6 +17,11 @@ bool off_boundary(const void* p, int bytes) { return (reinterpret_cast<uintptr_t
 constexpr int64_t kLimit = INT32_MAX;
 constexpr int64_t kMaxRank = 128, kMaxRouteExperts = 1024, kMaxRouteTopK = 16;
 
+bool route_sizes(int64_t rows, int64_t n_experts, int64_t top_k) {
+    return rows >= 0 && n_experts > 0 && n_experts <= kMaxRouteExperts && top_k > 0 && top_k <= kMaxRouteTopK && top_k <= n_experts && rows <= kLimit / top_k;
+}
+bool adapter_rank(int64_t rank) { return rank > 0 && rank <= kMaxRank && rank % 8 == 0; }
+
 // What the product entry points share.  (The context is looked at last, so that the arguments' checks need no GPU.)
 int32_t check_product(const void* d_a, int64_t lda, const void* d_w, const float* d_bias, const void* d_out, int64_t ldo,
                       int64_t M, int64_t N, int64_t K, int64_t groups, bool fp8, int32_t act, int32_t out_mode) {
@@ -40,21 +45,19 @@ int32_t check_product(const void* d_a, int64_t lda, const void* d_w, const float
 extern "C" {
 
 int64_t sb_route_topk_workspace(int64_t rows, int64_t n_experts, int64_t top_k) {
-    if (rows <= 0 || n_experts <= 0 || n_experts > kMaxRouteExperts || top_k <= 0 || rows > kLimit / top_k) return 0;
+    if (rows == 0 || !route_sizes(rows, n_experts, top_k)) return 0;
     return std::max<int64_t>(route_work_bytes(rows, n_experts, top_k), 16);
 }
 
 int64_t sb_adapter_gemm_workspace(int64_t M, int64_t rank) {
-    if (M <= 0 || M > kLimit - 512 || rank <= 0 || rank > kMaxRank) return 0;
+    if (M <= 0 || M > kLimit - 512 || !adapter_rank(rank)) return 0;
     return M * rank * 4;  // the rows' products with the adapters' first matrices, f32
 }
 
 int32_t sb_route_topk(sb_ctx* c, const void* d_logits, int32_t logits_bf16, int64_t ld, int64_t rows, int64_t n_experts, int64_t top_k,
                       int32_t normalize, int32_t* d_experts, float* d_weights, int32_t* d_offsets, int32_t* d_order, int32_t* d_slots,
                       void* d_work, int64_t work_bytes) {
-    if (rows < 0 || n_experts <= 0 || n_experts > kMaxRouteExperts || top_k <= 0 || top_k > kMaxRouteTopK || top_k > n_experts ||
-        rows > kLimit / top_k || ld < n_experts)
-        return fail(SB_INVALID_ARGUMENT, "bad router shape");
+    if (!route_sizes(rows, n_experts, top_k) || ld < n_experts) return fail(SB_INVALID_ARGUMENT, "bad router shape");
     if (!d_offsets || off_boundary(d_offsets, 4)) return fail(SB_INVALID_ARGUMENT, "the offsets are null or misaligned");
     if (rows > 0) {
         if (!d_logits || !d_experts || !d_weights || !d_order || !d_slots) return fail(SB_INVALID_ARGUMENT, "null argument");
@@ -132,7 +135,7 @@ int32_t sb_adapter_gemm(sb_ctx* c, const void* d_a, int64_t lda, const void* d_w
                         int64_t M, int64_t N, int64_t K, int32_t act, int32_t out_mode, float alpha, void* d_work, int64_t work_bytes) {
     int32_t st = check_product(d_a, lda, d_w, d_bias, d_out, ldo, M, N, K, 1, false, act, out_mode);
     if (st != SB_OK) return st;
-    if (n_adapters <= 0 || n_adapters > kLimit / std::max(N, kMaxRank) || rank <= 0 || rank > kMaxRank || rank % 8)
+    if (n_adapters <= 0 || n_adapters > kLimit / std::max(N, kMaxRank) || !adapter_rank(rank))
         return fail(SB_INVALID_ARGUMENT, "adapters: at least one, rank a multiple of 8 up to 128");
     if (M > 0 && (!d_down || !d_up || !d_row_adapter)) return fail(SB_INVALID_ARGUMENT, "null argument");
     if (off_boundary(d_down, 16) || off_boundary(d_up, 16) || off_boundary(d_work, 16) || off_boundary(d_scale, 4) || off_boundary(d_row_adapter, 4))

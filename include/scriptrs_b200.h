@@ -578,7 +578,8 @@ int32_t sb_route_topk(sb_ctx* ctx, const void* d_logits, int32_t logits_bf16, in
  *   d_offsets  [n_groups + 1] int32 in device memory, ascending, at most M: groups may be empty, of any size, and need not
  *              cover all M rows
  *   d_out      [M x N], row pitch ldo elements; rows outside the groups are left as they are
- * Any M, N and n_groups; K a multiple of 8 (bf16) or 16 (fp8).  d_a and d_w on 16-byte boundaries, lda * element size a
+ * M and n_groups up to 2^31 - 513, N and K below 2^30, n_groups * N < 2^31, (M / 128 + 1) * (N / 32 + 1) <= 2^25 (integer quotients);
+ * K a multiple of 8 (bf16) or 16 (fp8).  d_a and d_w on 16-byte boundaries, lda * element size a
  * multiple of 16.  bf16 results are rounded once from the 32-bit sum; a row's numbers depend neither on its place nor on the
  * other rows. */
 int32_t sb_grouped_gemm(sb_ctx* ctx, const void* d_a, int64_t lda, int64_t a_rows, const int32_t* d_rows, const void* d_w,
@@ -607,7 +608,7 @@ int32_t sb_combine_rows(sb_ctx* ctx, const void* d_y, int32_t y_f32, int64_t ldy
  *   d_work     sb_adapter_gemm_workspace(M, rank) bytes on a 16-byte boundary
  * Sums are held in 32 bits.  A[i] * down[a]^T enters with an error of at most 2^-16 for bf16 results, 2^-24 for f32 results (none in calls
  * of up to 32 rows), so a row's numbers differ between calls by no more than the result's rounding.
- * Any M, N and n_adapters (n_adapters * N < 2^31); K and rank multiples of 8, rank <= 128; alignment as for sb_grouped_gemm.
+ * M, N and K as for sb_grouped_gemm, n_adapters * max(N, 128) < 2^31; K and rank multiples of 8, rank <= 128; alignment as there.
  * Nothing of one adapter, inf and NaN included, reaches rows of another. */
 int32_t sb_adapter_gemm(sb_ctx* ctx, const void* d_a, int64_t lda, const void* d_w, const float* d_bias, const void* d_down,
                         const void* d_up, const float* d_scale, const int32_t* d_row_adapter, int64_t n_adapters,

@@ -25,7 +25,7 @@ bool adapter_rank(int64_t rank) { return rank > 0 && rank <= kMaxRank && rank % 
 // What the product entry points share.  (The context is looked at last, so that the arguments' checks need no GPU.)
 int32_t check_product(const void* d_a, int64_t lda, const void* d_w, const float* d_bias, const void* d_out, int64_t ldo,
                       int64_t M, int64_t N, int64_t K, int64_t groups, bool fp8, int32_t act, int32_t out_mode) {
-    if (M < 0 || N <= 0 || K <= 0 || groups <= 0 || M > kLimit - 512 || N > kLimit / 2 || K > kLimit / 2 || groups > kLimit || groups > kLimit / N)
+    if (M < 0 || N <= 0 || K <= 0 || groups <= 0 || M > kLimit - 512 || N > kLimit / 2 || K > kLimit / 2 || groups > kLimit - 512 || groups > kLimit / N)
         return fail(SB_INVALID_ARGUMENT, "bad product shape");
     // tiles of 128 rows x 32 columns are counted in 32 bits
     if ((M / 128 + 1) * (N / 32 + 1) > (int64_t)1 << 25) return fail(SB_INVALID_ARGUMENT, "the result is too large for one call");

@@ -24,3 +24,14 @@ def test_a_router_workspace_for_every_size_that_is_taken():
 def test_no_adapter_workspace_for_sizes_that_are_refused(M, rank):
     assert call("sb_adapter_gemm", ADAPTER, M=M, rank=rank, N=1, ldo=8) == 11 and message() != "ctx is null"
     assert lib().sb_adapter_gemm_workspace(M, rank) == 0
+
+
+@pytest.mark.parametrize("groups", [2 ** 31 - 1, 2 ** 31 - 127, 2 ** 31 - 512])
+def test_groups_whose_walk_would_pass_32_bits_are_refused(groups):
+    """The kernel steps through the groups 128 at a time in 32 bits: from 2^31 - 128 on the next step is negative, and an offset before the
+    first one would be read."""
+    assert call("sb_grouped_gemm", GROUPED, groups=groups, N=1, ldo=1) == 11 and message() == "bad product shape"
+
+
+def test_the_most_groups():
+    assert call("sb_grouped_gemm", GROUPED, groups=2 ** 31 - 513, N=1, ldo=1) == 11 and message() == "ctx is null"

@@ -548,7 +548,8 @@ int32_t sb_gemm(sb_ctx* ctx, const void* d_a, const void* d_w, const float* d_bi
  * All of them are asynchronous on the context's stream, allocate nothing and may be captured into a CUDA graph; scratch
  * memory is the caller's (d_work), and calls that may run at the same time need one each.  Sizes and offsets that live in
  * device memory are not read by the host.  Pointers are device pointers of the context's GPU.  Zero rows are a call
- * without effect (sb_route_topk still writes its offsets). */
+ * without effect (sb_route_topk still writes its offsets).  The first call on a context sets its kernels up, captured or not
+ * (some 15 ms on the host in a process's first context). */
 
 /* Scratch bytes of sb_route_topk and sb_adapter_gemm; 0 for no rows and for sizes (of those given) that they refuse. */
 int64_t sb_route_topk_workspace(int64_t rows, int64_t n_experts, int64_t top_k);

@@ -15,7 +15,6 @@
 #include "host/weights_file.h"
 #include "model.h"
 #include "pipeline.h"
-#include "rows.h"
 #include "vad.h"
 
 namespace sb {
@@ -261,9 +260,6 @@ int32_t sb_ctx_create(int32_t device, sb_ctx** out) {
     cudaError_t ge = gemm_configure(&why);
     if (ge != cudaSuccess)
         return bail(fail(SB_CUDA_ERROR, std::string("GEMM set-up failed: ") + (why ? why : cudaGetErrorString(ge))));
-    ge = rows_configure(&why);
-    if (ge != cudaSuccess)
-        return bail(fail(SB_CUDA_ERROR, std::string("row product set-up failed: ") + (why ? why : cudaGetErrorString(ge))));
     SB_CREATE_CUDA(encoder_configure());
 #undef SB_CREATE_CUDA
     c->enc_ws = new EncoderWorkspace();

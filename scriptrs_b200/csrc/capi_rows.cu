@@ -22,6 +22,22 @@ bool route_sizes(int64_t rows, int64_t n_experts, int64_t top_k) {
 }
 bool adapter_rank(int64_t rank) { return rank > 0 && rank <= kMaxRank && rank % 8 == 0; }
 
+// Sets up the kernels that an entry point may launch, in its first call on a context: loading them takes 12 ms in the first context of a
+// process, which one that only transcribes does not pay.  The call may be one that is captured: nothing here is work on a stream, so this
+// thread steps out of the capture's checks meanwhile.
+template <typename Fn>
+int32_t set_up(bool* ready, Fn configure) {
+    if (*ready) return SB_OK;
+    const char* why = nullptr;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    SB_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+    const cudaError_t e = configure(&why);
+    SB_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+    if (e != cudaSuccess) return fail(SB_CUDA_ERROR, std::string("row product set-up failed: ") + (why ? why : cudaGetErrorString(e)));
+    *ready = true;
+    return SB_OK;
+}
+
 // What the product entry points share.  (The context is looked at last, so that the arguments' checks need no GPU.)
 int32_t check_product(const void* d_a, int64_t lda, const void* d_w, const float* d_bias, const void* d_out, int64_t ldo,
                       int64_t M, int64_t N, int64_t K, int64_t groups, bool fp8, int32_t act, int32_t out_mode) {
@@ -69,6 +85,8 @@ int32_t sb_route_topk(sb_ctx* c, const void* d_logits, int32_t logits_bf16, int6
     }
     if (!c) return fail(SB_INVALID_ARGUMENT, "ctx is null");
     SB_CUDA(cudaSetDevice(c->device));
+    const int32_t st = set_up(&c->route_ready, [](const char**) { return route_configure(); });
+    if (st != SB_OK) return st;
     RouteArgs g{};
     g.logits = d_logits; g.ld = ld; g.rows = (int)rows; g.n_experts = (int)n_experts; g.top_k = (int)top_k;
     g.bf16 = logits_bf16 != 0; g.normalize = normalize != 0;
@@ -94,6 +112,8 @@ int32_t sb_grouped_gemm(sb_ctx* c, const void* d_a, int64_t lda, int64_t a_rows,
     if (!c) return fail(SB_INVALID_ARGUMENT, "ctx is null");
     if (M == 0) return SB_OK;
     SB_CUDA(cudaSetDevice(c->device));
+    st = set_up(&c->rows_ready, rows_configure);
+    if (st != SB_OK) return st;
     RowsArgs g{};
     g.a = d_a; g.rows = d_rows; g.w = d_w; g.bias = d_bias; g.row_scale = d_row_scale; g.col_scale = d_col_scale; g.offsets = d_offsets;
     g.out = d_out; g.a_rows = a_rows; g.lda = lda; g.ldo = ldo; g.M = (int)M; g.N = (int)N; g.K = (int)K; g.n_groups = (int)n_groups;
@@ -145,6 +165,8 @@ int32_t sb_adapter_gemm(sb_ctx* c, const void* d_a, int64_t lda, const void* d_w
     if (!c) return fail(SB_INVALID_ARGUMENT, "ctx is null");
     if (M == 0) return SB_OK;
     SB_CUDA(cudaSetDevice(c->device));
+    st = set_up(&c->rows_ready, rows_configure);
+    if (st != SB_OK) return st;
     float* low = static_cast<float*>(d_work);
     RowsArgs g{};
     g.a = d_a; g.w = d_w; g.bias = d_bias; g.out = d_out; g.a_rows = M; g.lda = lda; g.ldo = ldo; g.M = (int)M; g.N = (int)N; g.K = (int)K;

@@ -50,7 +50,7 @@ cudaError_t rows_configure(const char** why) {
         }
         g_rows_encode = reinterpret_cast<EncodeTiledFn>(fn);
     }
-    for (cudaError_t (*set)() : {rows_grouped_configure, rows_gathered_configure, rows_adapters_configure, rows_few_configure, adapter_down_configure, route_configure}) {
+    for (cudaError_t (*set)() : {rows_grouped_configure, rows_gathered_configure, rows_adapters_configure, rows_few_configure, adapter_down_configure}) {
         const cudaError_t e = set();
         if (e != cudaSuccess) {
             if (why) *why = "shared-memory opt-in for the row products failed";

@@ -610,7 +610,7 @@ int32_t sb_combine_rows(sb_ctx* ctx, const void* d_y, int32_t y_f32, int64_t ldy
  * Sums are held in 32 bits.  A[i] * down[a]^T enters with an error of at most 2^-16 for bf16 results, 2^-24 for f32 results (none in calls
  * of up to 32 rows), so a row's numbers differ between calls by no more than the result's rounding.
  * M, N and K as for sb_grouped_gemm, n_adapters * max(N, 128) < 2^31; K and rank multiples of 8, rank <= 128; alignment as there.
- * Nothing of one adapter, inf and NaN included, reaches rows of another. */
+ * Nothing of one adapter, inf and NaN included, reaches rows of another; its own rows get NaN where `up` holds inf. */
 int32_t sb_adapter_gemm(sb_ctx* ctx, const void* d_a, int64_t lda, const void* d_w, const float* d_bias, const void* d_down,
                         const void* d_up, const float* d_scale, const int32_t* d_row_adapter, int64_t n_adapters,
                         int64_t rank, void* d_out, int64_t ldo, int64_t M, int64_t N, int64_t K, int32_t act,

@@ -3,7 +3,7 @@
 //   adapters:  out[i] = alpha act(W x[i] + U_a low[i] + b)           with the adapter a of row i, low = scale_a D_a x[i]
 //
 // One CTA per SM, warp-specialised like the shared product of gemm.cu: a TMA producer, an MMA issuer (128 rows x BN columns per
-// CTA in tensor memory, two accumulators), eight epilogue warps.  What differs:
+// CTA in tensor memory, two accumulators), eight epilogue warps (sixteen for pairs in e4m3).  What differs:
 //   - The tiles are found on the device.  A tile belongs to one group: 128 consecutive rows of it per CTA (the last ones of a
 //     group may be missing) times BN columns.  Every warp walks the offsets 128 groups at a time with a prefix sum over its
 //     lanes, so no table of groups is kept and the host never learns the sizes.
@@ -21,7 +21,7 @@
 //   - Up to 32 rows (live streams, as a rule each with an adapter of its own): an MMA per adapter would take longer than all of
 //     K, so the addition is formed on CUDA cores by the four warps that stage `low` otherwise, in 32 bits, U_a on its way before
 //     `low` is there, and the epilogue adds it (24 rows with as many adapters, rank 16, 1024 -> 4096: 14.8 -> 10.1 us,
-//     and 6.5 us with A stages of 32 rows).
+//     and 7.1 us with A stages of 32 rows; 33 rows, by MMAs, 13.8 us).
 //   - The tensor core adds into its accumulator by truncation, 1e-6 of the result at K = 1024 and 4.4e-6 at 4096 (measured).
 //     Where the result is stored in 32 bits, it is collected in registers every 512 columns of K, rounded to nearest (4.7e-7 at
 //     either K in bf16; every 256 columns: 2.5e-7, but 16384 x 1024 x 1024 then takes 48 us instead of 36, a handshake per segment.  e4m3:
@@ -58,8 +58,8 @@ constexpr bool rows_few(int mode) { return mode == kFewAdapters || mode == kFewG
 constexpr bool rows_gathers(int mode) { return mode == kGathered || mode == kFewGathered; }
 
 // Parts of a tile's columns, four epilogue warps (128 rows) each.  A pair's e4m3 tile is over in half the time, so its epilogue sets the
-// pace: sixteen warps instead of eight (16384 x 4096 x 1024: 71 -> 67 us, gathered 88 -> 76, 16 groups 97 -> 87; their slabs take a
-// stage, which costs 26000 x 1024 x 4096 3 %).  bf16 gains nothing by them.
+// pace: sixteen warps instead of eight (16384 x 4096 x 1024: 75 -> 71 us, gathered 84 -> 76, 16 groups 87 -> 84; their slabs take a
+// stage, which costs 26000 x 1024 x 4096 1 %).  bf16 gains nothing by them.
 constexpr int rows_parts(int bn, int ctas, bool fp8, bool f32) { return bn == 256 && ctas == 2 && fp8 && !f32 ? 4 : gemm_halves(bn); }
 
 // CTAS = 2: a cluster of two CTAs on 256 rows x BN columns (tcgen05 cta_group::2); each stages its own 128 rows of A and its own
@@ -72,12 +72,12 @@ struct RCfg {
     static constexpr int kSlabBytes = 32 * 128;
     // Warps more where rows are picked (gathers) or have adapters (`low`): four, 32 rows each; two beside an epilogue that keeps 128
     // sums a thread in registers (168 registers for 12 warps, 144 for 14); eight for the gathers of bf16 results, which four warps only
-    // just issue in a stage's time (16384 x 4096 x 1024: 110 -> 106 us, 8064 rows of 16 groups 77 -> 71), where registers allow.
+    // just issue in a stage's time (16384 x 4096 x 1024: 111 -> 106 us, 8064 rows of 16 groups 73 -> 71), where registers allow.
     static constexpr int kAuxWarps = MODE == kGrouped ? 0 : (F32 && BN == 256 ? 2 : (MODE == kGathered && kEpiWarps == 8 && !F32 ? 8 : 4));
     static constexpr int kThreads = 32 * (2 + kEpiWarps + kAuxWarps);
     // The few-row forms stage 32 rows of A.  The MMA reads 128: the others are whatever lies behind, and so are their lanes of the
     // accumulator, which nobody reads.  What that saves goes into stages: narrow tiles are paced by the weights in flight
-    // (24 rows, 1024 -> 4096, no adapters, the adapters' kernel included: 9.6 -> 6.5 us).
+    // (24 rows with adapters, 1024 -> 4096: 10.1 -> 7.1 us, both kernels).
     static constexpr int kABytes = (rows_few(MODE) ? kFewRows : kBM) * kRowBytes;
     static constexpr int kBBytes = BN / CTAS * kRowBytes;
     static constexpr int kStageBytes = kABytes + kBBytes;

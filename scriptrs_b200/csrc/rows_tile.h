@@ -16,14 +16,16 @@ struct RowsTileShape {
 // device; the rows are taken as spread evenly over the groups, half a tile of each lost.  A result in 32 bits keeps its sums in
 // registers: 128 columns, or a pair where no warps gather rows (`picked`).  The end of a pair's last tile, 128 columns a thread, is
 // not hidden: a third of a wave more.  us, 128 columns / pairs, 32-bit results; rows (groups) x N x K:
-//   2503 (8) x 1030 x 640    10.7 / 17.2     4000 (1) x 1024 x 1024   11.9 / 13.3     1504 (1) x 4096 x 1024    16.1 / 17.6
-//   13160 (1) x 1024 x 1024  31.2 / 26.8     13160 (1) x 1024 x 4096  105 / 88        13160 (1) x 4096 x 1024   117 / 101
-//   8064 (16) x 1024 x 1024  23.7 / 32.2     13160 (16) x 1024 x 1024  46 / 42        52360 (32) x 1024 x 4096  460 / 408
-// Measured, us, at 32 / 64 / 128 / 256 columns / pairs, bf16 results; rows (groups) x N x K:
-//   128 (1) x 4096 x 1024    5.7 / 6.3 / 6.9 / 9.9 / 11.0       376 (1) x 4096 x 1024    11.1 / 9.5 / 7.6 / 10.7 / 11.6
-//   1504 (1) x 4096 x 1024   32 / 21 / 15.3 / 17.1 / 17.1       13160 (1) x 4096 x 1024  228 / 130 / 99 / 89 / 79
-//   8064 (16) x 4096 x 1024  165 / 101 / 79 / 71 / 67           8064 (16) x 1024 x 1024  48 / 29 / 21.5 / 19.8 / 23.6
-//   2000 (32) x 4096 x 1024  121 / 68 / 53 / 53 / 59            64 (32) x 4096 x 1024    118 / 64 / 48 / 50 / 53
+//   2503 (8) x 1030 x 640    12.7 / 14.1     4000 (1) x 1024 x 1024   12.2 / 12.8     1504 (1) x 4096 x 1024    16.8 / 18.4
+//   13160 (1) x 1024 x 1024  31.7 / 27.6     13160 (1) x 1024 x 4096   99 / 84        13160 (1) x 4096 x 1024   115 / 100
+//   8064 (16) x 1024 x 1024  23.7 / 28.0     13160 (16) x 1024 x 1024  36.4 / 39.1    52360 (32) x 1024 x 4096  406 / 350
+// Measured, us, at 32 / 64 / 128 / 256 columns / pairs, bf16 results with SiLU; rows (groups) x N x K:
+//   128 (1) x 4096 x 1024    8.4 / 9.7 / 11.0 / 16.5 / 18.0     376 (1) x 4096 x 1024    17.0 / 15.0 / 12.1 / 17.3 / 18.3
+//   1504 (1) x 4096 x 1024   48 / 31 / 22.5 / 26.4 / 26.2       13160 (1) x 4096 x 1024  354 / 162 / 109 / 101 / 91
+//   8064 (16) x 4096 x 1024  179 / 102 / 75 / 69 / 69           8064 (16) x 1024 x 1024  47 / 30 / 22.3 / 21.0 / 25.3
+//   2000 (32) x 4096 x 1024  113 / 65 / 53 / 53 / 61            64 (32) x 4096 x 1024    87 / 52 / 47 / 50 / 57
+// e4m3, whose steps of K take half the time, by the same costs: 13160 (16) x 4096 x 1024 gathered 211 / 137 / 88 / 76 / 79, 13160 (1)
+// 142 / 97 / 64 / 57 / 62: 5 to 8 % off the best.
 inline RowsTileShape rows_tile(int64_t M, int N, int n_groups, bool f32, bool picked, int sm_count) {
     const int64_t groups = std::min<int64_t>(n_groups, M);
     RowsTileShape best{128, 1};

@@ -221,8 +221,9 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
         : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// x * sigmoid(x) and v * sigmoid(g) through one hardware tanh: sigmoid(t) = 0.5 tanh(0.5 t) + 0.5 (relative error of
-// tanh.approx about 2^-11, below the bf16 rounding of the results these feed)
+// x * sigmoid(x) and v * sigmoid(g) through one hardware tanh: sigmoid(t) = 0.5 tanh(0.5 t) + 0.5.  tanh.approx has a relative error of
+// about 2^-11, so the sigmoid has an absolute one of 2^-12: below the bf16 rounding of the results these feed where the argument is
+// positive; where it is negative the sum cancels (1 % of the result at -4), small beside the other values of a row.
 __device__ __forceinline__ float tanh_approx(float x) {
     float y;
     asm("tanh.approx.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -138,3 +138,36 @@ def test_contexts_of_two_threads_at_once(ctx):
     for b in both:
         for x, y in zip(one[:8], b[:8]):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("mode", [0, 1, 2])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_a_row_has_the_same_bits_in_every_form(ctx, fp8, mode):
+    """Few rows and many, in place and through an index, alone and beside other groups."""
+    import scriptrs_b200 as sb
+
+    N, K, G, rows = 1030, 1040, 3, 9000
+    g = gen(7)
+    a, w = randn(g, rows, K), randn(g, G, N, K, std=K ** -0.5)
+    rs = torch.rand(rows, device="cuda", generator=g) + 0.5 if fp8 else None
+    cs = torch.rand(G, N, device="cuda", generator=g) + 0.5 if fp8 else None
+    a, w = (t.to(torch.float8_e4m3fn if fp8 else torch.bfloat16) for t in (a, w))
+    bias = randn(g, G, N)
+
+    def run(sizes, idx=None):
+        M = sum(sizes)
+        out, off = torch.zeros(M, N, device="cuda", dtype=torch.float32 if mode else torch.bfloat16), offsets_of(sizes)
+        torch.cuda.synchronize()
+        sb.grouped_gemm(ctx, a.data_ptr(), w.data_ptr(), out.data_ptr(), off.data_ptr(), G, M, N, K, d_rows=idx.data_ptr() if idx is not None else 0,
+                        a_rows=rows, d_bias=bias.data_ptr(), act=SILU, out_mode=mode, fp8=fp8, d_row_scale=rs.data_ptr() if fp8 else 0,
+                        d_col_scale=cs.data_ptr() if fp8 else 0)
+        ctx.synchronize()
+        return out
+
+    whole = run([0, rows, 0])
+    idx = torch.randperm(rows, device="cuda", generator=g).int()
+    for n in (1, 20, 32, 33, 130, 700, 3000):
+        assert torch.equal(run([0, n, 0]), whole[:n]), n
+        assert torch.equal(run([0, n, 0], idx), whole[idx[:n].long()]), n
+    assert torch.equal(run([3, 25, 4], idx)[3:28], whole[idx[3:28].long()])
+    assert torch.equal(run([300, 2500, 4000], idx)[300:2800], whole[idx[300:2800].long()])
